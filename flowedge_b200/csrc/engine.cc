@@ -369,6 +369,11 @@ int check_tokens(const fe_engine* e, const std::int32_t* tokens, std::size_t n) 
 
 }  // namespace
 
+namespace feb {
+void set_last_error(std::string message) { set_error(std::move(message)); }
+void clear_last_error() noexcept { clear_error(); }
+}  // namespace feb
+
 extern "C" {
 
 const char* fe_engine_last_error(void) { return last_error(); }

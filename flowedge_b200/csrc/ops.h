@@ -1,0 +1,44 @@
+// Operators on device buffers (include/flowedge_b200.h, part 3): the launch
+// functions behind the C entry points of ops.cc.  No CUDA types appear here;
+// `stream` is a cudaStream_t.  The entry points have checked every size,
+// pointer and stride before a launch function runs, and have made the buffers'
+// device current.  Each returns 0 or a CUDA error code of the launch.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <string>
+
+#include "../../include/flowedge_b200.h"
+
+namespace feb {
+
+int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept;
+
+std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept;
+int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept;
+
+// Last error of this thread (fe_engine_last_error); defined with the engine.
+void set_last_error(std::string message);
+void clear_last_error() noexcept;
+
+// Multiprocessors of the current device (looked up once per device).
+int current_sm_count() noexcept;
+
+// Makes `device` current for a scope (-1: leaves the current one).
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) noexcept;
+  ~DeviceScope();
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  [[nodiscard]] bool ok() const noexcept { return ok_; }
+
+ private:
+  int before_ = -1;
+  bool ok_ = true;
+};
+
+const char* cuda_error_text(int code) noexcept;
+
+}  // namespace feb

@@ -151,6 +151,10 @@ SIGNATURES = {
     "fe_device_malloc_count": (C.c_uint64, []),
     "fe_host_malloc_count": (C.c_uint64, []),
     "fe_engine_kernel_launches": (C.c_uint64, [C.c_void_p]),
+    # operators on device buffers (flowedge_b200.ops): packed argument structures
+    "fe_causal_conv_device": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "fe_selective_scan_device": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "fe_selective_scan_workspace": (C.c_size_t, [C.c_char_p]),
 }
 
 _lib = None

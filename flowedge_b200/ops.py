@@ -1,0 +1,185 @@
+"""Operators on CUDA tensors over the C ABI (include/flowedge_b200.h, part 3).
+
+The Mamba mixer's operators for many sequences whose states live in slots:
+ragged prompts (`offsets`) or one token per row, each sequence with a slot of
+a pool (`slots`; negative skips it) and, where `fresh` says so, a zero start.
+
+Each call checks its arguments, enqueues its kernels on the current stream of
+its tensors' device and returns; it keeps nothing.  A refused argument raises
+FlowEdgeError (status 1) before anything is launched.  These are inference
+operators: tensors that require a gradient are refused while gradients are
+being recorded.  Outputs share no element with inputs; states are updated in
+place.  With `out` given, rows of skipped sequences and rows behind the last
+sequence keep what they held; without it they are undefined.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
+
+from .engine import FlowEdgeError, load_library
+
+__all__ = ["conv", "scan", "BAD_OFFSETS", "BAD_SLOT", "DUPLICATE_SLOT"]
+
+# bits that `status` collects
+BAD_OFFSETS, BAD_SLOT, DUPLICATE_SLOT = 1, 2, 4
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CONV = struct.Struct("@IiII4Q3q9P")
+_SCAN = struct.Struct("@IiII5Q5q14PQ")
+
+
+def _refuse(message: str):
+    raise FlowEdgeError(1, message)
+
+
+def _check(rc: int):
+    if rc != 0:
+        raise FlowEdgeError(rc, load_library().fe_engine_last_error().decode())
+
+
+def _tensor(t, name: str, dtype, device):
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name} is a tensor")
+    if t.dtype != dtype:
+        _refuse(f"{name} is {dtype}, not {t.dtype}")
+    if t.device != device:
+        _refuse(f"{name} is on {t.device}, not {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name} requires a gradient: this operator has none")
+
+
+def _matrix(t, name: str, rows: int, width: int, dtype, device) -> int:
+    """Checks a matrix with contiguous rows and returns the distance of its rows."""
+    _tensor(t, name, dtype, device)
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        _refuse(f"{name} has shape {tuple(t.shape)}, not {(rows, width)}")
+    ld, inner = t.stride()
+    if inner != 1 and width > 1:
+        _refuse(f"{name} has rows that are not contiguous")
+    return ld if rows > 1 else max(ld, width)
+
+
+def _flat(t, name: str, shape: tuple, dtype, device):
+    """Checks a contiguous tensor of the given shape."""
+    _tensor(t, name, dtype, device)
+    if t.shape != shape or not t.is_contiguous():
+        _refuse(f"{name} is a contiguous tensor of shape {tuple(shape)}, not {tuple(t.shape)}")
+
+
+def _first(x, name: str):
+    """Checks the matrix that the other arguments go by."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _DTYPES:
+        _refuse(f"{name} is a matrix of float32, bfloat16 or float16")
+    if not x.is_cuda:
+        _refuse(f"{name} is on {x.device}, not on a GPU")
+    return x.shape[0], x.shape[1], x.dtype, x.device
+
+
+def _sequences(rows: int, offsets, slots, fresh, status, device) -> int:
+    """Checks the sequences' description and returns their number."""
+    n_seq = rows
+    if offsets is not None:
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1:
+            _refuse("offsets is a tensor of n_seq + 1 elements")
+        n_seq = offsets.shape[0] - 1
+        _flat(offsets, "offsets", (n_seq + 1,), torch.int32, device)
+    if slots is not None:
+        _flat(slots, "slots", (n_seq,), torch.int32, device)
+    if fresh is not None:
+        _tensor(fresh, "fresh", torch.bool if getattr(fresh, "dtype", None) == torch.bool else torch.uint8, device)
+        if fresh.shape != (n_seq,) or not fresh.is_contiguous():
+            _refuse(f"fresh is a contiguous tensor of shape {(n_seq,)}, not {tuple(fresh.shape)}")
+    if status is not None:
+        _flat(status, "status", (1,), torch.int32, device)
+    return n_seq
+
+
+def _pool(state, name: str, inner: tuple, device) -> tuple:
+    """Checks a pool of slot states and returns (slots, distance of two slots)."""
+    _tensor(state, name, torch.float32, device)
+    if state.dim() != 3 or state.shape[1:] != inner:
+        _refuse(f"{name} has shape {tuple(state.shape)}, not {('slots',) + inner}")
+    per = inner[0] * inner[1]
+    outer, mid, last = state.stride()
+    if (mid != inner[1] and inner[0] > 1) or (last != 1 and inner[1] > 1):
+        _refuse(f"{name} has slots that are not contiguous")
+    return state.shape[0], outer if state.shape[0] > 1 else max(outer, per)
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _out(out, like_rows: int, width: int, dtype, device) -> tuple:
+    if out is None:
+        return torch.empty((like_rows, width), dtype=dtype, device=device), width
+    return out, _matrix(out, "out", like_rows, width, dtype, device)
+
+
+def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, status=None, out=None):
+    """SiLU(short causal depthwise convolution): u[t, c] = SiLU(bias[c] + sum_k weight[c, k] x[t - (d_conv - 1) + k, c]).
+
+    x [rows, d_inner] float32 / bfloat16 / float16 (rows may be apart); weight [d_inner, d_conv] and bias [d_inner]
+    float32, d_conv 1 to 8.  `window` [slots, d_inner, d_conv] float32 holds each slot's last inputs, newest last; a
+    sequence reads the inputs before its first row there and leaves its own last ones.  Returns u like x.
+    """
+    rows, di, dtype, device = _first(x, "x")
+    x_ld = _matrix(x, "x", rows, di, dtype, device)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        _refuse("weight is a tensor of shape (d_inner, d_conv)")
+    dc = weight.shape[1]
+    _flat(weight, "weight", (di, dc), torch.float32, device)
+    _flat(bias, "bias", (di,), torch.float32, device)
+    n_seq = _sequences(rows, offsets, slots, fresh, status, device)
+    n_slots, stride = (0, 0) if window is None else _pool(window, "window", (di, dc), device)
+    u, u_ld = _out(out, rows, di, dtype, device)
+    args = _CONV.pack(_CONV.size, device.index, _DTYPES[dtype], dc, rows, di, n_seq, n_slots, x_ld, u_ld, stride,
+                      x.data_ptr(), weight.data_ptr(), bias.data_ptr(), u.data_ptr(), _ptr(window), _ptr(offsets),
+                      _ptr(slots), _ptr(fresh), _ptr(status))
+    _check(load_library().fe_causal_conv_device(args, _raw_stream(device.index)))
+    return u
+
+
+def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=None, fresh=None, status=None,
+         out=None):
+    """The selective scan with its step projection and gate.
+
+    A row of proj is [dt_in (dt_rank) | B (d_state) | C (d_state)].  Per row and channel: dt = softplus(dt_in dt_w +
+    dt_b), h = exp(dt a) h + dt B u, y = (d u + sum h C) SiLU(z); without z there is no gate.  u, z [rows, d_inner]
+    and proj are float32, bfloat16 or float16 alike (rows may be apart); a [d_state, d_inner] (negative), d [d_inner],
+    dt_w [dt_rank, d_inner] and dt_b [d_inner] float32, d_state 1 to 32, dt_rank 1 to 512.  `state` [slots, d_state,
+    d_inner] float32.  Returns y like u.
+    """
+    rows, di, dtype, device = _first(u, "u")
+    u_ld = _matrix(u, "u", rows, di, dtype, device)
+    if not isinstance(a, torch.Tensor) or a.dim() != 2 or not isinstance(dt_w, torch.Tensor) or dt_w.dim() != 2:
+        _refuse("a is a tensor of shape (d_state, d_inner) and dt_w one of shape (dt_rank, d_inner)")
+    ds, dr = a.shape[0], dt_w.shape[0]
+    proj_ld = _matrix(proj, "proj", rows, dr + 2 * ds, dtype, device)
+    z_ld = 0 if z is None else _matrix(z, "z", rows, di, dtype, device)
+    _flat(a, "a", (ds, di), torch.float32, device)
+    _flat(d, "d", (di,), torch.float32, device)
+    _flat(dt_w, "dt_w", (dr, di), torch.float32, device)
+    _flat(dt_b, "dt_b", (di,), torch.float32, device)
+    n_seq = _sequences(rows, offsets, slots, fresh, status, device)
+    n_slots, stride = (0, 0) if state is None else _pool(state, "state", (ds, di), device)
+    y, y_ld = _out(out, rows, di, dtype, device)
+    lib = load_library()
+
+    def pack(workspace, size):
+        return _SCAN.pack(_SCAN.size, device.index, _DTYPES[dtype], ds, rows, di, dr, n_seq, n_slots, u_ld, proj_ld,
+                          z_ld, y_ld, stride, u.data_ptr(), proj.data_ptr(), _ptr(z), a.data_ptr(), d.data_ptr(),
+                          dt_w.data_ptr(), dt_b.data_ptr(), y.data_ptr(), _ptr(state), _ptr(offsets), _ptr(slots),
+                          _ptr(fresh), _ptr(status), workspace, size)
+
+    workspace, size = None, 0
+    if offsets is not None:
+        size = lib.fe_selective_scan_workspace(pack(0, 0))
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _check(lib.fe_selective_scan_device(pack(_ptr(workspace), size), _raw_stream(device.index)))
+    return y

@@ -12,6 +12,9 @@
  * (the reference is batch-1 only), device-pointer entry points, load options,
  * capacity reservation and allocation / launch counters.
  *
+ * Part 3 declares operators on device buffers: the Mamba mixer's convolution
+ * and selective scan over ragged sequences with slot states.
+ *
  * All work runs on a B200; there is no CPU fallback.  Loading fails with a
  * message when no sm_100 device is present.
  */
@@ -366,6 +369,104 @@ uint64_t fe_device_malloc_count(void);
 uint64_t fe_host_malloc_count(void);
 /* Kernel launches issued by this engine so far (graph replays counted per node). */
 uint64_t fe_engine_kernel_launches(const fe_engine* engine);
+
+/* ------------------------------------------------------------------------- */
+/* Part 3: operators on device buffers (no counterpart in the reference)      */
+/*
+ * The Mamba mixer's operators over many independent sequences whose state is
+ * kept in slots.  Every pointer is a device pointer; the work is enqueued on
+ * `stream` (a cudaStream_t; NULL is the default stream) of the device
+ * args->device (-1: the calling thread's current device) and the call returns
+ * before it completes.  No call allocates, synchronises or keeps anything, so
+ * calls may be captured into CUDA graphs and may run at the same time on
+ * different streams as long as their outputs, states and workspaces differ.
+ * Returns FE_STATUS_OK, FE_STATUS_INVALID_ARGUMENT (nothing was launched;
+ * fe_engine_last_error names the argument) or FE_STATUS_RESOURCE_EXHAUSTED
+ * (the launch failed).
+ *
+ * Rows and sequences.  Activations are matrices of `rows` rows; a row is
+ * contiguous and `*_ld` elements from the next.  With `offsets` ([n_seq + 1],
+ * not decreasing, within 0 .. rows) sequence s is the rows offsets[s] ..
+ * offsets[s + 1] - 1, possibly none; rows outside every sequence are left as
+ * they were.  Without offsets every row is a sequence of one token and n_seq
+ * must equal rows.  Sequence s has slot slots[s] (without slots, slot s); a
+ * negative slot skips the sequence: neither its rows nor any slot change.  A
+ * sequence with fresh[s] != 0 starts from a zero state whatever its slot
+ * holds.  A state pointer of NULL means: every sequence starts from zero and
+ * no state is kept.
+ *
+ * Offsets and slots are read on the device.  A sequence whose offsets lie
+ * outside the rows, whose slot is n_slots or more, or whose slot an earlier
+ * sequence of the call has, is skipped, and the FE_SEQ_* bit is set in
+ * *status (an int32 in device memory that the call only adds bits to; may be
+ * NULL).
+ */
+enum { FE_DTYPE_F32 = 0, FE_DTYPE_BF16 = 1, FE_DTYPE_F16 = 2 };
+
+enum { FE_SEQ_BAD_OFFSETS = 1, FE_SEQ_BAD_SLOT = 2, FE_SEQ_DUPLICATE_SLOT = 4 };
+
+/* u[t][c] = SiLU(b[c] + sum_k w[c][k] x[t - (d_conv - 1) + k][c]), the inputs
+ * before a sequence's first row taken from its slot's window; then the window
+ * takes the sequence's last d_conv inputs (the layout of the decode state:
+ * [d_inner][d_conv], newest last, fp32; slot i is slot_stride floats after
+ * slot i - 1).  x and u are `dtype`, w and b fp32, sums fp32.  d_conv 1 .. 8.
+ * u may share no element with x. */
+typedef struct fe_conv_args {
+  uint32_t struct_size; /* sizeof(fe_conv_args) */
+  int32_t device;
+  uint32_t dtype; /* FE_DTYPE_* of x and u */
+  uint32_t d_conv;
+  uint64_t rows, d_inner, n_seq, n_slots;
+  int64_t x_ld, u_ld, slot_stride;
+  const void* x;
+  const float* w; /* [d_inner][d_conv] */
+  const float* b; /* [d_inner] */
+  void* u;
+  float* window; /* [n_slots][slot_stride], or NULL */
+  const int32_t* offsets;
+  const int32_t* slots;
+  const uint8_t* fresh;
+  int32_t* status;
+} fe_conv_args;
+int fe_causal_conv_device(const fe_conv_args* args, void* stream);
+
+/* The selective scan.  A row of proj is [dt_in (dt_rank) | B (d_state) | C
+ * (d_state)]; per row t and channel c
+ *   dt = softplus(dt_b[c] + sum_r dt_in[r] dt_w[r][c])
+ *   h_n = exp(dt a[n][c]) h_n + dt B_n u[t][c]
+ *   y[t][c] = (d[c] u[t][c] + sum_n h_n C_n) SiLU(z[t][c])    (no z: no gate)
+ * u, proj, z and y are `dtype`; weights, states ([d_state][d_inner] per slot)
+ * and all sums are fp32.  d_state 1 .. 32, dt_rank 1 .. 512.  y may share no
+ * element with u, z or proj.  `workspace` holds the partial states of prompts
+ * that are scanned in parallel pieces: at least
+ * fe_selective_scan_workspace(args) bytes (0 for single tokens), 16-byte
+ * aligned, in use until the call's work completes. */
+typedef struct fe_scan_args {
+  uint32_t struct_size; /* sizeof(fe_scan_args) */
+  int32_t device;
+  uint32_t dtype; /* FE_DTYPE_* of u, proj, z and y */
+  uint32_t d_state;
+  uint64_t rows, d_inner, dt_rank, n_seq, n_slots;
+  int64_t u_ld, proj_ld, z_ld, y_ld, slot_stride;
+  const void* u;
+  const void* proj;
+  const void* z; /* or NULL */
+  const float* a;    /* [d_state][d_inner], negative */
+  const float* d;    /* [d_inner] */
+  const float* dt_w; /* [dt_rank][d_inner] */
+  const float* dt_b; /* [d_inner] */
+  void* y;
+  float* state; /* [n_slots][slot_stride], or NULL */
+  const int32_t* offsets;
+  const int32_t* slots;
+  const uint8_t* fresh;
+  int32_t* status;
+  void* workspace;
+  uint64_t workspace_bytes;
+} fe_scan_args;
+int fe_selective_scan_device(const fe_scan_args* args, void* stream);
+/* Reads the sizes, device and offsets (only whether given) of args. */
+size_t fe_selective_scan_workspace(const fe_scan_args* args);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
