@@ -134,6 +134,67 @@ int check_scan(const fe_scan_args* args, const char* call, bool sizes_only) {
   return c.done();
 }
 
+int check_w4(const fe_w4_args* args, const char* call, bool reads_x, bool writes_y, bool per_row) {
+  Checks c(call);
+  c.need(args != nullptr && args->struct_size >= sizeof(fe_w4_args), "args are missing or of another size");
+  if (int rc = c.done(); rc != 0) return rc;
+  const fe_w4_args& a = *args;
+  const std::uint64_t e = dtype_bytes(a.dtype);
+  const std::uint64_t x_rows = per_row ? a.rows : a.m, y_rows = per_row ? a.rows : a.m, y_width = per_row ? a.m : a.k;
+  c.need(e != 0, "unknown dtype");
+  c.need(a.device >= -1, "unknown device");
+  c.need(a.group == 32 || a.group == 64 || a.group == 128, "group is 32, 64 or 128");
+  c.need(a.m >= 1 && a.m <= kMaxWidth && a.k >= 1 && a.k <= kMaxWidth, "m and k are from 1 to 2^20");
+  c.need(!per_row || a.rows <= kMaxWidth, "rows is at most 2^20");
+  c.need(a.packed != nullptr && aligned(a.packed, 16), "packed is required, 16-byte aligned");
+  c.need(a.scales != nullptr && aligned(a.scales, 2), "scales are required, aligned to their elements");
+  if (int rc = c.done(); rc != 0) return rc;
+  const bool some = !per_row || a.rows > 0;
+  if (reads_x && some) {
+    c.need(a.x != nullptr && aligned(a.x, e), "x is required, aligned to its elements");
+    c.need(row_ld(a.x_ld, a.k), "x_ld is at least k");
+  }
+  if (writes_y && some) {
+    c.need(a.y != nullptr && aligned(a.y, e), "y is required, aligned to its elements");
+    c.need(row_ld(a.y_ld, y_width), "y_ld is at least y's width");
+  }
+  if (int rc = c.done(); rc != 0) return rc;
+  if (reads_x && writes_y)
+    c.need(!overlap({a.x, x_rows, a.k, a.x_ld, e}, {a.y, y_rows, y_width, a.y_ld, e}), "y overlaps x");
+  return c.done();
+}
+
+int check_norm(const fe_norm_args* args) {
+  Checks c("fe_residual_norm_device");
+  c.need(args != nullptr && args->struct_size >= sizeof(fe_norm_args), "args are missing or of another size");
+  if (int rc = c.done(); rc != 0) return rc;
+  const fe_norm_args& a = *args;
+  const std::uint64_t e = dtype_bytes(a.dtype), r = dtype_bytes(a.residual_dtype);
+  c.need(e != 0, "unknown dtype");
+  c.need(r != 0 && (a.residual_dtype == a.dtype || a.residual_dtype == FE_DTYPE_F32),
+         "residual_dtype is fp32 or dtype");
+  c.need(a.device >= -1, "unknown device");
+  c.need(a.rows <= kMaxRows, "rows is at most 2^30");
+  c.need(a.dim >= 1 && a.dim <= 16384, "dim is from 1 to 16384");
+  c.need(a.eps >= 0.0f, "eps is not negative");
+  c.need(a.weight != nullptr && aligned(a.weight, 4) && aligned(a.post_weight, 4), "weight is required, 4-byte aligned");
+  if (int rc = c.done(); rc != 0 || a.rows == 0) return rc;
+  c.need(a.x != nullptr && a.residual != nullptr && a.out != nullptr, "x, residual and out are required");
+  c.need(aligned(a.x, e) && aligned(a.gate, e) && aligned(a.out, e) && aligned(a.residual, r),
+         "x, gate, residual and out are aligned to their elements");
+  c.need(row_ld(a.x_ld, a.dim) && row_ld(a.residual_ld, a.dim) && row_ld(a.out_ld, a.dim),
+         "x_ld, residual_ld and out_ld are at least dim");
+  c.need(a.gate == nullptr || a.gate_ld == 0 || row_ld(a.gate_ld, a.dim), "gate_ld is 0 or at least dim");
+  if (int rc = c.done(); rc != 0) return rc;
+  const Matrix x{a.x, a.rows, a.dim, a.x_ld, e}, out{a.out, a.rows, a.dim, a.out_ld, e};
+  const Matrix res{a.residual, a.rows, a.dim, a.residual_ld, r};
+  const Matrix gate = a.gate_ld == 0 ? Matrix{a.gate, 1, a.dim, static_cast<std::int64_t>(a.dim), e}
+                                     : Matrix{a.gate, a.rows, a.dim, a.gate_ld, e};
+  c.need(!overlap(out, x) && !overlap(out, res) && !overlap(out, gate), "out overlaps another argument");
+  c.need(!overlap(res, x) && !overlap(res, gate), "the residual overlaps another argument");
+  return c.done();
+}
+
 // The launch's result as a status.
 int launched(int code, const char* call) {
   if (code == 0) return FE_STATUS_OK;
@@ -204,6 +265,40 @@ int fe_selective_scan_device(const fe_scan_args* args, void* stream) {
            "the workspace is required, 16-byte aligned");
     if (int rc = c.done(); rc != 0) return rc;
     return launched(feb::launch_selective_scan(*args, stream), kCall);
+  });
+}
+
+int fe_w4_matvec_device(const fe_w4_args* args, void* stream) {
+  constexpr const char* kCall = "fe_w4_matvec_device";
+  return guarded([&] {
+    if (int rc = check_w4(args, kCall, true, true, true); rc != 0) return rc;
+    if (args->rows == 0) return static_cast<int>(FE_STATUS_OK);
+    return on_device(args->device, kCall, [&] { return feb::launch_w4_matvec(*args, stream); });
+  });
+}
+
+int fe_w4_quantize_device(const fe_w4_args* args, void* stream) {
+  constexpr const char* kCall = "fe_w4_quantize_device";
+  return guarded([&] {
+    if (int rc = check_w4(args, kCall, true, false, false); rc != 0) return rc;
+    return on_device(args->device, kCall, [&] { return feb::launch_w4_quantize(*args, stream); });
+  });
+}
+
+int fe_w4_dequantize_device(const fe_w4_args* args, void* stream) {
+  constexpr const char* kCall = "fe_w4_dequantize_device";
+  return guarded([&] {
+    if (int rc = check_w4(args, kCall, false, true, false); rc != 0) return rc;
+    return on_device(args->device, kCall, [&] { return feb::launch_w4_dequantize(*args, stream); });
+  });
+}
+
+int fe_residual_norm_device(const fe_norm_args* args, void* stream) {
+  constexpr const char* kCall = "fe_residual_norm_device";
+  return guarded([&] {
+    if (int rc = check_norm(args); rc != 0) return rc;
+    if (args->rows == 0) return static_cast<int>(FE_STATUS_OK);
+    return on_device(args->device, kCall, [&] { return feb::launch_residual_norm(*args, stream); });
   });
 }
 

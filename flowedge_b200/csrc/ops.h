@@ -18,6 +18,12 @@ int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept;
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept;
 int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept;
 
+int launch_w4_quantize(const fe_w4_args& a, void* stream) noexcept;
+int launch_w4_dequantize(const fe_w4_args& a, void* stream) noexcept;
+int launch_w4_matvec(const fe_w4_args& a, void* stream) noexcept;
+
+int launch_residual_norm(const fe_norm_args& a, void* stream) noexcept;
+
 // Last error of this thread (fe_engine_last_error); defined with the engine.
 void set_last_error(std::string message);
 void clear_last_error() noexcept;

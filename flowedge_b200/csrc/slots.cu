@@ -11,14 +11,13 @@
 // sequence keeps one), and a CTA finds its sequence from its tile index by a
 // search over the offsets.  The grid is rows / chunk + n_seq tiles, whatever
 // the lengths, so the host never reads them.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
 
 #include "common.cuh"
+#include "convert.cuh"
 #include "ops.h"
 
 namespace feb {
@@ -40,24 +39,6 @@ struct Seq {
   int slot;
   bool fresh, live;
 };
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) {
-  return __float2half_rn(v);
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
 
 // The sequence that owns tile index `tile` (see the file comment), or -1: a
 // 32-way search, every warp on its own.  The indices found are within
@@ -211,17 +192,18 @@ __global__ void __launch_bounds__(128) conv_prompt_kernel(const ConvParams p) {
 }
 
 template <typename T>
-void conv_typed(const ConvParams& p, cudaStream_t st) {
+int conv_typed(const ConvParams& p, cudaStream_t st) {
   const unsigned cb = static_cast<unsigned>((p.di + 127) / 128);
   if (p.q.offsets == nullptr) {
     conv_token_kernel<T><<<dim3(static_cast<unsigned>(p.q.n_seq), cb), 128, 0, st>>>(p);
-    return;
+    return static_cast<int>(cudaGetLastError());
   }
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
   if (p.dc <= 4)
     conv_prompt_kernel<T, 4><<<grid, 128, 0, st>>>(p);
   else
     conv_prompt_kernel<T, 8><<<grid, 128, 0, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
 }
 
 // --- selective scan -----------------------------------------------------------
@@ -541,13 +523,7 @@ int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept {
                a.x, a.w, a.b, a.u, a.window, a.x_ld, a.u_ld, a.slot_stride, static_cast<int>(a.d_inner),
                static_cast<int>(a.d_conv), 32};
   const auto st = static_cast<cudaStream_t>(stream);
-  if (a.dtype == FE_DTYPE_F32)
-    conv_typed<float>(p, st);
-  else if (a.dtype == FE_DTYPE_BF16)
-    conv_typed<__nv_bfloat16>(p, st);
-  else
-    conv_typed<__half>(p, st);
-  return static_cast<int>(cudaGetLastError());
+  return with_dtype(a.dtype, [&](auto t) { return conv_typed<decltype(t)>(p, st); });
 }
 
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept {
@@ -564,9 +540,7 @@ int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept {
                static_cast<int>(a.d_state), static_cast<int>(a.dt_rank), 0};
   if (a.offsets != nullptr) p.chunk = scan_chunk(p.q.rows, p.di);
   const auto st = static_cast<cudaStream_t>(stream);
-  if (a.dtype == FE_DTYPE_F32) return scan_sized<float>(p, st);
-  if (a.dtype == FE_DTYPE_BF16) return scan_sized<__nv_bfloat16>(p, st);
-  return scan_sized<__half>(p, st);
+  return with_dtype(a.dtype, [&](auto t) { return scan_sized<decltype(t)>(p, st); });
 }
 
 }  // namespace feb

@@ -1,0 +1,323 @@
+// Products of a few rows with 4-bit weights under group scales, and the
+// conversions to and from the packed form (include/flowedge_b200.h,
+// fe_w4_args).
+//
+// y = x W^T on the warp's matrix instruction (16 weight rows x 8 rows of x x
+// 16 elements of k): its cost does not grow up to 8 rows of x, and the weights'
+// whole numbers -8 .. 7 are exact in either 16-bit type, so the products are
+// exact and the sums fp32.  A group's sum is scaled when it is complete; no
+// weight is ever rounded.  x enters as it is (16-bit types) or as three bf16
+// terms that add up to its 24 bits (fp32).
+//
+// Bound by the weights' bytes for few rows; a warp reads 16 weight rows x 64
+// bytes per step, and the k range is split over the warps of a CTA where there
+// are too few rows of weights to fill the GPU.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "convert.cuh"
+#include "ops.h"
+
+namespace feb {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kBlock = 128;  // elements of a packed block of 64 bytes
+
+struct W4Params {
+  const void* x;
+  const uint4* packed;  // [m][blocks][4]
+  const __half* scales;
+  void* y;
+  long long x_ld, y_ld;
+  int rows, m, k, blocks, groups;
+  int kw;      // warps that share a tile of 16 weight rows, each with part of k
+  int stage;   // blocks of x staged in shared memory at a time
+};
+
+// D += A B, fp32 accumulators; A 16 x 16 and B 16 x 8 of fp16 or bf16
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight nibbles -> four pairs of exact q - 8.  A nibble under the exponent of
+// 2^10 (fp16) or 2^7 (bf16) reads as that power plus q.
+template <bool BF16>
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      const uint32_t b = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+      __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&b);
+      h = __hsub2(h, __nv_bfloat162(__float2bfloat16_rn(136.0f), __float2bfloat16_rn(136.0f)));
+      v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const uint32_t b = ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
+      __half2 h = *reinterpret_cast<const __half2*>(&b);
+      h = __hsub2(h, __floats2half2_rn(1032.0f, 1032.0f));
+      v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+}
+
+// Stages rows r0 .. r0 + n - 1, columns of `blocks` packed blocks from block
+// b0 on, as TERMS planes of [n][stride] 16-bit values; zero behind column k.
+template <typename T, int TERMS>
+__device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0, int blocks, unsigned short* sx, int stride) {
+  const int width = blocks * kBlock, first = b0 * kBlock;
+  for (int i = threadIdx.x; i < n * (width / 2); i += blockDim.x) {
+    const int r = i / (width / 2), c = (i - r * (width / 2)) * 2;
+    const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first + c;
+    T v0 = first + c < p.k ? src[0] : from_f32<T>(0.0f), v1 = first + c + 1 < p.k ? src[1] : from_f32<T>(0.0f);
+    unsigned short* dst = sx + r * stride + c;
+    if constexpr (TERMS == 1) {
+      *reinterpret_cast<uint32_t*>(dst) = static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v0)) |
+                                          static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v1)) << 16;
+    } else {
+      // the leading bits as bf16, then the rest's: 8 + 8 + 8 bits, nothing lost
+      float f0 = v0, f1 = v1;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) {
+        const float h0 = __uint_as_float(__float_as_uint(f0) & 0xFFFF0000u);
+        const float h1 = __uint_as_float(__float_as_uint(f1) & 0xFFFF0000u);
+        *reinterpret_cast<uint32_t*>(dst + t * n * stride) = __byte_perm(__float_as_uint(h0), __float_as_uint(h1), 0x7632);
+        f0 = isinf(h0) ? 0.0f : f0 - h0;
+        f1 = isinf(h1) ? 0.0f : f1 - h1;
+      }
+    }
+  }
+}
+
+// 16-bit elements between staged rows: 64 bytes over a multiple of 128, so
+// that the eight rows of a fragment fall into different banks
+__host__ __device__ constexpr int stage_stride(int blocks) { return blocks * kBlock + 32; }
+
+template <typename T, int NT, int GROUP>
+__global__ void __launch_bounds__(kWarps * 32) w4_matvec_kernel(const W4Params p) {
+  constexpr bool kBf16 = !std::is_same_v<T, __half>;
+  constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rw = kWarps / p.kw, wk = warp % p.kw, wr = warp / p.kw;
+  const int m0 = (blockIdx.x * rw + wr) * 16;
+  const int r0 = blockIdx.y * NT * 8, n = min(NT * 8, p.rows - r0);
+  unsigned short* sx = reinterpret_cast<unsigned short*>(smem);
+  const int stride = stage_stride(p.stage);
+  // rows behind the last read the last one and are not written
+  const int ra = min(m0 + g, p.m - 1), rb = min(m0 + g + 8, p.m - 1);
+  const uint4* wa = p.packed + static_cast<long long>(ra) * p.blocks * 4 + t;
+  const uint4* wb = p.packed + static_cast<long long>(rb) * p.blocks * 4 + t;
+  const __half* sa = p.scales + static_cast<long long>(ra) * p.groups;
+  const __half* sb = p.scales + static_cast<long long>(rb) * p.groups;
+  float acc[NT][4] = {};
+  constexpr int kPer = kBlock / GROUP;  // groups of a block
+  for (int b0 = 0; b0 < p.blocks; b0 += p.stage) {
+    const int nb = min(p.stage, p.blocks - b0);
+    if (b0 > 0) __syncthreads();
+    stage_x<T, kTerms>(p, r0, n, b0, nb, sx, stride);
+    __syncthreads();
+    constexpr int kAhead = 4;
+    for (int b = wk; b < nb; b += p.kw * kAhead) {
+      uint4 qa[kAhead], qb[kAhead];
+      __half ha[kAhead][kPer], hb[kAhead][kPer];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int blk = b0 + min(b + i * p.kw, nb - 1);
+        qa[i] = __ldg(wa + blk * 4);
+        qb[i] = __ldg(wb + blk * 4);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int grp = min(blk * kPer + j, p.groups - 1);
+          ha[i][j] = sa[grp];
+          hb[i][j] = sb[grp];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (b + i * p.kw >= nb) break;
+        const uint32_t ua[4] = {qa[i].x, qa[i].y, qa[i].z, qa[i].w}, ub[4] = {qb[i].x, qb[i].y, qb[i].z, qb[i].w};
+        const unsigned short* xs = sx + (b + i * p.kw) * kBlock + t * 8;
+        float part[NT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j % (4 / kPer) == 0)
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) part[q][e] = 0.0f;
+          uint32_t va[4], vb[4];
+          unpack8<kBf16>(ua[j], va);
+          unpack8<kBf16>(ub[j], vb);
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term) {
+              uint4 xb = make_uint4(0u, 0u, 0u, 0u);
+              if (q * 8 + g < n) xb = *reinterpret_cast<const uint4*>(xs + (term * n + q * 8 + g) * stride + j * 32);
+              mma_16816<kBf16>(part[q], va[0], vb[0], va[1], vb[1], xb.x, xb.y);
+              mma_16816<kBf16>(part[q], va[2], vb[2], va[3], vb[3], xb.z, xb.w);
+            }
+          if (j % (4 / kPer) == 4 / kPer - 1) {
+            const float fa = __half2float(ha[i][j / (4 / kPer)]), fb = __half2float(hb[i][j / (4 / kPer)]);
+#pragma unroll
+            for (int q = 0; q < NT; ++q) {
+              acc[q][0] = fmaf(fa, part[q][0], acc[q][0]);
+              acc[q][1] = fmaf(fa, part[q][1], acc[q][1]);
+              acc[q][2] = fmaf(fb, part[q][2], acc[q][2]);
+              acc[q][3] = fmaf(fb, part[q][3], acc[q][3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  // the warps' parts of k, joined in order: [warp][16][NT * 8 + 1]
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);
+  constexpr int kCols = NT * 8 + 1;
+  float* mine = red + warp * 16 * kCols;
+#pragma unroll
+  for (int q = 0; q < NT; ++q) {
+    mine[g * kCols + q * 8 + 2 * t] = acc[q][0];
+    mine[g * kCols + q * 8 + 2 * t + 1] = acc[q][1];
+    mine[(g + 8) * kCols + q * 8 + 2 * t] = acc[q][2];
+    mine[(g + 8) * kCols + q * 8 + 2 * t + 1] = acc[q][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rw * 16 * n; i += blockDim.x) {
+    const int r = i / (rw * 16), o = i - r * (rw * 16);
+    const int m = blockIdx.x * rw * 16 + o;
+    if (m >= p.m) continue;
+    float sum = 0.0f;
+    for (int w = 0; w < p.kw; ++w) sum += red[((o >> 4) * p.kw + w) * 16 * kCols + (o & 15) * kCols + r];
+    static_cast<T*>(p.y)[(r0 + r) * p.y_ld + m] = from_f32<T>(sum);
+  }
+}
+
+template <typename T, int NT, int GROUP>
+int matvec_launch(W4Params p, cudaStream_t st) {
+  constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
+  const int n = std::min(p.rows, NT * 8);
+  // warps over k until there are about 16 on every SM, of 16 weight rows each
+  const int tiles = (p.m + 15) / 16;
+  p.kw = 1;
+  while (p.kw < kWarps && p.kw * 2 <= p.blocks && tiles * p.kw < 16 * current_sm_count()) p.kw *= 2;
+  // x in shared memory: at most 48 KB, so that several CTAs share an SM
+  const int room = 48 * 1024 / (kTerms * n * 2);
+  p.stage = std::max(1, std::min(p.blocks, (room - 32) / kBlock));
+  const std::size_t xs = static_cast<std::size_t>(kTerms) * n * stage_stride(p.stage) * 2;
+  const std::size_t rs = static_cast<std::size_t>(kWarps) * 16 * (NT * 8 + 1) * 4;
+  const int rw = kWarps / p.kw;
+  const dim3 grid(static_cast<unsigned>((tiles + rw - 1) / rw), static_cast<unsigned>((p.rows + NT * 8 - 1) / (NT * 8)));
+  w4_matvec_kernel<T, NT, GROUP><<<grid, kWarps * 32, std::max(xs, rs), st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int GROUP>
+int matvec_rows(const W4Params& p, cudaStream_t st) {
+  if (p.rows <= 8) return matvec_launch<T, 1, GROUP>(p, st);
+  if (p.rows <= 16) return matvec_launch<T, 2, GROUP>(p, st);
+  return matvec_launch<T, 4, GROUP>(p, st);
+}
+
+// One warp per group: the scale, then the group's words.
+template <typename T>
+__global__ void __launch_bounds__(256) w4_quantize_kernel(const T* __restrict__ w, long long ld, int m, int k, int group,
+                                                          int groups, int blocks, uint32_t* packed, __half* scales) {
+  const int lane = threadIdx.x & 31;
+  const long long id = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) >> 5;
+  const int per = kBlock / group;
+  if (id >= static_cast<long long>(m) * blocks * per) return;  // whole warps
+  const int row = static_cast<int>(id / (blocks * per)), grp = static_cast<int>(id - static_cast<long long>(row) * blocks * per);
+  const T* src = w + row * ld + static_cast<long long>(grp) * group;
+  const int have = min(group, k - grp * group);  // none behind the last group
+  float big = 0.0f;
+  for (int i = lane; i < have; i += 32) big = fmaxf(big, fabsf(to_f32(src[i])));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+  const __half scale = __float2half_rn(fminf(big / 7.0f, 65504.0f));
+  const float s = __half2float(scale);
+  if (lane == 0 && grp < groups) scales[static_cast<long long>(row) * groups + grp] = scale;
+  // word i of the group holds its elements 8 i .. 8 i + 7
+  if (lane < group / 8) {
+    uint32_t word = 0;
+    for (int e = 0; e < 8; ++e) {
+      int q = 8;
+      if (lane * 8 + e < have && s > 0.0f) {
+        const float v = fminf(fmaxf(rintf(to_f32(src[lane * 8 + e]) / s), -8.0f), 7.0f);
+        q = static_cast<int>(v) + 8;
+      }
+      word |= static_cast<uint32_t>(q) << (4 * ((e >> 1) + (e & 1) * 4));
+    }
+    const int at = grp * group + lane * 8, blk = at / kBlock, j = at % kBlock / 32, t = at % 32 / 8;
+    packed[(static_cast<long long>(row) * blocks + blk) * 16 + 4 * t + j] = word;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __restrict__ packed,
+                                                            const __half* __restrict__ scales, int m, int k, int group,
+                                                            int groups, int blocks, T* w, long long ld) {
+  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  if (i >= static_cast<long long>(m) * k) return;
+  const int row = static_cast<int>(i / k), c = static_cast<int>(i - static_cast<long long>(row) * k);
+  const int blk = c / kBlock, j = c % kBlock / 32, t = c % 32 / 8, e = c % 8;
+  const uint32_t word = packed[(static_cast<long long>(row) * blocks + blk) * 16 + 4 * t + j];
+  const int q = static_cast<int>(word >> (4 * ((e >> 1) + (e & 1) * 4)) & 15u) - 8;
+  w[row * ld + c] = from_f32<T>(static_cast<float>(q) * __half2float(scales[static_cast<long long>(row) * groups + c / group]));
+}
+
+int blocks_of(const fe_w4_args& a) { return static_cast<int>((a.k + kBlock - 1) / kBlock); }
+int groups_of(const fe_w4_args& a) { return static_cast<int>((a.k + a.group - 1) / a.group); }
+
+}  // namespace
+
+int launch_w4_matvec(const fe_w4_args& a, void* stream) noexcept {
+  const W4Params p{a.x, static_cast<const uint4*>(a.packed), static_cast<const __half*>(a.scales), a.y, a.x_ld, a.y_ld,
+                   static_cast<int>(a.rows), static_cast<int>(a.m), static_cast<int>(a.k), blocks_of(a), groups_of(a),
+                   1, 1};
+  const auto st = static_cast<cudaStream_t>(stream);
+  return with_dtype(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    if (a.group == 32) return matvec_rows<T, 32>(p, st);
+    if (a.group == 64) return matvec_rows<T, 64>(p, st);
+    return matvec_rows<T, 128>(p, st);
+  });
+}
+
+int launch_w4_quantize(const fe_w4_args& a, void* stream) noexcept {
+  const long long warps = static_cast<long long>(a.m) * blocks_of(a) * (kBlock / static_cast<int>(a.group));
+  return with_dtype(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    w4_quantize_kernel<T><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const T*>(a.x), a.x_ld, static_cast<int>(a.m), static_cast<int>(a.k), static_cast<int>(a.group),
+        groups_of(a), blocks_of(a), static_cast<uint32_t*>(a.packed), static_cast<__half*>(a.scales));
+    return static_cast<int>(cudaGetLastError());
+  });
+}
+
+int launch_w4_dequantize(const fe_w4_args& a, void* stream) noexcept {
+  const long long total = static_cast<long long>(a.m) * static_cast<long long>(a.k);
+  return with_dtype(a.dtype, [&](auto t) {
+    using T = decltype(t);
+    w4_dequantize_kernel<T><<<static_cast<unsigned>((total + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint32_t*>(a.packed), static_cast<const __half*>(a.scales), static_cast<int>(a.m),
+        static_cast<int>(a.k), static_cast<int>(a.group), groups_of(a), blocks_of(a), static_cast<T*>(a.y), a.y_ld);
+    return static_cast<int>(cudaGetLastError());
+  });
+}
+
+}  // namespace feb

@@ -155,6 +155,10 @@ SIGNATURES = {
     "fe_causal_conv_device": (C.c_int, [C.c_char_p, C.c_void_p]),
     "fe_selective_scan_device": (C.c_int, [C.c_char_p, C.c_void_p]),
     "fe_selective_scan_workspace": (C.c_size_t, [C.c_char_p]),
+    "fe_w4_matvec_device": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "fe_w4_quantize_device": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "fe_w4_dequantize_device": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "fe_residual_norm_device": (C.c_int, [C.c_char_p, C.c_void_p]),
 }
 
 _lib = None

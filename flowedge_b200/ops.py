@@ -2,7 +2,8 @@
 
 The Mamba mixer's operators for many sequences whose states live in slots:
 ragged prompts (`offsets`) or one token per row, each sequence with a slot of
-a pool (`slots`; negative skips it) and, where `fresh` says so, a zero start.
+a pool (`slots`; negative skips it) and, where `fresh` says so, a zero start;
+products of a few rows with 4-bit weights; the residual and the norms around it.
 
 Each call checks its arguments, enqueues its kernels on the current stream of
 its tensors' device and returns; it keeps nothing.  A refused argument raises
@@ -22,7 +23,8 @@ from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from .engine import FlowEdgeError, load_library
 
-__all__ = ["conv", "scan", "BAD_OFFSETS", "BAD_SLOT", "DUPLICATE_SLOT"]
+__all__ = ["conv", "scan", "w4_quantize", "w4_dequantize", "w4_matvec", "residual_norm", "BAD_OFFSETS", "BAD_SLOT",
+           "DUPLICATE_SLOT"]
 
 # bits that `status` collects
 BAD_OFFSETS, BAD_SLOT, DUPLICATE_SLOT = 1, 2, 4
@@ -30,6 +32,8 @@ BAD_OFFSETS, BAD_SLOT, DUPLICATE_SLOT = 1, 2, 4
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _CONV = struct.Struct("@IiII4Q3q9P")
 _SCAN = struct.Struct("@IiII5Q5q14PQ")
+_W4 = struct.Struct("@IiII3Q2q4P")
+_NORM = struct.Struct("@IiII2Q4q6Pff")
 
 
 def _refuse(message: str):
@@ -182,4 +186,95 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=device)
     _check(lib.fe_selective_scan_device(pack(_ptr(workspace), size), _raw_stream(device.index)))
+    return y
+
+
+def _w4_shapes(m: int, k: int, group: int) -> tuple:
+    if group not in (32, 64, 128):
+        _refuse(f"group is 32, 64 or 128, not {group}")
+    return (m, (k + 127) // 128 * 64), (m, (k + group - 1) // group)
+
+
+def w4_quantize(weight, group: int = 64) -> tuple:
+    """(packed, scales) of a finite weight matrix [m, k]: 4 bits per element, one float16 scale per `group` of k.
+
+    packed is uint8 [m, ceil(k / 128) * 64] in the layout of include/flowedge_b200.h (fe_w4_args), scales
+    [m, ceil(k / group)].
+    """
+    m, k, dtype, device = _first(weight, "weight")
+    ld = _matrix(weight, "weight", m, k, dtype, device)
+    packed_shape, scales_shape = _w4_shapes(m, k, group)
+    packed = torch.empty(packed_shape, dtype=torch.uint8, device=device)
+    scales = torch.empty(scales_shape, dtype=torch.float16, device=device)
+    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, 0, m, k, ld, 0, weight.data_ptr(),
+                    packed.data_ptr(), scales.data_ptr(), 0)
+    _check(load_library().fe_w4_quantize_device(args, _raw_stream(device.index)))
+    return packed, scales
+
+
+def _w4_weight(packed, scales, k: int, group: int, device) -> int:
+    """Checks a packed weight of k columns and returns its rows."""
+    if not isinstance(packed, torch.Tensor) or packed.dim() != 2:
+        _refuse("packed is a tensor of shape (m, ceil(k / 128) * 64)")
+    m = packed.shape[0]
+    packed_shape, scales_shape = _w4_shapes(m, k, group)
+    _flat(packed, "packed", packed_shape, torch.uint8, device)
+    _flat(scales, "scales", scales_shape, torch.float16, device)
+    return m
+
+
+def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float32):
+    """The matrix [m, k] that a packed weight stands for, rounded to `dtype`."""
+    if dtype not in _DTYPES:
+        _refuse("dtype is float32, bfloat16 or float16")
+    device = getattr(packed, "device", None)
+    m = _w4_weight(packed, scales, k, group, device)
+    if not packed.is_cuda:
+        _refuse(f"packed is on {device}, not on a GPU")
+    weight = torch.empty((m, k), dtype=dtype, device=device)
+    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, 0, m, k, 0, k, 0, packed.data_ptr(),
+                    scales.data_ptr(), weight.data_ptr())
+    _check(load_library().fe_w4_dequantize_device(args, _raw_stream(device.index)))
+    return weight
+
+
+def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
+    """x [rows, k] times the transpose of a packed weight [m, k], for a few rows (32 read the weight once).
+
+    float32, bfloat16 or float16 x and result; sums in float32, the weight exact.
+    """
+    rows, k, dtype, device = _first(x, "x")
+    x_ld = _matrix(x, "x", rows, k, dtype, device)
+    m = _w4_weight(packed, scales, k, group, device)
+    y, y_ld = _out(out, rows, m, dtype, device)
+    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(),
+                    packed.data_ptr(), scales.data_ptr(), y.data_ptr())
+    _check(load_library().fe_w4_matvec_device(args, _raw_stream(device.index)))
+    return y
+
+
+def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-5, out=None):
+    """residual += scale * gate * RMSNorm(x; post_weight), in place; returns RMSNorm(residual; weight).
+
+    x, gate ([rows, dim], or [1, dim] for all rows) and the result are float32, bfloat16 or float16 alike; residual
+    float32 or the same; weights [dim] float32, dim 1 to 16384.  Without post_weight x is added as it is.  The returned
+    norm is taken before the residual is rounded to its type.
+    """
+    rows, dim, dtype, device = _first(x, "x")
+    x_ld = _matrix(x, "x", rows, dim, dtype, device)
+    r_dtype = getattr(residual, "dtype", None)
+    r_ld = _matrix(residual, "residual", rows, dim, dtype if r_dtype == dtype else torch.float32, device)
+    _flat(weight, "weight", (dim,), torch.float32, device)
+    if post_weight is not None:
+        _flat(post_weight, "post_weight", (dim,), torch.float32, device)
+    gate_ld = 0
+    if gate is not None:
+        one = isinstance(gate, torch.Tensor) and gate.dim() == 2 and gate.shape[0] == 1
+        gate_ld = _matrix(gate, "gate", 1 if one else rows, dim, dtype, device)
+        gate_ld = 0 if one else gate_ld
+    y, y_ld = _out(out, rows, dim, dtype, device)
+    args = _NORM.pack(_NORM.size, device.index, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
+                      x.data_ptr(), _ptr(post_weight), _ptr(gate), residual.data_ptr(), weight.data_ptr(),
+                      y.data_ptr(), scale, eps)
+    _check(load_library().fe_residual_norm_device(args, _raw_stream(device.index)))
     return y

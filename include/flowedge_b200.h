@@ -13,7 +13,8 @@
  * capacity reservation and allocation / launch counters.
  *
  * Part 3 declares operators on device buffers: the Mamba mixer's convolution
- * and selective scan over ragged sequences with slot states.
+ * and selective scan over ragged sequences with slot states, products with
+ * 4-bit weights, and the residual norm.
  *
  * All work runs on a B200; there is no CPU fallback.  Loading fails with a
  * message when no sm_100 device is present.
@@ -373,8 +374,8 @@ uint64_t fe_engine_kernel_launches(const fe_engine* engine);
 /* ------------------------------------------------------------------------- */
 /* Part 3: operators on device buffers (no counterpart in the reference)      */
 /*
- * The Mamba mixer's operators over many independent sequences whose state is
- * kept in slots.  Every pointer is a device pointer; the work is enqueued on
+ * The operators of a Mamba layer over many independent sequences, the mixer's
+ * state kept in slots.  Every pointer is a device pointer; the work is enqueued on
  * `stream` (a cudaStream_t; NULL is the default stream) of the device
  * args->device (-1: the calling thread's current device) and the call returns
  * before it completes.  No call allocates, synchronises or keeps anything, so
@@ -467,6 +468,65 @@ typedef struct fe_scan_args {
 int fe_selective_scan_device(const fe_scan_args* args, void* stream);
 /* Reads the sizes, device and offsets (only whether given) of args. */
 size_t fe_selective_scan_workspace(const fe_scan_args* args);
+
+/* Weights of 4 bits with group scales: w[m][k] = (q[m][k] - 8) scales[m][k / group],
+ * q from 0 to 15, scales fp16 [m][ceil(k / group)], group 32, 64 or 128.
+ * `packed` [m][ceil(k / 128)][64 bytes], 16-byte aligned: the 32-bit word at
+ * place 4 t + j (t, j from 0 to 3) of a block of 128 elements holds the eight
+ * elements from 32 j + 8 t on; its nibbles 0 .. 7, lowest first, are the
+ * elements 0, 2, 4, 6, 1, 3, 5, 7 of the eight (so that one mask takes out two
+ * neighbours).  Elements behind the last are 8, that is zero.
+ *
+ * fe_w4_matvec_device: y[r][m] = sum_k x[r][k] w[m][k] for a few rows; x and y
+ * are `dtype`, sums fp32 (an fp32 x enters the products unrounded).  Up to 32
+ * rows read the weights once; more rows run in passes of 32.  y may share no
+ * element with x.
+ * fe_w4_quantize_device: packed and scales from the weight matrix x
+ * ([m][x_ld], `dtype`, finite): scale = the group's largest magnitude / 7
+ * rounded to fp16 (at most 65504), q = round(w / scale) + 8 within 0 .. 15,
+ * ties to even (rows is not read).
+ * fe_w4_dequantize_device: the weights as `dtype` into y ([m][y_ld]). */
+typedef struct fe_w4_args {
+  uint32_t struct_size; /* sizeof(fe_w4_args) */
+  int32_t device;
+  uint32_t dtype;
+  uint32_t group;
+  uint64_t rows, m, k;
+  int64_t x_ld, y_ld;
+  const void* x;
+  void* packed;
+  void* scales;
+  void* y;
+} fe_w4_args;
+int fe_w4_matvec_device(const fe_w4_args* args, void* stream);
+int fe_w4_quantize_device(const fe_w4_args* args, void* stream);
+int fe_w4_dequantize_device(const fe_w4_args* args, void* stream);
+
+/* The residual between two blocks and the norms around it, per row:
+ *   t = x post_weight / sqrt(mean(x^2) + eps)      (t = x without post_weight)
+ *   residual = residual + scale gate t             (gate 1 without gate)
+ *   out = residual weight / sqrt(mean(residual^2) + eps)
+ * x, gate and out are `dtype`, the residual (updated in place) fp32 or
+ * `dtype`, weights fp32; sums and the norm's input are fp32, before the
+ * residual's rounding.  gate_ld 0 gives every row the same gate.  dim 1 ..
+ * 16384.  out, residual, x and gate share no element. */
+typedef struct fe_norm_args {
+  uint32_t struct_size; /* sizeof(fe_norm_args) */
+  int32_t device;
+  uint32_t dtype;
+  uint32_t residual_dtype;
+  uint64_t rows, dim;
+  int64_t x_ld, residual_ld, gate_ld, out_ld;
+  const void* x;
+  const float* post_weight; /* [dim], or NULL */
+  const void* gate;         /* or NULL */
+  void* residual;
+  const float* weight; /* [dim] */
+  void* out;
+  float scale;
+  float eps;
+} fe_norm_args;
+int fe_residual_norm_device(const fe_norm_args* args, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

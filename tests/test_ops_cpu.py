@@ -62,3 +62,42 @@ def test_null_arguments(lib):
 def test_cpu_tensors_are_refused():
     with pytest.raises(fe.FlowEdgeError, match="not on a GPU"):
         ops.conv(torch.zeros(2, 8), torch.zeros(8, 4), torch.zeros(8))
+
+
+def _w4(lib, call="fe_w4_matvec_device", **kw):
+    v = {"size": ops._W4.size, "device": -1, "dtype": 0, "group": 64, "rows": 4, "m": 100, "k": 200, "x_ld": 200,
+         "y_ld": 200, "x": BIG, "packed": 64, "scales": 64, "y": 2 * BIG} | kw
+    return getattr(lib, call)(ops._W4.pack(*v.values()), None)
+
+
+@pytest.mark.parametrize("call", ["fe_w4_matvec_device", "fe_w4_quantize_device", "fe_w4_dequantize_device"])
+@pytest.mark.parametrize("change,said", [
+    ({"size": 8}, "size"), ({"dtype": 7}, "dtype"), ({"group": 16}, "group"), ({"m": 0}, "m and k"),
+    ({"k": 2 ** 21}, "m and k"), ({"packed": 72}, "packed"), ({"scales": 0}, "scales"), ({"device": -3}, "device")])
+def test_w4_refusals(lib, call, change, said):
+    assert _w4(lib, call, **change) == 1
+    text = lib.fe_engine_last_error().decode()
+    assert text.startswith(call) and said in text
+
+
+def test_w4_matrix_refusals(lib):
+    for call, change, said in [("fe_w4_matvec_device", {"x_ld": 199}, "x_ld"), ("fe_w4_matvec_device", {"y_ld": 99}, "y_ld"),
+                               ("fe_w4_matvec_device", {"y": BIG}, "overlaps"), ("fe_w4_matvec_device", {"x": 0}, "x is"),
+                               ("fe_w4_quantize_device", {"x": BIG + 1}, "x is"), ("fe_w4_dequantize_device", {"y": 0}, "y is"),
+                               ("fe_w4_dequantize_device", {"y_ld": 199}, "y_ld")]:
+        assert _w4(lib, call, **change) == 1 and said in lib.fe_engine_last_error().decode()
+    assert _w4(lib, rows=0, x=0, y=0) == 0  # nothing to do
+
+
+@pytest.mark.parametrize("change,said", [
+    ({"size": 8}, "size"), ({"dtype": 3}, "dtype"), ({"r_dtype": 2}, "residual_dtype"), ({"dim": 0}, "dim"),
+    ({"dim": 16385}, "dim"), ({"x": 0}, "required"), ({"x_ld": 63}, "x_ld"), ({"gate_ld": 5}, "gate_ld"),
+    ({"out": BIG}, "out overlaps"), ({"residual": BIG}, "residual overlaps"), ({"gate": 4 * BIG}, "out overlaps"),
+    ({"eps": -1.0}, "eps"), ({"eps": float("nan")}, "eps"), ({"weight": 0}, "weight")])
+def test_norm_refusals(lib, change, said):
+    v = {"size": ops._NORM.size, "device": -1, "dtype": 0, "r_dtype": 0, "rows": 4, "dim": 64, "x_ld": 64, "r_ld": 64,
+         "gate_ld": 64, "out_ld": 64, "x": BIG, "post": 0, "gate": 2 * BIG, "residual": 3 * BIG, "weight": 64,
+         "out": 4 * BIG, "scale": 1.0, "eps": 1e-5} | change
+    assert lib.fe_residual_norm_device(ops._NORM.pack(*v.values()), None) == 1
+    text = lib.fe_engine_last_error().decode()
+    assert text.startswith("fe_residual_norm_device") and said in text
