@@ -59,7 +59,8 @@ static __global__ void __launch_bounds__(128) simt_conv_kernel(const SimtConvPar
       const int b = tok / p.L_out;
       const int t = tok - b * p.L_out;
       const int ti = t * p.stride + sl.t_off;
-      if (ti >= 0 && ti < src.length)
+      // (a slice may be padded beyond the source's last channel)
+      if (ti >= 0 && ti < src.length && sl.ch_begin + c < src.channels)
         v = src.ptr[(static_cast<long long>(b) * src.length + ti) * src.channels + sl.ch_begin + c];
     }
     xs[i] = v;
