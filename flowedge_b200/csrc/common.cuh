@@ -51,6 +51,7 @@ enum DeviceError : int {
   kErrProgramLayout = 6,
   kErrDependencyTimeout = 7,
   kErrStageTimeout = 8,
+  kErrTokenRange = 9,
 };
 
 // Every mbarrier wait gives up after kWaitNs of wall time (read from the

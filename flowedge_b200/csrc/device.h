@@ -138,10 +138,27 @@ class MambaDevice {
   [[nodiscard]] virtual std::size_t state_floats() const noexcept = 0;
   virtual int read_state(float* dst, std::string& err) noexcept = 0;
   virtual int write_state(const float* src, std::string& err) noexcept = 0;
+  // A pool of decode states for many sequences: ragged prompts and single
+  // tokens over slots.  The host variants take arguments that the caller has
+  // checked (tokens in the vocabulary, distinct slots within the pool, lengths
+  // of at least one); the device variants check on the device.
+  [[nodiscard]] virtual std::size_t slots() const noexcept = 0;
+  virtual int reserve_slots(std::size_t n_slots, std::string& err) noexcept = 0;
+  virtual int reset_slots(const std::int32_t* slots, std::size_t n, std::string& err) noexcept = 0;
+  virtual int prompt_device(const std::int32_t* tokens, std::size_t rows, const std::int32_t* offsets,
+                            const std::int32_t* slots, const std::uint8_t* fresh, std::size_t n_seq,
+                            float* last_hidden, std::int32_t* status, void* stream, std::string& err) noexcept = 0;
+  virtual int step_device(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                          std::int32_t* status, void* stream, std::string& err) noexcept = 0;
+  virtual int prompt(const std::int32_t* tokens, const std::size_t* lengths, const std::int32_t* slots, bool resume,
+                     std::size_t n_seq, float* last_hidden, std::string& err) noexcept = 0;
+  virtual int step_slots(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                         std::string& err) noexcept = 0;
 };
 
+// w4_group 32, 64 or 128: the projections' weights in 4 bits; 0: as `precision` says.
 std::unique_ptr<MambaDevice> make_mamba_device(const TensorTable& tensors, std::shared_ptr<DeviceContext> ctx,
-                                               Precision precision, std::string& err);
+                                               Precision precision, int w4_group, std::string& err);
 
 struct SmolVLAConfig {
   std::size_t expert_width{}, action_dim{}, vlm_width{}, state_dim{}, layers{};

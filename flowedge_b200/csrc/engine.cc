@@ -7,6 +7,7 @@
 #include <atomic>
 #include <charconv>
 #include <cmath>
+#include <cstddef>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -134,6 +135,10 @@ fe_engine* create_engine(std::shared_ptr<const feb::ModelWeights> weights, const
     set_error("Invalid null model weights");
     return nullptr;
   }
+  if (opt.weights4_group != 0 && opt.weights4_group != 32 && opt.weights4_group != 64 && opt.weights4_group != 128) {
+    set_error("weights4_group must be 0, 32, 64 or 128");
+    return nullptr;
+  }
   if (env_flag("FLOWEDGE_CUDA_FORCE_HOST")) {
     set_error("FLOWEDGE_CUDA_FORCE_HOST=1 is not supported: this library has no host kernels");
     return nullptr;
@@ -189,7 +194,7 @@ fe_engine* create_engine(std::shared_ptr<const feb::ModelWeights> weights, const
       }
     }
     if (t.find("backbone.embeddings.weight") != nullptr) {
-      engine->mamba = feb::make_mamba_device(t, engine->ctx, precision, err);
+      engine->mamba = feb::make_mamba_device(t, engine->ctx, precision, static_cast<int>(opt.weights4_group), err);
       if (!engine->mamba) {
         set_error("Mamba backbone failed to load: " + err);
         return nullptr;
@@ -255,6 +260,16 @@ fe_engine_options default_options(unsigned threads) {
   o.worker_threads = threads;
   o.device = -1;
   o.precision = FE_PRECISION_MODE_AUTO;
+  return o;
+}
+
+// The caller's options: struct_size tells a structure that ends before the
+// fields added since, which then read as zero.
+std::optional<fe_engine_options> read_options(const fe_engine_options* options) {
+  constexpr std::size_t kFirst = offsetof(fe_engine_options, weights4_group);
+  if (options == nullptr || options->struct_size < kFirst) return std::nullopt;
+  fe_engine_options o{};
+  std::memcpy(&o, options, options->struct_size < sizeof(o) ? kFirst : sizeof(o));
   return o;
 }
 
@@ -392,11 +407,12 @@ fe_engine* fe_engine_load_with_threads(const char* path, unsigned worker_threads
 
 fe_engine* fe_engine_load_with_options(const char* path, const fe_engine_options* options) {
   clear_error();
-  if (options == nullptr || options->struct_size < sizeof(fe_engine_options)) {
+  const auto o = read_options(options);
+  if (!o) {
     set_error("Invalid engine options");
     return nullptr;
   }
-  return load_path(path, *options);
+  return load_path(path, *o);
 }
 
 fe_weights* fe_weights_load(const char* path) {
@@ -447,11 +463,12 @@ fe_engine* fe_engine_create_from_weights_auto(const fe_weights* weights) {
 
 fe_engine* fe_engine_create_from_weights_with_options(const fe_weights* weights, const fe_engine_options* options) {
   clear_error();
-  if (weights == nullptr || options == nullptr || options->struct_size < sizeof(fe_engine_options)) {
+  const auto o = read_options(options);
+  if (weights == nullptr || !o) {
     set_error("Invalid arguments to fe_engine_create_from_weights_with_options");
     return nullptr;
   }
-  return create_engine(weights->value, *options);
+  return create_engine(weights->value, *o);
 }
 
 void fe_engine_free(fe_engine* engine) { delete engine; }
@@ -986,6 +1003,159 @@ int fe_engine_step(fe_engine* engine, int32_t token, float* out) {
     set_error("Mamba decode step failed: " + err);
     return FE_STATUS_RESOURCE_EXHAUSTED;
   }
+  return FE_STATUS_OK;
+}
+
+// ---- many sequences over slots ---------------------------------------------------
+
+namespace {
+
+// Whether the engine has a backbone with slots, for the call `what`.
+int check_slots_engine(const fe_engine* engine, const char* what) {
+  if (!engine->mamba) {
+    set_error("Model has no backbone");
+    return FE_STATUS_UNSUPPORTED_MODEL;
+  }
+  if (engine->mamba->slots() == 0) {
+    set_error(std::string("No slots are reserved for ") + what);
+    return FE_STATUS_STATE_UNAVAILABLE;
+  }
+  return FE_STATUS_OK;
+}
+
+// Host slots: within the pool, each at most once.
+int check_slot_list(const fe_engine* engine, const std::int32_t* slots, std::size_t n) {
+  std::vector<bool> seen(engine->mamba->slots());
+  for (std::size_t i = 0; i < n; ++i) {
+    if (slots[i] < 0 || static_cast<std::size_t>(slots[i]) >= seen.size()) {
+      set_error("Slot is outside the reserved slots");
+      return FE_STATUS_INVALID_ARGUMENT;
+    }
+    if (seen[static_cast<std::size_t>(slots[i])]) {
+      set_error("Slot is given twice in one call");
+      return FE_STATUS_INVALID_ARGUMENT;
+    }
+    seen[static_cast<std::size_t>(slots[i])] = true;
+  }
+  return FE_STATUS_OK;
+}
+
+constexpr std::size_t kMaxSlotRows = std::size_t(1) << 30;
+
+int slots_failed(const char* what, const std::string& err) {
+  set_error(std::string(what) + " failed: " + err);
+  return FE_STATUS_RESOURCE_EXHAUSTED;
+}
+
+}  // namespace
+
+int fe_engine_reserve_slots(fe_engine* engine, size_t n_slots) {
+  clear_error();
+  if (engine == nullptr || n_slots == 0 || n_slots > kMaxSlotRows) {
+    set_error("Invalid arguments to fe_engine_reserve_slots");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (!engine->mamba) {
+    set_error("Model has no backbone");
+    return FE_STATUS_UNSUPPORTED_MODEL;
+  }
+  std::string err;
+  if (engine->mamba->reserve_slots(n_slots, err) != 0) return slots_failed("Slot reservation", err);
+  return FE_STATUS_OK;
+}
+
+int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n) {
+  clear_error();
+  if (engine == nullptr || slots == nullptr || n == 0) {
+    set_error("Invalid arguments to fe_engine_reset_slots");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (int rc = check_slots_engine(engine, "fe_engine_reset_slots"); rc != 0) return rc;
+  try {
+    if (int rc = check_slot_list(engine, slots, n); rc != 0) return rc;
+    std::string err;
+    if (engine->mamba->reset_slots(slots, n, err) != 0) return slots_failed("Slot reset", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_reset_slots (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
+}
+
+int fe_engine_prompt_batch(fe_engine* engine, const int32_t* tokens, const size_t* lengths, const int32_t* slots,
+                           size_t n_seq, int resume, float* last_hidden) {
+  clear_error();
+  if (engine == nullptr || tokens == nullptr || lengths == nullptr || slots == nullptr || last_hidden == nullptr ||
+      n_seq == 0) {
+    set_error("Invalid arguments to fe_engine_prompt_batch");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (int rc = check_slots_engine(engine, "fe_engine_prompt_batch"); rc != 0) return rc;
+  try {
+    if (int rc = check_slot_list(engine, slots, n_seq); rc != 0) return rc;
+    std::size_t rows = 0;
+    for (std::size_t s = 0; s < n_seq; ++s) {
+      if (lengths[s] == 0 || lengths[s] > kMaxSlotRows || (rows += lengths[s]) > kMaxSlotRows) {
+        set_error("Prompt lengths must be at least 1, and their sum at most 2^30");
+        return FE_STATUS_INVALID_ARGUMENT;
+      }
+    }
+    if (const int rc = check_tokens(engine, tokens, rows); rc != 0) return rc;
+    std::string err;
+    if (engine->mamba->prompt(tokens, lengths, slots, resume != 0, n_seq, last_hidden, err) != 0)
+      return slots_failed("Mamba prompt", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_prompt_batch (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
+}
+
+int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t rows, const int32_t* offsets,
+                            const int32_t* slots, const uint8_t* fresh, size_t n_seq, float* last_hidden,
+                            int32_t* status, void* stream) {
+  clear_error();
+  if (engine == nullptr || tokens == nullptr || offsets == nullptr || slots == nullptr || last_hidden == nullptr ||
+      rows == 0 || n_seq == 0) {
+    set_error("Invalid arguments to fe_engine_prompt_device");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (int rc = check_slots_engine(engine, "fe_engine_prompt_device"); rc != 0) return rc;
+  std::string err;
+  if (engine->mamba->prompt_device(tokens, rows, offsets, slots, fresh, n_seq, last_hidden, status, stream, err) != 0)
+    return slots_failed("Mamba prompt", err);
+  return FE_STATUS_OK;
+}
+
+int fe_engine_step_batch(fe_engine* engine, const int32_t* tokens, const int32_t* slots, size_t n, float* out) {
+  clear_error();
+  if (engine == nullptr || tokens == nullptr || slots == nullptr || out == nullptr || n == 0) {
+    set_error("Invalid arguments to fe_engine_step_batch");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (int rc = check_slots_engine(engine, "fe_engine_step_batch"); rc != 0) return rc;
+  try {
+    if (int rc = check_slot_list(engine, slots, n); rc != 0) return rc;
+    if (const int rc = check_tokens(engine, tokens, n); rc != 0) return rc;
+    std::string err;
+    if (engine->mamba->step_slots(tokens, slots, n, out, err) != 0) return slots_failed("Mamba step", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_step_batch (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
+}
+
+int fe_engine_step_device(fe_engine* engine, const int32_t* tokens, const int32_t* slots, size_t n, float* out,
+                          int32_t* status, void* stream) {
+  clear_error();
+  if (engine == nullptr || tokens == nullptr || slots == nullptr || out == nullptr || n == 0) {
+    set_error("Invalid arguments to fe_engine_step_device");
+    return FE_STATUS_INVALID_ARGUMENT;
+  }
+  if (int rc = check_slots_engine(engine, "fe_engine_step_device"); rc != 0) return rc;
+  std::string err;
+  if (engine->mamba->step_device(tokens, slots, n, out, status, stream, err) != 0) return slots_failed("Mamba step", err);
   return FE_STATUS_OK;
 }
 

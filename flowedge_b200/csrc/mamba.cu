@@ -16,6 +16,14 @@
 // bf16 mode.  Streaming decode keeps the per-layer conv window and SSM state
 // on the device in the reference's snapshot layout ([di][dc] window, newest
 // last, then [ds][di] state).
+//
+// Many sequences at once (prompt_device, step_device): ragged prompts and
+// single tokens over a pool of such states, on the operators of ops.h:
+//   normed = RMSNorm(hidden) of the first layer
+//   per layer: [x | z] = normed W_in^T, u = conv (slot windows), dbl = u W_x^T,
+//   y = scan (slot states), t = y W_out^T, then the residual norm: hidden += t
+//   and the next layer's (or the final) RMSNorm in one pass.
+// With 4-bit weights, few rows take the projections from the packed weights.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -23,6 +31,7 @@
 #include <map>
 #include <tuple>
 
+#include "ops.h"
 #include "runtime.cuh"
 #include "simt.cuh"
 
@@ -48,6 +57,8 @@ struct Mat {
   void* w3 = nullptr;  // fp32 engines: fp16 [rows_pad][3 cols_pad] = [hi | hi | lo] for the tensor path
   SimtSlice* slices = nullptr;
   int nslices = 0;
+  void* packed = nullptr;  // 4-bit weights (fe_w4_args), w then holds what they stand for
+  void* scales = nullptr;
 };
 
 struct Layer {
@@ -56,6 +67,7 @@ struct Layer {
   float* conv_w = nullptr;  // [di][dc]
   float* conv_b = nullptr;
   float* dt_w = nullptr;    // [di][dr] fp32 (widened)
+  float* dt_t = nullptr;    // [dr][di], for the scan over slots
   float* dt_b = nullptr;
   float* a_neg = nullptr;   // [ds][di] = -exp(A_log)^T (mamba.cc:167-176)
   float* d = nullptr;
@@ -788,6 +800,44 @@ __global__ void embed_kernel(const int* tokens, long long n_tok, const float* em
   }
 }
 
+// embed_kernel for ids that the host has not checked: a row whose id is out of
+// range becomes zeros and the fault is recorded
+__global__ void embed_checked_kernel(const int* tokens, long long n_tok, const float* emb, int dm, int vocab,
+                                     float* hidden, int* err) {
+  const long long total = n_tok * dm;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long tok = i / dm;
+    const int c = static_cast<int>(i - tok * dm), id = tokens[tok];
+    const bool ok = id >= 0 && id < vocab;
+    hidden[i] = ok ? emb[static_cast<long long>(id) * dm + c] : 0.0f;
+    if (!ok && c == 0) atomicCAS(err, 0, kErrTokenRange);
+  }
+}
+
+// fp32 rows as the tensor path's 16-bit operand (store_act16)
+__global__ void act16_kernel(const float* in, long long rows, int width, __half* out, int split) {
+  const long long total = rows * width;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x)
+    store_act16(out, i / width, width, static_cast<int>(i % width), in[i], split);
+}
+
+// Row offsets[s + 1] - 1 (row s without offsets) of every sequence with a slot
+// and at least one row -> out[s]
+__global__ void gather_slots_kernel(const float* hidden, const int* offsets, const int* slots, int n_seq,
+                                    long long rows, int dm, float* out) {
+  const long long total = static_cast<long long>(n_seq) * dm;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long q = i / dm;
+    const int c = static_cast<int>(i - q * dm);
+    const long long begin = offsets != nullptr ? offsets[q] : q, end = offsets != nullptr ? offsets[q + 1] : q + 1;
+    if (slots[q] < 0 || begin < 0 || end <= begin || end > rows) continue;
+    out[i] = hidden[(end - 1) * dm + c];
+  }
+}
+
 // last position of each sequence -> dense [B][dm]
 __global__ void gather_last_kernel(const float* hidden, int B, int L, int dm, float* out) {
   const long long total = static_cast<long long>(B) * dm;
@@ -987,10 +1037,13 @@ __global__ void __launch_bounds__(kDecThreads, 1) mamba_decode_kernel(const Deco
 
 class Mamba final : public MambaDevice {
  public:
-  Mamba(std::shared_ptr<DeviceContext> ctx, Precision prec) : ctx_(std::move(ctx)), prec_(prec) {}
+  Mamba(std::shared_ptr<DeviceContext> ctx, Precision prec, int w4_group)
+      : ctx_(std::move(ctx)), prec_(prec), w4_group_(w4_group) {}
   ~Mamba() override {
     if (step_graph_ != nullptr) cudaGraphExecDestroy(step_graph_);
     for (auto& [k, g] : fwd_graphs_) cudaGraphExecDestroy(g);
+    drop_slot_graphs();
+    if (slot_pinned_ != nullptr) cudaFreeHost(slot_pinned_);
     if (pinned_ != nullptr) cudaFreeHost(pinned_);
   }
   bool load(const TensorTable& t, std::string& err);
@@ -1009,8 +1062,40 @@ class Mamba final : public MambaDevice {
   }
   int read_state(float* dst, std::string& err) noexcept override;
   int write_state(const float* src, std::string& err) noexcept override;
+  std::size_t slots() const noexcept override { return n_slots_; }
+  int reserve_slots(std::size_t n_slots, std::string& err) noexcept override;
+  int reset_slots(const std::int32_t* slots, std::size_t n, std::string& err) noexcept override;
+  int prompt_device(const std::int32_t* tokens, std::size_t rows, const std::int32_t* offsets,
+                    const std::int32_t* slots, const std::uint8_t* fresh, std::size_t n_seq, float* last_hidden,
+                    std::int32_t* status, void* stream, std::string& err) noexcept override;
+  int step_device(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                  std::int32_t* status, void* stream, std::string& err) noexcept override;
+  int prompt(const std::int32_t* tokens, const std::size_t* lengths, const std::int32_t* slots, bool resume,
+             std::size_t n_seq, float* last_hidden, std::string& err) noexcept override;
+  int step_slots(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                 std::string& err) noexcept override;
 
  private:
+  // every layer over rows of tokens_ already embedded in hidden_; the final norm's rows to out_
+  bool run_slots(long long rows, int n_seq, const int* offsets, const int* slots, const std::uint8_t* fresh,
+                 std::int32_t* status, cudaStream_t st, std::string& err);
+  // out = in W^T for run_slots
+  bool project(const Mat& m, const float* in, int in_ld, __half* in16, long long rows, float* out, int out_ld,
+               cudaStream_t st, std::string& err);
+  bool embed_and_run(long long rows, int n_seq, const int* offsets, const int* slots, const std::uint8_t* fresh,
+                     std::int32_t* status, cudaStream_t st, std::string& err);
+  void drop_slot_graphs() noexcept {
+    for (auto& [k, g] : slot_graphs_) cudaGraphExecDestroy(g);
+    slot_graphs_.clear();
+  }
+  int finish_slots(cudaStream_t st, std::string& err) noexcept;
+  // capacity for `rows` tokens, the batch capacity kept
+  int make_room(std::size_t rows, std::string& err) noexcept {
+    if (rows <= cap_tokens_) return slot_rows_ >= rows ? 0 : reserve_slots(n_slots_, err);
+    const std::size_t batch = std::max<std::size_t>(cap_batch_, 1);
+    return reserve(batch, (rows + batch - 1) / batch, err);
+  }
+
   // conv: the layer whose causal conv runs in the epilogue (tensor path,
   // in-projection; sequences of conv_seq tokens; u to u_ (fp32, when
   // conv_u32) and ub_ (fp16))
@@ -1049,6 +1134,22 @@ class Mamba final : public MambaDevice {
   DecodeLayer* dec_layers_ = nullptr;
   unsigned* dec_sync_ = nullptr;
   bool dec_fused_ = false;
+  // slots: a pool of decode states, and buffers for a call's description
+  int w4_group_ = 0;
+  DeviceArena pool_, slot_ws_;
+  float* pool_state_ = nullptr;  // [n_slots_][state_floats()]
+  std::size_t n_slots_ = 0;
+  int *slot_ids_ = nullptr, *slot_offsets_ = nullptr;
+  unsigned char* slot_fresh_ = nullptr;
+  float* proj_out_ = nullptr;  // [cap_rows_][dm]
+  void* scan_ws_ = nullptr;
+  std::size_t scan_ws_bytes_ = 0;
+  std::size_t slot_rows_ = 0, slot_pool_ = 0;  // rows and slots that the buffers hold
+  char* slot_pinned_ = nullptr;                // a call's description, then from slot_pinned_rows_ on its result
+  std::size_t slot_pinned_bytes_ = 0, slot_pinned_rows_ = 0;
+  // the step of n rows (its tokens and slots in tokens_ and slot_ids_, its
+  // rows in out_) as one graph per n
+  std::map<std::size_t, cudaGraphExec_t> slot_graphs_;
 };
 
 bool Mamba::load(const TensorTable& t, std::string& err) {
@@ -1090,7 +1191,8 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
   auto mat_bytes = [&](std::size_t rows, std::size_t cols) {
     const std::size_t rp = (rows + 127) / 128 * 128, cp = (cols + 63) / 64 * 64;
     // bf16: 16-bit W; fp32: fp32 W (CUDA cores) and the [hi | hi | lo] fp16 copy
-    return rp * cp * (bf ? 2 : 4 + 6) + ((cp + 255) / 256) * sizeof(SimtSlice) + 1024;
+    return rp * cp * (bf ? 2 : 4 + 6) + ((cp + 255) / 256) * sizeof(SimtSlice) + 1024 +
+           (w4_group_ > 0 ? rows * ((cols + 127) / 128 * 64 + 2 * ((cols + 31) / 32)) + 1024 : 0);
   };
   ArenaPlan plan;
   plan.add_n<float>(cfg_.vocab * dm + dm);
@@ -1098,7 +1200,7 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
     plan.add(mat_bytes(2 * di, dm));
     plan.add(mat_bytes(dr + 2 * ds, di));
     plan.add(mat_bytes(dm, di));
-    plan.add_n<float>(dm + di * dc + di + di * dr + di + ds * di + di);
+    plan.add_n<float>(dm + di * dc + di + 2 * di * dr + di + ds * di + di);
   }
   if (!wts_.init(plan.total(), err)) return false;
   auto get = [&](std::size_t layer, const std::string& sub, std::initializer_list<std::size_t> shape,
@@ -1127,7 +1229,33 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
     cudaMemcpy(d, h.data(), h.size() * 4, cudaMemcpyHostToDevice);
     return d;
   };
-  auto put_mat = [&](const std::vector<float>& w, int rows, int cols, Mat& m) {
+  // 4-bit weights: the packed form, and in w the values that it stands for
+  bool packed_ok = true;
+  auto pack_w4 = [&](std::vector<float>& w, int rows, int cols, Mat& m) {
+    fe_w4_args a{};
+    a.struct_size = sizeof(a);
+    a.device = -1;
+    a.dtype = FE_DTYPE_F32;
+    a.group = static_cast<std::uint32_t>(w4_group_);
+    a.m = static_cast<std::uint64_t>(rows);
+    a.k = static_cast<std::uint64_t>(cols);
+    a.x_ld = a.y_ld = cols;
+    m.packed = a.packed = wts_.take(static_cast<std::size_t>(rows) * ((cols + 127) / 128 * 64));
+    m.scales = a.scales = wts_.take(static_cast<std::size_t>(rows) * ((cols + w4_group_ - 1) / w4_group_) * 2);
+    DeviceArena scratch;
+    ArenaPlan room;
+    room.add_n<float>(w.size());
+    if (scratch.init(room.total(), err)) a.x = a.y = scratch.take_n<float>(w.size());
+    if (!packed_ok || a.packed == nullptr || a.scales == nullptr || a.y == nullptr ||
+        cudaMemcpy(a.y, w.data(), w.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess) {
+      packed_ok = false;
+      return;
+    }
+    packed_ok = launch_w4_quantize(a, nullptr) == 0 && launch_w4_dequantize(a, nullptr) == 0 &&
+                cudaMemcpy(w.data(), a.y, w.size() * 4, cudaMemcpyDeviceToHost) == cudaSuccess;
+  };
+  auto put_mat = [&](std::vector<float>& w, int rows, int cols, Mat& m) {
+    if (w4_group_ > 0) pack_w4(w, rows, cols, m);
     m.rows = rows;
     m.cols = cols;
     m.rows_pad = (rows + 127) / 128 * 128;
@@ -1138,7 +1266,9 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
                   static_cast<std::size_t>(cols) * 4);
     if (bf) {
       std::vector<std::uint16_t> hb(padded.size());
-      for (std::size_t i = 0; i < hb.size(); ++i) hb[i] = fp16_bits_of_bf16_rounded(padded[i]);
+      // 4-bit weights are not rounded to bf16 on top
+      for (std::size_t i = 0; i < hb.size(); ++i)
+        hb[i] = w4_group_ > 0 ? __half_as_ushort(__float2half_rn(padded[i])) : fp16_bits_of_bf16_rounded(padded[i]);
       m.w = wts_.take(hb.size() * 2);
       cudaMemcpy(m.w, hb.data(), hb.size() * 2, cudaMemcpyHostToDevice);
     } else {
@@ -1194,6 +1324,12 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
       }
     }
     L.dt_w = put(v);
+    {
+      std::vector<float> t(v.size());
+      for (std::size_t c = 0; c < di; ++c)
+        for (std::size_t r = 0; r < dr; ++r) t[r * di + c] = v[c * dr + r];
+      L.dt_t = put(t);
+    }
     if (!get(i, "mixer.dt_proj.bias", {di}, false, v)) return false;
     L.dt_b = put(v);
     if (!get(i, "mixer.A_log", {di, ds}, false, v)) return false;
@@ -1208,6 +1344,10 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
   }
   if (wts_.overflowed()) {
     err = "internal error: Mamba weight arena too small";
+    return false;
+  }
+  if (!packed_ok) {
+    if (err.empty()) err = "packing the 4-bit weights failed";
     return false;
   }
   for (const void* k : {reinterpret_cast<const void*>(scan_chunked_kernel<16, 32, false>),
@@ -1250,6 +1390,7 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   }
   for (auto& [k, g] : fwd_graphs_) cudaGraphExecDestroy(g);
   fwd_graphs_.clear();
+  drop_slot_graphs();
   const std::size_t dm = cfg_.d_model, di = cfg_.d_inner, wd = cfg_.dt_rank + 2 * cfg_.d_state;
   const std::size_t rows = (tokens + 255) / 256 * 256;
   std::size_t nsl = 1;
@@ -1283,6 +1424,7 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
     cudaMemcpy(saved.data(), state_, saved.size() * 4, cudaMemcpyDeviceToHost);
   }
   ws_.release();
+  slot_rows_ = 0;  // the slots' calls use these buffers too
   if (!ws_.init(plan.total(), err)) {
     cap_tokens_ = 0;
     return 2;
@@ -1342,6 +1484,7 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   cap_tokens_ = tokens;
   cap_batch_ = batch;
   cap_rows_ = rows;
+  if (n_slots_ > 0 && reserve_slots(n_slots_, err) != 0) return 2;
   return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
 }
 
@@ -1730,12 +1873,370 @@ int Mamba::write_state(const float* src, std::string& err) noexcept {
   return 0;
 }
 
+// --- many sequences over slots --------------------------------------------------
+
+// Rows up to which 4-bit weights are read packed; above, the tensor path's
+// 16-bit copy of the same values is faster (the products, not the weights'
+// bytes, bound it).
+constexpr long long kW4Rows = 64;
+
+// The pool grows and keeps its states; the buffers of a call are sized for
+// the rows that reserve() made room for.
+int Mamba::reserve_slots(std::size_t n_slots, std::string& err) noexcept {
+  cudaSetDevice(ctx_->device);
+  const std::size_t dm = cfg_.d_model;
+  if (dm > 16384 || cfg_.d_inner > (std::size_t(1) << 20) || cfg_.dt_rank < 1) {
+    err = "slots need d_model <= 16384";
+    return 2;
+  }
+  if (n_slots > n_slots_) {
+    DeviceArena grown;
+    const std::size_t bytes = n_slots * state_floats() * 4, kept = n_slots_ * state_floats() * 4;
+    ArenaPlan room;
+    room.add(bytes);
+    if (!grown.init(room.total(), err)) return 2;
+    auto* p = static_cast<float*>(grown.take(bytes));
+    if (p == nullptr || cudaMemset(p, 0, bytes) != cudaSuccess ||
+        (kept > 0 && (synchronize_context(*ctx_) != 0 ||
+                      cudaMemcpy(p, pool_state_, kept, cudaMemcpyDeviceToDevice) != cudaSuccess)) ||
+        cudaDeviceSynchronize() != cudaSuccess) {
+      err = "slot state set-up failed";
+      return 2;
+    }
+    drop_slot_graphs();
+    pool_.swap(grown);
+    pool_state_ = p;
+    n_slots_ = n_slots;
+  }
+  if (slot_rows_ < cap_tokens_ || slot_pool_ < n_slots_) {
+    cudaDeviceSynchronize();
+    drop_slot_graphs();
+    slot_rows_ = slot_pool_ = 0;
+    scan_ws_bytes_ = selective_scan_workspace_most(cap_tokens_, n_slots_, cfg_.d_inner, cfg_.d_state);
+    ArenaPlan plan;
+    plan.add_n<int>(cap_tokens_);
+    plan.add_n<int>(cap_tokens_ + 1);
+    plan.add(cap_tokens_);
+    plan.add_n<float>(cap_rows_ * dm);
+    plan.add(scan_ws_bytes_);
+    slot_ws_.release();
+    if (!slot_ws_.init(plan.total(), err)) return 2;
+    slot_ids_ = slot_ws_.take_n<int>(cap_tokens_);
+    slot_offsets_ = slot_ws_.take_n<int>(cap_tokens_ + 1);
+    slot_fresh_ = static_cast<unsigned char*>(slot_ws_.take(cap_tokens_));
+    proj_out_ = slot_ws_.take_n<float>(cap_rows_ * dm);
+    scan_ws_ = slot_ws_.take(scan_ws_bytes_);
+    if (slot_ws_.overflowed()) {
+      err = "internal error: slot workspace arena too small";
+      return 2;
+    }
+    slot_pinned_rows_ = (cap_tokens_ * 13 + 19) / 16 * 16;
+    const std::size_t need = slot_pinned_rows_ + std::min(n_slots_, cap_tokens_) * dm * 4;
+    if (slot_pinned_bytes_ < need) {
+      if (slot_pinned_ != nullptr) cudaFreeHost(slot_pinned_);
+      slot_pinned_ = nullptr;
+      slot_pinned_bytes_ = 0;
+      if (counted_host_malloc(reinterpret_cast<void**>(&slot_pinned_), need) != cudaSuccess) {
+        err = "pinned host allocation failed";
+        return 2;
+      }
+      slot_pinned_bytes_ = need;
+    }
+    slot_rows_ = cap_tokens_;
+    slot_pool_ = n_slots_;
+  }
+  return 0;
+}
+
+int Mamba::reset_slots(const std::int32_t* slots, std::size_t n, std::string& err) noexcept {
+  cudaSetDevice(ctx_->device);
+  for (std::size_t i = 0; i < n; ++i)
+    if (cudaMemsetAsync(pool_state_ + static_cast<std::size_t>(slots[i]) * state_floats(), 0, state_floats() * 4,
+                        ctx_->stream) != cudaSuccess) {
+      err = "slot reset failed";
+      return 2;
+    }
+  if (cudaStreamSynchronize(ctx_->stream) != cudaSuccess) {
+    err = "slot reset failed";
+    return 2;
+  }
+  return 0;
+}
+
+bool Mamba::project(const Mat& m, const float* in, int in_ld, __half* in16, long long rows, float* out, int out_ld,
+                    cudaStream_t st, std::string& err) {
+  if (m.packed != nullptr && rows <= kW4Rows) {
+    fe_w4_args a{};
+    a.struct_size = sizeof(a);
+    a.device = -1;
+    a.dtype = FE_DTYPE_F32;
+    a.group = static_cast<std::uint32_t>(w4_group_);
+    a.rows = static_cast<std::uint64_t>(rows);
+    a.m = static_cast<std::uint64_t>(m.rows);
+    a.k = static_cast<std::uint64_t>(m.cols);
+    a.x_ld = in_ld;
+    a.y_ld = out_ld;
+    a.x = in;
+    a.packed = m.packed;
+    a.scales = m.scales;
+    a.y = out;
+    return launch_w4_matvec(a, st) == 0;
+  }
+  // the tensor path takes whole 64-column blocks of its input
+  const bool tc = rows >= kTcMinTokens && in_ld % 64 == 0;
+  if (tc) {
+    const int split = prec_ != Precision::kBF16 ? 1 : 0;
+    act16_kernel<<<ew_grid(rows * in_ld, 256, *ctx_), 256, 0, st>>>(in, rows, in_ld, in16, split);
+  }
+  return gemm(m, tc ? static_cast<const void*>(in16) : in, in_ld, rows, out, out_ld, false, tc, st, err);
+}
+
+bool Mamba::run_slots(long long rows, int n_seq, const int* offsets, const int* slots, const std::uint8_t* fresh,
+                      std::int32_t* status, cudaStream_t st, std::string& err) {
+  const int dm = static_cast<int>(cfg_.d_model), di = static_cast<int>(cfg_.d_inner);
+  const int ds = static_cast<int>(cfg_.d_state), dc = static_cast<int>(cfg_.d_conv);
+  const int dr = static_cast<int>(cfg_.dt_rank), wd = dr + 2 * ds;
+  const std::size_t per = static_cast<std::size_t>(di) * (dc + ds);
+  float* normed = out_;
+  launch_rmsnorm(hidden_, layers_[0].norm, rows, dm, normed, nullptr, 0, st);
+  fe_conv_args c{};
+  c.struct_size = sizeof(c);
+  c.device = -1;
+  c.dtype = FE_DTYPE_F32;
+  c.d_conv = static_cast<std::uint32_t>(dc);
+  c.rows = static_cast<std::uint64_t>(rows);
+  c.d_inner = static_cast<std::uint64_t>(di);
+  c.n_seq = static_cast<std::uint64_t>(n_seq);
+  c.n_slots = n_slots_;
+  c.x_ld = 2 * di;
+  c.u_ld = di;
+  c.slot_stride = static_cast<std::int64_t>(state_floats());
+  c.x = xz_;
+  c.u = u_;
+  c.offsets = offsets;
+  c.slots = slots;
+  c.fresh = fresh;
+  c.status = status;
+  fe_scan_args q{};
+  q.struct_size = sizeof(q);
+  q.device = -1;
+  q.dtype = FE_DTYPE_F32;
+  q.d_state = static_cast<std::uint32_t>(ds);
+  q.rows = c.rows;
+  q.d_inner = c.d_inner;
+  q.dt_rank = static_cast<std::uint64_t>(dr);
+  q.n_seq = c.n_seq;
+  q.n_slots = c.n_slots;
+  q.u_ld = q.y_ld = di;
+  q.proj_ld = wd;
+  q.z_ld = 2 * di;
+  q.slot_stride = c.slot_stride;
+  q.u = u_;
+  q.proj = dbl_;
+  q.z = xz_ + di;
+  q.y = y_;
+  q.offsets = offsets;
+  q.slots = slots;
+  q.fresh = fresh;
+  q.workspace = scan_ws_;
+  q.workspace_bytes = scan_ws_bytes_;
+  if (selective_scan_workspace(q) > scan_ws_bytes_) {
+    err = "internal error: scan workspace too small";
+    return false;
+  }
+  fe_norm_args r{};
+  r.struct_size = sizeof(r);
+  r.device = -1;
+  r.dtype = r.residual_dtype = FE_DTYPE_F32;
+  r.rows = c.rows;
+  r.dim = static_cast<std::uint64_t>(dm);
+  r.x_ld = r.residual_ld = r.out_ld = dm;
+  r.x = proj_out_;
+  r.residual = hidden_;
+  r.out = normed;
+  r.scale = 1.0f;
+  r.eps = 1e-5f;
+  for (std::size_t li = 0; li < layers_.size(); ++li) {
+    const Layer& Ly = layers_[li];
+    if (!project(Ly.in_proj, normed, dm, nb_, rows, xz_, 2 * di, st, err)) return false;
+    c.w = Ly.conv_w;
+    c.b = Ly.conv_b;
+    c.window = pool_state_ + li * per;
+    if (launch_causal_conv(c, st) != 0) return false;
+    c.status = nullptr;  // the first layer reports
+    if (!project(Ly.x_proj, u_, di, ub_, rows, dbl_, wd, st, err)) return false;
+    q.a = Ly.a_neg;
+    q.d = Ly.d;
+    q.dt_w = Ly.dt_t;
+    q.dt_b = Ly.dt_b;
+    q.state = c.window + static_cast<std::size_t>(di) * dc;
+    if (launch_selective_scan(q, st) != 0) return false;
+    if (!project(Ly.out_proj, y_, di, yb_, rows, proj_out_, dm, st, err)) return false;
+    r.weight = li + 1 < layers_.size() ? layers_[li + 1].norm : norm_f_;
+    if (launch_residual_norm(r, st) != 0) return false;
+  }
+  return cudaGetLastError() == cudaSuccess;
+}
+
+bool Mamba::embed_and_run(long long rows, int n_seq, const int* offsets, const int* slots, const std::uint8_t* fresh,
+                          std::int32_t* status, cudaStream_t st, std::string& err) {
+  const int dm = static_cast<int>(cfg_.d_model);
+  embed_checked_kernel<<<ew_grid(rows * dm, 256, *ctx_), 256, 0, st>>>(tokens_, rows, emb_, dm,
+                                                                      static_cast<int>(cfg_.vocab), hidden_, ctx_->d_err);
+  return run_slots(rows, n_seq, offsets, slots, fresh, status, st, err);
+}
+
+int Mamba::prompt_device(const std::int32_t* tokens, std::size_t rows, const std::int32_t* offsets,
+                         const std::int32_t* slots, const std::uint8_t* fresh, std::size_t n_seq, float* last_hidden,
+                         std::int32_t* status, void* stream, std::string& err) noexcept {
+  if (slot_rows_ == 0 || rows > slot_rows_ || n_seq > slot_pool_) {
+    err = slot_rows_ == 0 ? "no slots are reserved" : "rows or sequences exceed the reserved capacity";
+    return 2;
+  }
+  cudaSetDevice(ctx_->device);
+  cudaStream_t st = stream != nullptr ? static_cast<cudaStream_t>(stream) : ctx_->stream;
+  if (tokens != tokens_ && cudaMemcpyAsync(tokens_, tokens, rows * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess) {
+    err = "token copy failed";
+    return 2;
+  }
+  const int dm = static_cast<int>(cfg_.d_model);
+  if (!embed_and_run(static_cast<long long>(rows), static_cast<int>(n_seq), offsets, slots, fresh, status, st, err)) {
+    if (err.empty()) err = std::string("prompt launch failed: ") + cudaGetErrorString(cudaGetLastError());
+    return 2;
+  }
+  gather_slots_kernel<<<ew_grid(static_cast<long long>(n_seq) * dm, 256, *ctx_), 256, 0, st>>>(
+      out_, offsets, slots, static_cast<int>(n_seq), static_cast<long long>(rows), dm, last_hidden);
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+// One token for each of n sequences.  The layers replay as a graph over fixed
+// buffers, unless the caller's own stream is being captured, which takes the
+// launches themselves.
+int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                       std::int32_t* status, void* stream, std::string& err) noexcept {
+  if (slot_rows_ == 0 || n > slot_rows_) {
+    err = slot_rows_ == 0 ? "no slots are reserved" : "rows exceed the reserved capacity";
+    return 2;
+  }
+  cudaSetDevice(ctx_->device);
+  cudaStream_t st = stream != nullptr ? static_cast<cudaStream_t>(stream) : ctx_->stream;
+  const int rows = static_cast<int>(n), dm = static_cast<int>(cfg_.d_model);
+  if ((tokens != tokens_ && cudaMemcpyAsync(tokens_, tokens, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess) ||
+      (slots != slot_ids_ && cudaMemcpyAsync(slot_ids_, slots, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess)) {
+    err = "token copy failed";
+    return 2;
+  }
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  cudaStreamIsCapturing(st, &capturing);
+  if (capturing != cudaStreamCaptureStatusNone || status != nullptr) {
+    if (!embed_and_run(rows, rows, nullptr, slot_ids_, nullptr, status, st, err)) {
+      if (err.empty()) err = std::string("step launch failed: ") + cudaGetErrorString(cudaGetLastError());
+      return 2;
+    }
+  } else {
+    auto it = slot_graphs_.find(n);
+    if (it == slot_graphs_.end()) {
+      cudaStream_t cap = nullptr;
+      cudaGraph_t graph = nullptr;
+      cudaGraphExec_t exec = nullptr;
+      bool ok = cudaStreamCreateWithFlags(&cap, cudaStreamNonBlocking) == cudaSuccess &&
+                cudaStreamBeginCapture(cap, cudaStreamCaptureModeThreadLocal) == cudaSuccess;
+      if (ok) {
+        const bool ran = embed_and_run(rows, rows, nullptr, slot_ids_, nullptr, nullptr, cap, err);
+        ok = cudaStreamEndCapture(cap, &graph) == cudaSuccess && ran && graph != nullptr &&
+             cudaGraphInstantiate(&exec, graph, 0) == cudaSuccess;
+      }
+      if (graph != nullptr) cudaGraphDestroy(graph);
+      if (cap != nullptr) cudaStreamDestroy(cap);
+      if (!ok) {
+        cudaGetLastError();
+        if (err.empty()) err = "step graph capture failed";
+        return 2;
+      }
+      if (slot_graphs_.size() >= 64) {  // a server's few batch sizes; not one graph for every size ever seen
+        cudaDeviceSynchronize();
+        drop_slot_graphs();
+      }
+      it = slot_graphs_.emplace(n, exec).first;
+    }
+    if (cudaGraphLaunch(it->second, st) != cudaSuccess) {
+      err = std::string("step launch failed: ") + cudaGetErrorString(cudaGetLastError());
+      return 2;
+    }
+  }
+  gather_slots_kernel<<<ew_grid(static_cast<long long>(n) * dm, 256, *ctx_), 256, 0, st>>>(
+      out_, nullptr, slot_ids_, rows, rows, dm, out);
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+int Mamba::finish_slots(cudaStream_t st, std::string& err) noexcept {
+  if (cudaStreamSynchronize(st) != cudaSuccess) {
+    err = cudaGetErrorString(cudaGetLastError());
+    return 2;
+  }
+  if (const int code = take_device_error(*ctx_, st); code != 0) {
+    err = device_error_text(code);
+    return 2;
+  }
+  return 0;
+}
+
+// Host buffers: the description goes to the device and the rows come back
+// through pinned memory: [tokens | slots | offsets | fresh], then the rows.
+int Mamba::prompt(const std::int32_t* tokens, const std::size_t* lengths, const std::int32_t* slots, bool resume,
+                  std::size_t n_seq, float* last_hidden, std::string& err) noexcept {
+  std::size_t rows = 0;
+  for (std::size_t s = 0; s < n_seq; ++s) rows += lengths[s];
+  if (make_room(rows, err) != 0) return 2;
+  cudaSetDevice(ctx_->device);
+  cudaStream_t st = ctx_->stream;
+  const std::size_t dm = cfg_.d_model;
+  auto* ptok = reinterpret_cast<std::int32_t*>(slot_pinned_);
+  auto* pslot = ptok + rows;
+  auto* poff = pslot + n_seq;
+  auto* pfresh = reinterpret_cast<unsigned char*>(poff + n_seq + 1);
+  std::memcpy(ptok, tokens, rows * 4);
+  std::memcpy(pslot, slots, n_seq * 4);
+  poff[0] = 0;
+  for (std::size_t s = 0; s < n_seq; ++s) poff[s + 1] = poff[s] + static_cast<std::int32_t>(lengths[s]);
+  std::memset(pfresh, resume ? 0 : 1, n_seq);
+  cudaMemcpyAsync(tokens_, ptok, rows * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_ids_, pslot, n_seq * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_offsets_, poff, (n_seq + 1) * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_fresh_, pfresh, n_seq, cudaMemcpyHostToDevice, st);
+  if (prompt_device(tokens_, rows, slot_offsets_, slot_ids_, slot_fresh_, n_seq, proj_out_, nullptr, st, err) != 0) return 2;
+  auto* prows = reinterpret_cast<float*>(slot_pinned_ + slot_pinned_rows_);
+  cudaMemcpyAsync(prows, proj_out_, n_seq * dm * 4, cudaMemcpyDeviceToHost, st);
+  if (finish_slots(st, err) != 0) return 2;
+  std::memcpy(last_hidden, prows, n_seq * dm * 4);
+  return 0;
+}
+
+int Mamba::step_slots(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
+                      std::string& err) noexcept {
+  if (make_room(n, err) != 0) return 2;
+  cudaSetDevice(ctx_->device);
+  cudaStream_t st = ctx_->stream;
+  const std::size_t dm = cfg_.d_model;
+  auto* ptok = reinterpret_cast<std::int32_t*>(slot_pinned_);
+  std::memcpy(ptok, tokens, n * 4);
+  std::memcpy(ptok + n, slots, n * 4);
+  cudaMemcpyAsync(tokens_, ptok, n * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_ids_, ptok + n, n * 4, cudaMemcpyHostToDevice, st);
+  if (step_device(tokens_, slot_ids_, n, proj_out_, nullptr, st, err) != 0) return 2;
+  auto* prows = reinterpret_cast<float*>(slot_pinned_ + slot_pinned_rows_);
+  cudaMemcpyAsync(prows, proj_out_, n * dm * 4, cudaMemcpyDeviceToHost, st);
+  if (finish_slots(st, err) != 0) return 2;
+  std::memcpy(out, prows, n * dm * 4);
+  return 0;
+}
+
 }  // namespace
 
 std::unique_ptr<MambaDevice> make_mamba_device(const TensorTable& tensors, std::shared_ptr<DeviceContext> ctx,
-                                               Precision precision, std::string& err) {
+                                               Precision precision, int w4_group, std::string& err) {
   cudaSetDevice(ctx->device);
-  auto m = std::make_unique<Mamba>(std::move(ctx), precision);
+  auto m = std::make_unique<Mamba>(std::move(ctx), precision, w4_group);
   if (!m->load(tensors, err)) return nullptr;
   return m;
 }

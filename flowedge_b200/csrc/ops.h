@@ -16,6 +16,10 @@ namespace feb {
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept;
 
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept;
+// At least selective_scan_workspace() of any call of up to `rows` rows and
+// `n_seq` sequences on the current device.
+std::size_t selective_scan_workspace_most(std::size_t rows, std::size_t n_seq, std::size_t d_inner,
+                                          std::size_t d_state) noexcept;
 int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept;
 
 int launch_w4_quantize(const fe_w4_args& a, void* stream) noexcept;

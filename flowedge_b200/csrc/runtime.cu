@@ -185,6 +185,7 @@ const char* device_error_text(int code) noexcept {
     case kErrProgramLayout: return "internal error: small-batch program layout check failed";
     case kErrDependencyTimeout: return "a program dependency wait timed out (small-batch U-Net or tensor-core flow solve)";
     case kErrStageTimeout: return "a staged-input wait of the selective scan timed out";
+    case kErrTokenRange: return "a token ID is out of the vocabulary's range";
     default: return "a device pipeline wait timed out";
   }
 }

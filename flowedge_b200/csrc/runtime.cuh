@@ -8,6 +8,7 @@
 
 #include <cstdint>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "device.h"
@@ -48,6 +49,12 @@ class DeviceArena {
   [[nodiscard]] bool overflowed() const noexcept { return overflowed_; }
   void reset() noexcept { used_ = 0; }
   void release() noexcept;
+  void swap(DeviceArena& other) noexcept {
+    std::swap(base_, other.base_);
+    std::swap(size_, other.size_);
+    std::swap(used_, other.used_);
+    std::swap(overflowed_, other.overflowed_);
+  }
 
  private:
   char* base_ = nullptr;

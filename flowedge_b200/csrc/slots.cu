@@ -443,12 +443,14 @@ __global__ void __launch_bounds__(128) scan_carry_kernel(const ScanParams p) {
   }
 }
 
-// Rows of a tile: enough tiles for about 512 channels' threads on every SM,
-// as powers of two from 16 to 2048.
+// Rows of a tile, a power of two: as many tiles as keep about kFillThreads
+// threads (one per channel) on every SM.
+constexpr int kMinChunk = 16, kMaxChunk = 2048, kFillThreads = 512;
+
 int scan_chunk(long long rows, int di) {
-  const long long want = rows * di / (512LL * current_sm_count());
-  int chunk = 16;
-  while (chunk < 2048 && chunk * 2 <= want) chunk *= 2;
+  const long long want = rows * di / (static_cast<long long>(kFillThreads) * current_sm_count());
+  int chunk = kMinChunk;
+  while (chunk < kMaxChunk && chunk * 2 <= want) chunk *= 2;
   return chunk;
 }
 
@@ -531,6 +533,18 @@ std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept {
   const int chunk = scan_chunk(static_cast<long long>(a.rows), static_cast<int>(a.d_inner));
   if (a.rows <= static_cast<std::uint64_t>(chunk)) return 0;
   return (a.rows / static_cast<std::uint64_t>(chunk) + a.n_seq) * (1 + a.d_state) * a.d_inner * sizeof(float);
+}
+
+std::size_t selective_scan_workspace_most(std::size_t rows, std::size_t n_seq, std::size_t d_inner,
+                                          std::size_t d_state) noexcept {
+  // the most tiles of rows cut by each chunk that scan_chunk gives for fewer
+  std::size_t tiles = 0;
+  for (std::size_t chunk = kMinChunk; chunk <= kMaxChunk; chunk *= 2) {
+    std::size_t most = rows;
+    if (chunk < kMaxChunk) most = std::min(most, 2 * chunk * kFillThreads * current_sm_count() / d_inner + 1);
+    tiles = std::max(tiles, most / chunk);
+  }
+  return (tiles + n_seq) * (1 + d_state) * d_inner * sizeof(float);
 }
 
 int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept {

@@ -63,7 +63,8 @@ class ActionMetadata(C.Structure):
 
 class EngineOptions(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("worker_threads", C.c_uint32), ("device", C.c_int32),
-                ("precision", C.c_uint32), ("max_batch", C.c_uint64), ("max_sequence", C.c_uint64)]
+                ("precision", C.c_uint32), ("max_batch", C.c_uint64), ("max_sequence", C.c_uint64),
+                ("weights4_group", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 # name -> (restype, argtypes) for every entry point of include/flowedge_b200.h
@@ -138,6 +139,14 @@ SIGNATURES = {
                                                     C.c_int, C.c_void_p, C.c_void_p]),
     "fe_engine_run_batch": (C.c_int, [C.c_void_p, _i32p, C.c_size_t, C.c_size_t, _f32p]),
     "fe_engine_run_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "fe_engine_reserve_slots": (C.c_int, [C.c_void_p, C.c_size_t]),
+    "fe_engine_reset_slots": (C.c_int, [C.c_void_p, _i32p, C.c_size_t]),
+    "fe_engine_prompt_batch": (C.c_int, [C.c_void_p, _i32p, _size_p, _i32p, C.c_size_t, C.c_int, _f32p]),
+    "fe_engine_prompt_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fe_engine_step_batch": (C.c_int, [C.c_void_p, _i32p, _i32p, C.c_size_t, _f32p]),
+    "fe_engine_step_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p,
+                                        C.c_void_p]),
     "fe_engine_sample_batch": (C.c_int, [C.c_void_p, _i32p, C.c_size_t, C.c_size_t, _f32p, C.c_size_t, C.c_int,
                                          _f32p]),
     "fe_engine_smolvla_sample_batch": (C.c_int, [C.c_void_p, _f32p, C.c_size_t, C.c_size_t, C.c_size_t, _f32p,
@@ -200,10 +209,11 @@ class Engine:
     """One engine on one GPU (the reference `flowedge.Engine`)."""
 
     def __init__(self, path, threads: int | None = None, *, device: int | None = None, precision: str = "auto",
-                 max_batch: int = 0, max_sequence: int = 0):
+                 max_batch: int = 0, max_sequence: int = 0, weights4_group: int = 0):
         self.lib = load_library()
         opts = EngineOptions(C.sizeof(EngineOptions), 0 if threads is None else threads,
-                             -1 if device is None else device, PRECISIONS[precision], max_batch, max_sequence)
+                             -1 if device is None else device, PRECISIONS[precision], max_batch, max_sequence,
+                             weights4_group, 0)
         self.handle = self.lib.fe_engine_load_with_options(str(path).encode(), C.byref(opts))
         if not self.handle:
             raise RuntimeError(self.lib.fe_engine_last_error().decode())
@@ -409,6 +419,51 @@ class Engine:
         out = np.empty(self.d_model, np.float32)
         self._check(self.lib.fe_engine_step(self.handle, int(token), _p(out)))
         return out
+
+    # many sequences over slots
+    def reserve_slots(self, n_slots: int):
+        self._check(self.lib.fe_engine_reserve_slots(self.handle, n_slots))
+
+    def reset_slots(self, slots):
+        ids = np.ascontiguousarray(slots, np.int32)
+        self._check(self.lib.fe_engine_reset_slots(self.handle, ids.ctypes.data_as(_i32p), ids.size))
+
+    def prompt_batch(self, prompts, slots, resume: bool = False):
+        """Ragged prompts (a list of token sequences), each into a slot of its own: the hidden state of each prompt's
+        last token [n, d_model]; the slots keep the states behind them.  `resume` continues from the slots' states."""
+        parts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        toks = np.ascontiguousarray(np.concatenate(parts)) if parts else np.empty(0, np.int32)
+        lengths = (C.c_size_t * len(parts))(*(p.size for p in parts))
+        ids = np.ascontiguousarray(slots, np.int32)
+        if ids.size != len(parts):
+            raise FlowEdgeError(1, f"{len(parts)} prompts for {ids.size} slots")
+        out = np.empty((len(parts), self.d_model), np.float32)
+        self._check(self.lib.fe_engine_prompt_batch(self.handle, toks.ctypes.data_as(_i32p), lengths,
+                                                    ids.ctypes.data_as(_i32p), len(parts), int(resume), _p(out)))
+        return out
+
+    def prompt_device(self, tokens_ptr: int, rows: int, offsets_ptr: int, slots_ptr: int, n_seq: int,
+                      last_hidden_ptr: int, fresh_ptr: int = 0, status_ptr: int = 0, stream: int = 0):
+        """prompt_batch on device buffers; asynchronous.  No fresh flags: every sequence continues from its slot."""
+        self._check(self.lib.fe_engine_prompt_device(self.handle, tokens_ptr, rows, offsets_ptr, slots_ptr,
+                                                     fresh_ptr or None, n_seq, last_hidden_ptr, status_ptr or None,
+                                                     stream or None))
+
+    def step_batch(self, tokens, slots):
+        """One token for each of the given slots: [n, d_model]."""
+        toks, ids = np.ascontiguousarray(tokens, np.int32), np.ascontiguousarray(slots, np.int32)
+        if toks.size != ids.size:
+            raise FlowEdgeError(1, f"{toks.size} tokens for {ids.size} slots")
+        out = np.empty((toks.size, self.d_model), np.float32)
+        self._check(self.lib.fe_engine_step_batch(self.handle, toks.ctypes.data_as(_i32p), ids.ctypes.data_as(_i32p),
+                                                  toks.size, _p(out)))
+        return out
+
+    def step_device(self, tokens_ptr: int, slots_ptr: int, n: int, out_ptr: int, status_ptr: int = 0,
+                    stream: int = 0):
+        """step_batch on device buffers; asynchronous.  Rows with a negative slot are left as they were."""
+        self._check(self.lib.fe_engine_step_device(self.handle, tokens_ptr, slots_ptr, n, out_ptr, status_ptr or None,
+                                                   stream or None))
 
     def reset(self):
         self.lib.fe_engine_reset(self.handle)

@@ -281,6 +281,13 @@ typedef struct fe_engine_options {
   uint32_t precision;      /* FE_PRECISION_MODE_*; AUTO = bf16 if the file stores bf16 weights */
   uint64_t max_batch;      /* batch capacity reserved at load (0 = FLOWEDGE_MAX_BATCH or 1) */
   uint64_t max_sequence;   /* Mamba prefill capacity in tokens (0 = 512) */
+  /* 32, 64 or 128: the Mamba in / x / out projections' weights are rounded to
+   * 4 bits with one scale per that many inputs (the rule of
+   * fe_w4_quantize_device); every Mamba entry point computes with them, the
+   * calls of up to 64 rows over slots from the packed form.  0: off.  A
+   * structure that ends before this field (struct_size 40) reads as 0. */
+  uint32_t weights4_group;
+  uint32_t reserved;
 } fe_engine_options;
 
 /* Load with explicit options (device, precision, batch capacity). */
@@ -333,6 +340,40 @@ int fe_engine_run_batch(fe_engine* engine, const int32_t* tokens, size_t batch, 
  * completes; batch * seq_len must fit the reserved capacity. */
 int fe_engine_run_device(fe_engine* engine, const int32_t* tokens, size_t batch, size_t seq_len, float* last_hidden,
                          void* stream);
+/* Many sequences over slots: a pool of decode states on the device, so that
+ * ragged prompts leave the state that single tokens then continue from.
+ * fe_engine_reserve_slots makes room for slots 0 .. n_slots - 1 (zero states;
+ * a larger pool keeps the states of a smaller one) and, together with
+ * fe_engine_reserve_batch and max_batch x max_sequence, is what allocates.
+ * Slots are apart from the one state of fe_engine_step. */
+int fe_engine_reserve_slots(fe_engine* engine, size_t n_slots);
+/* Zero states for n slots. */
+int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n);
+/* Prompts of lengths[s] >= 1 tokens, one after the other in `tokens`, each
+ * for a slot of its own: from a zero state, or with resume != 0 from the
+ * slot's.  last_hidden [n_seq][d_model] takes the final-normed hidden state
+ * of each prompt's last token (the flow condition); the slots take the states
+ * behind it.  Host buffers, synchronous. */
+int fe_engine_prompt_batch(fe_engine* engine, const int32_t* tokens, const size_t* lengths, const int32_t* slots,
+                           size_t n_seq, int resume, float* last_hidden);
+/* The same with DEVICE pointers, enqueued on `stream` (NULL = the engine's
+ * stream): offsets [n_seq + 1] into the rows, slots [n_seq] (negative: the
+ * sequence is skipped), fresh [n_seq] (nonzero: from a zero state; NULL: all
+ * continue), sequences checked as in part 3 with their bits in *status (may
+ * be NULL).  Rows of last_hidden without a sequence that ran are left as they
+ * were.  A token outside the vocabulary reads as a zero embedding, and
+ * fe_engine_synchronize reports it.  rows must fit max_batch x max_sequence
+ * and n_seq the reserved slots.  Calls of one engine share its workspace:
+ * they must not overlap. */
+int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t rows, const int32_t* offsets,
+                            const int32_t* slots, const uint8_t* fresh, size_t n_seq, float* last_hidden,
+                            int32_t* status, void* stream);
+/* One token for each of n slots: out [n][d_model].  Host buffers, synchronous. */
+int fe_engine_step_batch(fe_engine* engine, const int32_t* tokens, const int32_t* slots, size_t n, float* out);
+/* The same with DEVICE pointers, as fe_engine_prompt_device; rows of out with
+ * a negative slot are left as they were (a padded batch). */
+int fe_engine_step_device(fe_engine* engine, const int32_t* tokens, const int32_t* slots, size_t n, float* out,
+                          int32_t* status, void* stream);
 /* Batched fe_engine_sample: tokens [batch][seq_len], noise/action [batch][A]. */
 int fe_engine_sample_batch(fe_engine* engine, const int32_t* tokens, size_t batch, size_t seq_len,
                            const float* noise, size_t steps, int method, float* action);
