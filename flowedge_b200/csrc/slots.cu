@@ -326,16 +326,63 @@ __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
   }
 }
 
-constexpr int kTok = 8;  // rows of a step of the prompt kernel
+// 2^x for a pair of x <= 0 on the FMA pipe.  x = k + r with k whole and r in
+// [-1/2, 1/2] (k by adding and taking away 1.5 * 2^23), 2^r = 1 + r q(r) with
+// q the degree-5 Chebyshev interpolant of (2^r - 1) / r, 2^k added to the
+// exponent field; below 2^-125 the result stays there.  The leading 1 is exact
+// and the error is that of the last addition (at most 7.2e-8, mean 3e-10), so
+// that a decay near 1 keeps its distance from 1 over thousands of steps.
+__device__ __forceinline__ float2 exp2_neg2(float2 x) {
+  constexpr float kRound = 12582912.0f;
+  x.x = fmaxf(x.x, -125.0f);
+  x.y = fmaxf(x.y, -125.0f);
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 k = __fadd2_rn(t, make_float2(-kRound, -kRound));
+  const float2 r = __ffma2_rn(k, make_float2(-1.0f, -1.0f), x);
+  float2 p = __ffma2_rn(make_float2(1.5453163e-4f, 1.5453163e-4f), r, make_float2(1.3390863e-3f, 1.3390863e-3f));
+  p = __ffma2_rn(p, r, make_float2(9.6180830e-3f, 9.6180830e-3f));
+  p = __ffma2_rn(p, r, make_float2(5.5503570e-2f, 5.5503570e-2f));
+  p = __ffma2_rn(p, r, make_float2(2.4022651e-1f, 2.4022651e-1f));
+  p = __ffma2_rn(p, r, make_float2(6.9314718e-1f, 6.9314718e-1f));
+  p = __ffma2_rn(p, r, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// softplus_rel for a pair
+__device__ __forceinline__ float2 softplus_rel2(float2 x) {
+  return make_float2(softplus_rel(x.x), softplus_rel(x.y));
+}
+
+constexpr int kTok = 8;        // rows of a step of the prompt kernel
+constexpr int kScanWarps = 4;  // warps of its CTA, 32 channels each
+constexpr int kAhead = 4;      // 32-column pieces of a proj row that are requested a step ahead
+// State pairs whose exponentials go to the FMA pipe: the MUFU unit then has
+// 2 (DS - 2 kPolyPairs) / 2 + 4 results per row and channel to make, the FMA
+// pipe about 4 per state and 12 per exponential; DS / 8 of the pairs balance
+// them.
+template <int DS>
+constexpr int kPolyPairs = DS / 8;
+
+// The shared memory of a step: dt_in of its rows [dr][kTok], then per row
+// [B (DS) | C (DS)], zero behind ds.
+__host__ __device__ constexpr int scan_stage(int dr, int ds_padded) { return kTok * (dr + 2 * ds_padded); }
 
 // One thread per channel, the states in registers, over the rows of one tile.
 // SUMMARY: the tile's sum of dt and its state from a zero start, for the tiles
 // whose sequence goes on (the recurrence over a tile is h -> exp(A sum dt) h +
 // end, so the sum of dt stands for the product of decays).  Otherwise: from
 // the state that enters the tile, with y.
+//
+// Bound by arithmetic: per row and channel DS exponentials (MUFU and FMA pipe
+// share them), dr products for dt and 4 DS for the states; u, z, y and proj
+// pass through once.  Rows go in steps of kTok: the step's proj rows sit in
+// shared memory (read by every channel), the next step's proj, u and z are
+// requested before the arithmetic.  All arithmetic on pairs (FFMA2): states
+// two and two, dt rows two and two.
 template <typename T, int DS, bool SUMMARY>
-__global__ void __launch_bounds__(128) scan_prompt_kernel(const ScanParams p) {
-  extern __shared__ float sp[];  // [dr + 2 ds][kTok]: dt_in, B and C of the step's rows
+__global__ void __launch_bounds__(kScanWarps * 32) scan_prompt_kernel(const ScanParams p) {
+  extern __shared__ __align__(16) float sp[];  // two stages
   if (!SUMMARY) report_offsets(p.q);
   const int s = find_sequence(p.q, blockIdx.x, p.chunk);
   if (s < 0) return;
@@ -346,79 +393,169 @@ __global__ void __launch_bounds__(128) scan_prompt_kernel(const ScanParams p) {
   const bool last = t0 + p.chunk >= q.len;
   if (SUMMARY && last) return;
   const int t1 = min(t0 + p.chunk, q.len);
-  const int c = blockIdx.y * 128 + threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.y * (kScanWarps * 32) + threadIdx.x;
   const bool on = c < p.di;
-  const int cc = on ? c : 0;
-  const int wd = p.dr + 2 * p.ds;
+  const int cc = on ? c : p.di - 1;
+  const int ds = p.ds, dr = p.dr, wd = dr + 2 * ds;
+  const int stage = scan_stage(dr, DS);
   float* st = p.state == nullptr ? nullptr : p.state + q.slot * p.slot_stride + cc;
-  float* ws = p.ws == nullptr ? nullptr : p.ws + static_cast<long long>(blockIdx.x) * (1 + p.ds) * p.di + cc;
-  float h[DS], an[DS];
+  float* ws = p.ws == nullptr ? nullptr : p.ws + static_cast<long long>(blockIdx.x) * (1 + ds) * p.di + cc;
+  const T* proj = static_cast<const T*>(p.proj) + (q.begin + t0) * p.proj_ld;
+  const T* u = static_cast<const T*>(p.u) + (q.begin + t0) * p.u_ld + cc;
+  const T* z = SUMMARY || p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + (q.begin + t0) * p.z_ld + cc;
+  T* y = static_cast<T*>(p.y) + (q.begin + t0) * p.y_ld + cc;
+  const int rows = t1 - t0;
+  // a warp brings two rows of a step: rows 2 warp and 2 warp + 1, a lane
+  // their columns lane + 32 m; column e goes to place(e) + its row's distance
+  auto place = [&](int e, int j) {
+    if (e < dr) return e * kTok + j;
+    const int b = e - dr;
+    return dr * kTok + j * 2 * DS + (b < ds ? b : DS + b - ds);
+  };
+  T pn[2][kAhead];
+  auto request = [&](int t) {
 #pragma unroll
-  for (int n = 0; n < DS; ++n) {
-    an[n] = n < p.ds ? p.a[static_cast<long long>(n) * p.di + cc] * 1.4426950408889634f : 0.0f;
-    h[n] = 0.0f;
-    if (!SUMMARY && n < p.ds) {
-      if (k > 0 || !last)
-        h[n] = ws[static_cast<long long>(1 + n) * p.di];
-      else if (st != nullptr && !q.fresh)
-        h[n] = st[static_cast<long long>(n) * p.di];
+    for (int i = 0; i < 2; ++i) {
+      const int j = t + 2 * warp + i;
+#pragma unroll
+      for (int m = 0; m < kAhead; ++m) {
+        const int e = lane + 32 * m;
+        pn[i][m] = from_f32<T>(0.0f);
+        if (e < wd && j < rows) pn[i][m] = proj[j * p.proj_ld + e];
+      }
     }
+  };
+  auto settle = [&](int t, float* to) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = 2 * warp + i;
+#pragma unroll
+      for (int m = 0; m < kAhead; ++m) {
+        const int e = lane + 32 * m;
+        if (e < wd) to[place(e, j)] = to_f32(pn[i][m]);
+      }
+      for (int e = lane + 32 * kAhead; e < wd; e += 32)
+        to[place(e, j)] = t + j < rows ? to_f32(proj[(t + j) * p.proj_ld + e]) : 0.0f;
+    }
+  };
+  T un[kTok], zn[kTok];
+  auto request_uz = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      un[j] = zn[j] = from_f32<T>(0.0f);
+      if (t + j < rows) {
+        un[j] = u[(t + j) * p.u_ld];
+        if (z != nullptr) zn[j] = z[(t + j) * p.z_ld];
+      }
+    }
+  };
+  if (rows > 0) {
+    request(0);
+    request_uz(0);
+  }
+  if (ds < DS)
+    for (int i = threadIdx.x; i < 2 * kTok * 2 * DS; i += kScanWarps * 32) {
+      const int b = i / (kTok * 2 * DS), e = i % (kTok * 2 * DS);
+      if (e % DS >= ds) sp[b * stage + dr * kTok + e] = 0.0f;
+    }
+  float2 h[DS / 2], an[DS / 2];
+  auto load_state = [&](int n) {
+    if (SUMMARY || n >= ds) return 0.0f;
+    if (k > 0 || !last) return ws[static_cast<long long>(1 + n) * p.di];
+    return st != nullptr && !q.fresh ? st[static_cast<long long>(n) * p.di] : 0.0f;
+  };
+  auto load_a = [&](int n) { return n < ds ? p.a[static_cast<long long>(n) * p.di + cc] * 1.4426950408889634f : 0.0f; };
+#pragma unroll
+  for (int n = 0; n < DS / 2; ++n) {
+    an[n] = make_float2(load_a(2 * n), load_a(2 * n + 1));
+    h[n] = make_float2(load_state(2 * n), load_state(2 * n + 1));
   }
   const float bdt = p.dt_b[cc], dk = p.d[cc];
+  const float* dt_w = p.dt_w + cc;
   float total = 0.0f;
-  const T* u = static_cast<const T*>(p.u) + q.begin * p.u_ld + cc;
-  const T* z = p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + q.begin * p.z_ld + cc;
-  const T* proj = static_cast<const T*>(p.proj) + q.begin * p.proj_ld;
-  T* y = static_cast<T*>(p.y) + q.begin * p.y_ld + cc;
-  for (int t = t0; t < t1; t += kTok) {
-    const int n_tok = min(kTok, t1 - t);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTok * wd; i += 128) {
-      const int j = i / wd, e = i - j * wd;
-      sp[e * kTok + j] = j < n_tok ? to_f32(proj[(t + j) * p.proj_ld + e]) : 0.0f;
+  if (rows > 0) settle(0, sp);
+  for (int t = 0, b = 0; t < rows; t += kTok, b ^= 1) {
+    __syncthreads();  // this step's stage is written, the other one has been read
+    const float* now = sp + b * stage;
+    float uv[kTok], zv[kTok];
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      uv[j] = to_f32(un[j]);
+      zv[j] = to_f32(zn[j]);
     }
-    __syncthreads();
-    float step_total = 0.0f;  // summed apart: fewer roundings than one long sum
-    float dt[kTok];
+    const bool more = t + kTok < rows;
+    if (more) {
+      request(t + kTok);
+      request_uz(t + kTok);
+    }
+    float2 dt[kTok / 2];
 #pragma unroll
-    for (int j = 0; j < kTok; ++j) dt[j] = bdt;
-#pragma unroll 4
-    for (int r = 0; r < p.dr; ++r) {
-      const float w = p.dt_w[static_cast<long long>(r) * p.di + cc];
+    for (int j = 0; j < kTok / 2; ++j) dt[j] = make_float2(bdt, bdt);
+#pragma unroll 8
+    for (int r = 0; r < dr; ++r) {
+      const float w = __ldg(dt_w + static_cast<long long>(r) * p.di);
+      const float4 v0 = *reinterpret_cast<const float4*>(now + r * kTok);
+      const float4 v1 = *reinterpret_cast<const float4*>(now + r * kTok + 4);
+      const float2 w2 = make_float2(w, w);
+      dt[0] = __ffma2_rn(make_float2(v0.x, v0.y), w2, dt[0]);
+      dt[1] = __ffma2_rn(make_float2(v0.z, v0.w), w2, dt[1]);
+      dt[2] = __ffma2_rn(make_float2(v1.x, v1.y), w2, dt[2]);
+      dt[3] = __ffma2_rn(make_float2(v1.z, v1.w), w2, dt[3]);
+    }
 #pragma unroll
-      for (int j = 0; j < kTok; ++j) dt[j] = fmaf(sp[r * kTok + j], w, dt[j]);
+    for (int j = 0; j < kTok / 2; ++j) {
+      dt[j] = softplus_rel2(dt[j]);
+      // rows behind the tile's last leave the state: a step of zero
+      if (t + 2 * j >= rows) dt[j].x = 0.0f;
+      if (t + 2 * j + 1 >= rows) dt[j].y = 0.0f;
+    }
+    if (SUMMARY) {
+      const float2 sum = __fadd2_rn(__fadd2_rn(dt[0], dt[1]), __fadd2_rn(dt[2], dt[3]));
+      total += sum.x + sum.y;
     }
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
-      if (j >= n_tok) break;
-      const float uv = to_f32(u[(t + j) * p.u_ld]);
-      const float d = softplus_rel(dt[j]), dtu = d * uv;
-      const float* col = sp + p.dr * kTok + j;
-      float yv = dk * uv;
-      step_total += d;
+      const float d = j & 1 ? dt[j / 2].y : dt[j / 2].x;
+      const float dtu = d * uv[j];
+      const float2 d2 = make_float2(d, d), dtu2 = make_float2(dtu, dtu);
+      const float* bc = now + dr * kTok + j * 2 * DS;
+      float2 y0 = make_float2(dk * uv[j], 0.0f), y1 = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int n = 0; n < DS; ++n) {
-        if (n >= p.ds) break;
-        h[n] = fmaf(ex2_approx(d * an[n]), h[n], dtu * col[n * kTok]);
-        if (!SUMMARY) yv = fmaf(h[n], col[(p.ds + n) * kTok], yv);
+      for (int n = 0; n < DS / 2; n += 2) {
+        const float4 bq = *reinterpret_cast<const float4*>(bc + 2 * n);
+        const float2 e0 = __fmul2_rn(d2, an[n]), e1 = __fmul2_rn(d2, an[n + 1]);
+        const float2 a0 = n < kPolyPairs<DS> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
+        const float2 a1 = n + 1 < kPolyPairs<DS> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
+        h[n] = __ffma2_rn(a0, h[n], __fmul2_rn(dtu2, make_float2(bq.x, bq.y)));
+        h[n + 1] = __ffma2_rn(a1, h[n + 1], __fmul2_rn(dtu2, make_float2(bq.z, bq.w)));
+        if (!SUMMARY) {
+          const float4 cq = *reinterpret_cast<const float4*>(bc + DS + 2 * n);
+          y0 = __ffma2_rn(h[n], make_float2(cq.x, cq.y), y0);
+          y1 = __ffma2_rn(h[n + 1], make_float2(cq.z, cq.w), y1);
+        }
       }
       if (!SUMMARY) {
-        if (z != nullptr) yv *= silu_f(to_f32(z[(t + j) * p.z_ld]));
-        if (on) y[(t + j) * p.y_ld] = from_f32<T>(yv);
+        float yv = (y0.x + y1.x) + (y0.y + y1.y);
+        if (z != nullptr) yv *= silu_fast(zv[j]);
+        if (on && t + j < rows) y[(t + j) * p.y_ld] = from_f32<T>(yv);
       }
     }
-    total += step_total;
+    if (more) settle(t + kTok, sp + (b ^ 1) * stage);
   }
   if (!on) return;
+  auto store = [&](float* to) {
+#pragma unroll
+    for (int n = 0; n < DS / 2; ++n) {
+      if (2 * n < ds) to[static_cast<long long>(2 * n) * p.di] = h[n].x;
+      if (2 * n + 1 < ds) to[static_cast<long long>(2 * n + 1) * p.di] = h[n].y;
+    }
+  };
   if (SUMMARY) {
     ws[0] = total;
-#pragma unroll
-    for (int n = 0; n < DS; ++n)
-      if (n < p.ds) ws[static_cast<long long>(1 + n) * p.di] = h[n];
+    store(ws + p.di);
   } else if (last && st != nullptr) {
-#pragma unroll
-    for (int n = 0; n < DS; ++n)
-      if (n < p.ds) st[static_cast<long long>(n) * p.di] = h[n];
+    store(st);
   }
 }
 
@@ -466,11 +603,12 @@ int scan_typed(const ScanParams& p, cudaStream_t st) {
     return static_cast<int>(cudaGetLastError());
   }
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
+  const std::size_t smem = 2 * static_cast<std::size_t>(scan_stage(p.dr, DS)) * sizeof(float);
   if (p.q.rows > p.chunk) {
-    scan_prompt_kernel<T, DS, true><<<grid, 128, kTok * row, st>>>(p);
+    scan_prompt_kernel<T, DS, true><<<grid, kScanWarps * 32, smem, st>>>(p);
     scan_carry_kernel<<<dim3(static_cast<unsigned>(p.q.n_seq), cb, static_cast<unsigned>(p.ds)), 128, 0, st>>>(p);
   }
-  scan_prompt_kernel<T, DS, false><<<grid, 128, kTok * row, st>>>(p);
+  scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, smem, st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
