@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "convert.cuh"
@@ -63,7 +64,9 @@ __device__ int find_sequence(const SeqParams& q, long long tile, int chunk) {
 // live is false for a sequence that is skipped: a negative slot, or one of the
 // faults that set a status bit (offsets outside the rows, a slot outside the
 // pool, a slot that an earlier sequence of the call has).
-__device__ Seq resolve(const SeqParams& q, int s, bool report) {
+// `distinct` false leaves that last test out, for work on a sequence's own
+// buffers.
+__device__ __forceinline__ Seq resolve(const SeqParams& q, int s, bool report, bool distinct = true) {
   Seq r;
   int bad = 0;
   if (q.offsets != nullptr) {
@@ -79,7 +82,7 @@ __device__ Seq resolve(const SeqParams& q, int s, bool report) {
   if (q.stateful && r.slot >= q.n_slots) bad |= FE_SEQ_BAD_SLOT;
   r.fresh = q.fresh != nullptr && q.fresh[s] != 0;
   int dup = 0;
-  if (q.stateful && q.slots != nullptr && r.slot >= 0) {
+  if (distinct && q.stateful && q.slots != nullptr && r.slot >= 0) {
     for (int i = threadIdx.x; i < s; i += blockDim.x) dup |= q.slots[i] == r.slot;
     dup = __syncthreads_or(dup);
   }
@@ -214,34 +217,54 @@ struct ScanParams {
   const float *a, *d, *dt_w, *dt_b;  // a [ds][di], dt_w [dr][di]
   void* y;
   float* state;  // [slot][ds][di]
+  float* steps;  // [rows][di], dt of every row (prompts)
   float* ws;     // [tile][1 + ds][di]: sum of dt, then the tile's state (its end from zero; later its start)
   long long u_ld, proj_ld, z_ld, y_ld, slot_stride;
   int di, ds, dr, chunk;
 };
 
-// softplus(x) to a few ulp of the result: e = exp(-|x|) with the rounding error
-// of x log2(e) carried into the exponential, log(1 + e) = 2 atanh(e / (2 + e))
-// by its series (the argument is at most 1/3; the first term left out is
-// below 2^-26 of the sum).  log(1 + e) as it stands would lose dt's relative
-// precision for the small steps that the scan lives on.
-__device__ __forceinline__ float softplus_rel(float x) {
-  constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911e-8f;
-  const float ax = fminf(fabsf(x), 120.0f);
-  const float hi = -ax * kLog2e;
-  const float lo = fmaf(-ax, kLog2e, -hi) - ax * kLog2eLow;
-  const float e2 = ex2_approx(hi);
-  const float e = fmaf(e2 * 0.69314718f, lo, e2);
-  const float s = __fdividef(e, 2.0f + e), s2 = s * s;
-  float r = fmaf(s2, 1.0f / 15.0f, 1.0f / 13.0f);
-  r = fmaf(r, s2, 1.0f / 11.0f);
-  r = fmaf(r, s2, 1.0f / 9.0f);
-  r = fmaf(r, s2, 1.0f / 7.0f);
-  r = fmaf(r, s2, 1.0f / 5.0f);
-  r = fmaf(r, s2, 1.0f / 3.0f);
-  r = fmaf(r * s2, s, s);
-  const float sp = fmaf(2.0f, r, fmaxf(x, 0.0f));
-  return x != x ? x : sp;
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+__device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// softplus of a pair to a few ulp of the result: e = exp(-|x|) with the
+// rounding error of |x| log2(e) carried into the exponential, log(1 + e) =
+// 2 atanh(e / (2 + e)) by its series (the argument s is at most 1/3; the first
+// term left out is below 2^-26 of the sum).  log(1 + e) as it stands would
+// lose dt's relative precision for the small steps that the scan lives on.
+__device__ __forceinline__ float2 softplus_rel2(float2 x) {
+  constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911e-8f;
+  const float2 ax = make_float2(min_nan(fabsf(x.x), 120.0f), min_nan(fabsf(x.y), 120.0f));
+  const float2 hi = __fmul2_rn(ax, splat(-kLog2e));
+  const float2 off = __ffma2_rn(ax, splat(kLog2eLow), __ffma2_rn(ax, splat(kLog2e), hi));  // the exponent is hi - off
+  const float2 e2 = make_float2(ex2_approx(hi.x), ex2_approx(hi.y));
+  const float2 e = __ffma2_rn(__fmul2_rn(e2, splat(-0.69314718f)), off, e2);
+  const float2 den = __fadd2_rn(e, splat(2.0f));
+  const float2 s = __fmul2_rn(e, make_float2(rcp_approx(den.x), rcp_approx(den.y))), s2 = __fmul2_rn(s, s);
+  float2 r = __ffma2_rn(s2, splat(1.0f / 15.0f), splat(1.0f / 13.0f));
+  r = __ffma2_rn(r, s2, splat(1.0f / 11.0f));
+  r = __ffma2_rn(r, s2, splat(1.0f / 9.0f));
+  r = __ffma2_rn(r, s2, splat(1.0f / 7.0f));
+  r = __ffma2_rn(r, s2, splat(1.0f / 5.0f));
+  r = __ffma2_rn(r, s2, splat(1.0f / 3.0f));
+  r = __ffma2_rn(__fmul2_rn(r, s2), s, s);
+  return __ffma2_rn(r, splat(2.0f), make_float2(max_nan(x.x, 0.0f), max_nan(x.y, 0.0f)));
+}
+__device__ __forceinline__ float softplus_rel(float x) { return softplus_rel2(splat(x)).x; }
 
 // One token for each of up to RT sequences, one thread per channel.  The dt
 // projection's weights are read once for the RT tokens; then each sequence's
@@ -349,24 +372,161 @@ __device__ __forceinline__ float2 exp2_neg2(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-// softplus_rel for a pair
-__device__ __forceinline__ float2 softplus_rel2(float2 x) {
-  return make_float2(softplus_rel(x.x), softplus_rel(x.y));
+// Lets a kernel have `bytes` of shared memory (always the same limit, so that
+// calls on several threads do not change each other's).
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              227 * 1024);
 }
 
-constexpr int kTok = 8;        // rows of a step of the prompt kernel
-constexpr int kScanWarps = 4;  // warps of its CTA, 32 channels each
-constexpr int kAhead = 4;      // 32-column pieces of a proj row that are requested a step ahead
-// State pairs whose exponentials go to the FMA pipe: the MUFU unit then has
-// 2 (DS - 2 kPolyPairs) / 2 + 4 results per row and channel to make, the FMA
-// pipe about 4 per state and 12 per exponential; DS / 8 of the pairs balance
-// them.
-template <int DS>
-constexpr int kPolyPairs = DS / 8;
+// --- the steps dt of a prompt call's rows --------------------------------------
+//
+// dt[t][c] = softplus(dt_b[c] + sum_r dt_in[t][r] dt_w[r][c]) for every row, into
+// the workspace: a matrix product once per call, on the warp's matrix
+// instruction, instead of dt_rank products per row and channel on the FMA pipe
+// in each of the scan's passes.  The products are those of fp32: every operand
+// is a sum of bf16 terms (dt_w of three; dt_in of one, two or three as it is
+// bf16, fp16 or fp32: 8, 11 or 24 bits), and all pairs of terms are multiplied
+// whose product is above 2^-25 of the whole, smallest first.
+template <typename T>
+constexpr int kDtTerms = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;
 
-// The shared memory of a step: dt_in of its rows [dr][kTok], then per row
-// [B (DS) | C (DS)], zero behind ds.
-__host__ __device__ constexpr int scan_stage(int dr, int ds_padded) { return kTok * (dr + 2 * ds_padded); }
+// the next bf16 term of a pair, packed; the rest stays in a and b
+__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const float2 f = __bfloat1622float2(h);
+  a = isinf(f.x) ? 0.0f : a - f.x;
+  b = isinf(f.y) ? 0.0f : b - f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A warp takes 16 rows x COLS channels at a time and walks the rows; dt_in goes
+// from memory into fragments, the weights' terms sit in shared memory for the
+// whole kernel: [term][16 of dt_rank][t][channel][2], t and the pair being the
+// fragment's, a lane's two words side by side and the lanes of a half warp on
+// different banks.
+constexpr int kDtWarps = 8;
+constexpr int dt_stride(int cols) { return 2 * cols + 8; }
+
+template <typename T, int COLS>
+__global__ void __launch_bounds__(kDtWarps * 32) scan_steps_kernel(const ScanParams p) {
+  constexpr int kTerms = kDtTerms<T>, kStride = dt_stride(COLS);
+  extern __shared__ __align__(16) uint32_t sb[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int c0 = blockIdx.y * COLS, nk = (p.dr + 15) / 16;
+  for (int i = threadIdx.x; i < nk * 8 * COLS; i += kDtWarps * 32) {
+    const int n = i % COLS, k2 = i / COLS, r = 2 * k2, c = c0 + n;
+    float a = c < p.di && r < p.dr ? p.dt_w[static_cast<long long>(r) * p.di + c] : 0.0f;
+    float b = c < p.di && r + 1 < p.dr ? p.dt_w[static_cast<long long>(r + 1) * p.di + c] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < 3; ++m)
+      sb[((m * nk + k2 / 8) * 4 + k2 % 4) * kStride + 2 * n + k2 % 8 / 4] = take_bf16(a, b);
+  }
+  __syncthreads();
+  const long long step = static_cast<long long>(gridDim.x) * kDtWarps * 16;
+  for (long long row0 = (static_cast<long long>(blockIdx.x) * kDtWarps + warp) * 16; row0 < p.q.rows; row0 += step) {
+    float acc[COLS / 8][4] = {};
+    const bool lo = row0 + g < p.q.rows, hi = row0 + g + 8 < p.q.rows;
+    const T* ra = static_cast<const T*>(p.proj) + (row0 + g) * p.proj_ld;
+    const T* rb = ra + 8 * p.proj_ld;
+    T raw[8];  // rows g, g + 8 x columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the next 16
+    auto request = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 16 * k + 2 * t + (i & 1) + (i & 2) * 4;
+        raw[i] = from_f32<T>(0.0f);
+        if (r < p.dr && (i < 4 ? lo : hi)) raw[i] = (i < 4 ? ra : rb)[r];
+      }
+    };
+    request(0);
+    for (int k = 0; k < nk; ++k) {
+      uint32_t fa[kTerms][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // fragment words: (g, 2t), (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
+        const int at = (i & 1) * 4 + (i & 2);
+        float a = to_f32(raw[at]), b = to_f32(raw[at + 1]);
+#pragma unroll
+        for (int q = 0; q < kTerms; ++q) fa[q][i] = take_bf16(a, b);
+      }
+      if (k + 1 < nk) request(k + 1);
+      // eight tiles at a time, so that the products in flight have sums of their own
+#pragma unroll
+      for (int n0 = 0; n0 < COLS / 8; n0 += 8) {
+#pragma unroll
+        for (int m = 2; m >= 0; --m) {
+          uint2 b[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            b[n] = *reinterpret_cast<const uint2*>(sb + ((m * nk + k) * 4 + t) * kStride + 2 * (8 * (n0 + n) + g));
+#pragma unroll
+          for (int q = kTerms - 1; q >= 0; --q)
+            if (q + m <= 2)
+#pragma unroll
+              for (int n = 0; n < 8; ++n) mma_bf16(acc[n0 + n], fa[q], b[n].x, b[n].y);
+        }
+      }
+    }
+    float* to = p.steps + (row0 + g) * p.di;
+#pragma unroll
+    for (int n = 0; n < COLS / 8; ++n) {
+      const int c = c0 + 8 * n + 2 * t;
+      const float b0 = c < p.di ? p.dt_b[c] : 0.0f, b1 = c + 1 < p.di ? p.dt_b[c + 1] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 v = softplus_rel2(make_float2(acc[n][2 * i] + b0, acc[n][2 * i + 1] + b1));
+        if (!(i ? hi : lo)) continue;
+        float* at = to + static_cast<long long>(8 * i) * p.di + c;
+        if (c + 1 < p.di && p.di % 2 == 0) {
+          *reinterpret_cast<float2*>(at) = v;
+        } else {
+          if (c < p.di) at[0] = v.x;
+          if (c + 1 < p.di) at[1] = v.y;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int COLS>
+int steps_launch_cols(const ScanParams& p, cudaStream_t st) {
+  const int smem = 4 * 3 * ((p.dr + 15) / 16) * 4 * dt_stride(COLS);
+  if (const cudaError_t rc = allow_smem(scan_steps_kernel<T, COLS>, smem); rc != cudaSuccess) return static_cast<int>(rc);
+  const long long tiles = (p.q.rows + 15) / 16, cols = (p.di + COLS - 1) / COLS;
+  // two CTAs on every SM, or the row tiles that there are
+  const long long ctas = std::max(1LL, std::min((tiles + kDtWarps - 1) / kDtWarps, 2LL * current_sm_count() / cols));
+  scan_steps_kernel<T, COLS><<<dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(cols)), kDtWarps * 32,
+                               static_cast<std::size_t>(smem), st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// 128 channels to a CTA, or 64 where the weights' terms of 128 do not fit the
+// shared memory (dt_rank above 256).
+template <typename T>
+int steps_launch(const ScanParams& p, cudaStream_t st) {
+  if (p.q.rows == 0) return 0;
+  return p.dr <= 256 ? steps_launch_cols<T, 128>(p, st) : steps_launch_cols<T, 64>(p, st);
+}
+
+// --- the scan of prompts ----------------------------------------------------------
+
+constexpr int kScanWarps = 4;  // warps of a CTA, 32 channels each
+constexpr int kStage = 16;     // rows whose B and C are in shared memory at a time
+constexpr int kTok = 4;        // rows whose dt, u and z are requested ahead
+// State pairs whose exponentials go to the FMA pipe: one of eight, the first
+// (where a grows with n, as it does at the start of training, the slowest
+// states).  Measured at 16384 rows x 2048 channels, DS 16: none 466 us, one
+// 472, two 490, three 523 (issue slots and the MUFU unit are then level); the
+// one is kept for its exactness near 1.
+template <int DS>
+constexpr int kPolyPairs = DS / 16;
 
 // One thread per channel, the states in registers, over the rows of one tile.
 // SUMMARY: the tile's sum of dt and its state from a zero start, for the tiles
@@ -374,91 +534,93 @@ __host__ __device__ constexpr int scan_stage(int dr, int ds_padded) { return kTo
 // end, so the sum of dt stands for the product of decays).  Otherwise: from
 // the state that enters the tile, with y.
 //
-// Bound by arithmetic: per row and channel DS exponentials (MUFU and FMA pipe
-// share them), dr products for dt and 4 DS for the states; u, z, y and proj
-// pass through once.  Rows go in steps of kTok: the step's proj rows sit in
-// shared memory (read by every channel), the next step's proj, u and z are
-// requested before the arithmetic.  All arithmetic on pairs (FFMA2): states
-// two and two, dt rows two and two.
+// Bound by arithmetic: per row and channel DS exponentials, which MUFU and FMA
+// pipe share, and 4 DS products; dt, u, z and y pass through once.  The rows'
+// B and C sit in shared memory (every channel reads them), the next kStage
+// rows' are requested before the arithmetic; dt, u and z are requested kTok
+// rows ahead.  All arithmetic on pairs (FFMA2): states two and two.
 template <typename T, int DS, bool SUMMARY>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_prompt_kernel(const ScanParams p) {
-  extern __shared__ __align__(16) float sp[];  // two stages
+__global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt_kernel(const ScanParams p) {
+  __shared__ __align__(16) float sbc[2][kStage][2 * DS];
   if (!SUMMARY) report_offsets(p.q);
   const int s = find_sequence(p.q, blockIdx.x, p.chunk);
   if (s < 0) return;
-  const Seq q = resolve(p.q, s, !SUMMARY && blockIdx.y == 0);
+  const Seq q = resolve(p.q, s, !SUMMARY && blockIdx.y == 0, !SUMMARY);
   const long long k = blockIdx.x - (q.begin / p.chunk + s);
   if (!q.live || (k > 0 && k * p.chunk >= q.len)) return;
   const int t0 = static_cast<int>(k * p.chunk);
   const bool last = t0 + p.chunk >= q.len;
   if (SUMMARY && last) return;
-  const int t1 = min(t0 + p.chunk, q.len);
+  const int rows = min(p.chunk, q.len - t0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.y * (kScanWarps * 32) + threadIdx.x;
   const bool on = c < p.di;
   const int cc = on ? c : p.di - 1;
-  const int ds = p.ds, dr = p.dr, wd = dr + 2 * ds;
-  const int stage = scan_stage(dr, DS);
+  const int ds = p.ds;
   float* st = p.state == nullptr ? nullptr : p.state + q.slot * p.slot_stride + cc;
   float* ws = p.ws == nullptr ? nullptr : p.ws + static_cast<long long>(blockIdx.x) * (1 + ds) * p.di + cc;
-  const T* proj = static_cast<const T*>(p.proj) + (q.begin + t0) * p.proj_ld;
-  const T* u = static_cast<const T*>(p.u) + (q.begin + t0) * p.u_ld + cc;
-  const T* z = SUMMARY || p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + (q.begin + t0) * p.z_ld + cc;
-  T* y = static_cast<T*>(p.y) + (q.begin + t0) * p.y_ld + cc;
-  const int rows = t1 - t0;
-  // a warp brings two rows of a step: rows 2 warp and 2 warp + 1, a lane
-  // their columns lane + 32 m; column e goes to place(e) + its row's distance
-  auto place = [&](int e, int j) {
-    if (e < dr) return e * kTok + j;
-    const int b = e - dr;
-    return dr * kTok + j * 2 * DS + (b < ds ? b : DS + b - ds);
-  };
-  T pn[2][kAhead];
+  const long long row0 = q.begin + t0;
+  const T* bc = static_cast<const T*>(p.proj) + row0 * p.proj_ld + p.dr;
+  const float* dt = p.steps + row0 * p.di + cc;
+  const T* u = static_cast<const T*>(p.u) + row0 * p.u_ld + cc;
+  const T* z = SUMMARY || p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + row0 * p.z_ld + cc;
+  T* y = static_cast<T*>(p.y) + row0 * p.y_ld + cc;
+
+  // B and C: a warp brings four rows of a stage, a lane the columns lane + 32 m
+  // of [B (DS) | C (DS)], zero behind ds and behind the last row
+  constexpr int kPieces = (2 * DS + 31) / 32, kMine = kStage / kScanWarps;
+  T pn[kMine][kPieces];
   auto request = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = t + 2 * warp + i;
+    for (int i = 0; i < kMine; ++i) {
+      const int j = t + kMine * warp + i;
 #pragma unroll
-      for (int m = 0; m < kAhead; ++m) {
-        const int e = lane + 32 * m;
+      for (int m = 0; m < kPieces; ++m) {
+        const int e = lane + 32 * m, n = e % DS;
         pn[i][m] = from_f32<T>(0.0f);
-        if (e < wd && j < rows) pn[i][m] = proj[j * p.proj_ld + e];
+        if (e < 2 * DS && n < ds && j < rows) pn[i][m] = bc[j * p.proj_ld + (e < DS ? n : ds + n)];
       }
     }
   };
-  auto settle = [&](int t, float* to) {
+  auto settle = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int j = 2 * warp + i;
+    for (int i = 0; i < kMine; ++i)
 #pragma unroll
-      for (int m = 0; m < kAhead; ++m) {
-        const int e = lane + 32 * m;
-        if (e < wd) to[place(e, j)] = to_f32(pn[i][m]);
-      }
-      for (int e = lane + 32 * kAhead; e < wd; e += 32)
-        to[place(e, j)] = t + j < rows ? to_f32(proj[(t + j) * p.proj_ld + e]) : 0.0f;
-    }
+      for (int m = 0; m < kPieces; ++m)
+        if (lane + 32 * m < 2 * DS) sbc[b][kMine * warp + i][lane + 32 * m] = to_f32(pn[i][m]);
   };
+  // dt, u and z of the next kTok rows; the pointers stand behind the last
+  // whole step requested
+  float dn[kTok];
   T un[kTok], zn[kTok];
-  auto request_uz = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      un[j] = zn[j] = from_f32<T>(0.0f);
-      if (t + j < rows) {
-        un[j] = u[(t + j) * p.u_ld];
-        if (z != nullptr) zn[j] = z[(t + j) * p.z_ld];
-      }
+  const bool gated = z != nullptr;
+  auto request_row = [&](int j) {
+    dn[j] = dt[j * static_cast<long long>(p.di)];
+    un[j] = u[j * p.u_ld];
+    if (gated) zn[j] = z[j * p.z_ld];
+  };
+  auto advance = [&] {
+    dt += kTok * static_cast<long long>(p.di);
+    u += kTok * p.u_ld;
+    if (gated) z += kTok * p.z_ld;
+  };
+  // the stage after the next one into L2: a lane its row's line of this warp
+  auto prefetch = [&](int t) {
+    const int j = t + lane;
+    if (lane < kStage && j < rows) {
+      const long long row = row0 + j;
+      const int cw = min(c - lane, p.di - 1);
+      prefetch_l2(p.steps + row * p.di + cw);
+      prefetch_l2(static_cast<const T*>(p.u) + row * p.u_ld + cw);
+      if (gated) prefetch_l2(static_cast<const T*>(p.z) + row * p.z_ld + cw);
     }
   };
-  if (rows > 0) {
-    request(0);
-    request_uz(0);
-  }
-  if (ds < DS)
-    for (int i = threadIdx.x; i < 2 * kTok * 2 * DS; i += kScanWarps * 32) {
-      const int b = i / (kTok * 2 * DS), e = i % (kTok * 2 * DS);
-      if (e % DS >= ds) sp[b * stage + dr * kTok + e] = 0.0f;
-    }
+  request(0);
+#pragma unroll
+  for (int j = 0; j < kTok; ++j)
+    if (j < rows) request_row(j);
+  advance();
+  prefetch(kTok);
   float2 h[DS / 2], an[DS / 2];
   auto load_state = [&](int n) {
     if (SUMMARY || n >= ds) return 0.0f;
@@ -471,77 +633,70 @@ __global__ void __launch_bounds__(kScanWarps * 32) scan_prompt_kernel(const Scan
     an[n] = make_float2(load_a(2 * n), load_a(2 * n + 1));
     h[n] = make_float2(load_state(2 * n), load_state(2 * n + 1));
   }
-  const float bdt = p.dt_b[cc], dk = p.d[cc];
-  const float* dt_w = p.dt_w + cc;
+  const float dk = p.d[cc];
   float total = 0.0f;
-  if (rows > 0) settle(0, sp);
-  for (int t = 0, b = 0; t < rows; t += kTok, b ^= 1) {
-    __syncthreads();  // this step's stage is written, the other one has been read
-    const float* now = sp + b * stage;
-    float uv[kTok], zv[kTok];
+  float sum_dt = 0.0f;  // summed apart: fewer roundings than one long sum
+  auto one_row = [&](const float* row, float d, float uv, float zv) {
+    const float dtu = d * uv;
+    const float2 d2 = splat(d), dtu2 = splat(dtu);
+    float2 y0 = make_float2(dk * uv, 0.0f), y1 = splat(0.0f);
+    if (SUMMARY) sum_dt += d;
 #pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      uv[j] = to_f32(un[j]);
-      zv[j] = to_f32(zn[j]);
-    }
-    const bool more = t + kTok < rows;
-    if (more) {
-      request(t + kTok);
-      request_uz(t + kTok);
-    }
-    float2 dt[kTok / 2];
-#pragma unroll
-    for (int j = 0; j < kTok / 2; ++j) dt[j] = make_float2(bdt, bdt);
-#pragma unroll 8
-    for (int r = 0; r < dr; ++r) {
-      const float w = __ldg(dt_w + static_cast<long long>(r) * p.di);
-      const float4 v0 = *reinterpret_cast<const float4*>(now + r * kTok);
-      const float4 v1 = *reinterpret_cast<const float4*>(now + r * kTok + 4);
-      const float2 w2 = make_float2(w, w);
-      dt[0] = __ffma2_rn(make_float2(v0.x, v0.y), w2, dt[0]);
-      dt[1] = __ffma2_rn(make_float2(v0.z, v0.w), w2, dt[1]);
-      dt[2] = __ffma2_rn(make_float2(v1.x, v1.y), w2, dt[2]);
-      dt[3] = __ffma2_rn(make_float2(v1.z, v1.w), w2, dt[3]);
-    }
-#pragma unroll
-    for (int j = 0; j < kTok / 2; ++j) {
-      dt[j] = softplus_rel2(dt[j]);
-      // rows behind the tile's last leave the state: a step of zero
-      if (t + 2 * j >= rows) dt[j].x = 0.0f;
-      if (t + 2 * j + 1 >= rows) dt[j].y = 0.0f;
-    }
-    if (SUMMARY) {
-      const float2 sum = __fadd2_rn(__fadd2_rn(dt[0], dt[1]), __fadd2_rn(dt[2], dt[3]));
-      total += sum.x + sum.y;
-    }
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      const float d = j & 1 ? dt[j / 2].y : dt[j / 2].x;
-      const float dtu = d * uv[j];
-      const float2 d2 = make_float2(d, d), dtu2 = make_float2(dtu, dtu);
-      const float* bc = now + dr * kTok + j * 2 * DS;
-      float2 y0 = make_float2(dk * uv[j], 0.0f), y1 = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int n = 0; n < DS / 2; n += 2) {
-        const float4 bq = *reinterpret_cast<const float4*>(bc + 2 * n);
-        const float2 e0 = __fmul2_rn(d2, an[n]), e1 = __fmul2_rn(d2, an[n + 1]);
-        const float2 a0 = n < kPolyPairs<DS> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
-        const float2 a1 = n + 1 < kPolyPairs<DS> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
-        h[n] = __ffma2_rn(a0, h[n], __fmul2_rn(dtu2, make_float2(bq.x, bq.y)));
-        h[n + 1] = __ffma2_rn(a1, h[n + 1], __fmul2_rn(dtu2, make_float2(bq.z, bq.w)));
-        if (!SUMMARY) {
-          const float4 cq = *reinterpret_cast<const float4*>(bc + DS + 2 * n);
-          y0 = __ffma2_rn(h[n], make_float2(cq.x, cq.y), y0);
-          y1 = __ffma2_rn(h[n + 1], make_float2(cq.z, cq.w), y1);
-        }
-      }
+    for (int n = 0; n < DS / 2; n += 2) {
+      const float4 bq = *reinterpret_cast<const float4*>(row + 2 * n);
+      const float2 e0 = __fmul2_rn(d2, an[n]), e1 = __fmul2_rn(d2, an[n + 1]);
+      const float2 a0 = n < kPolyPairs<DS> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
+      const float2 a1 = n + 1 < kPolyPairs<DS> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
+      h[n] = __ffma2_rn(a0, h[n], __fmul2_rn(dtu2, make_float2(bq.x, bq.y)));
+      h[n + 1] = __ffma2_rn(a1, h[n + 1], __fmul2_rn(dtu2, make_float2(bq.z, bq.w)));
       if (!SUMMARY) {
-        float yv = (y0.x + y1.x) + (y0.y + y1.y);
-        if (z != nullptr) yv *= silu_fast(zv[j]);
-        if (on && t + j < rows) y[(t + j) * p.y_ld] = from_f32<T>(yv);
+        const float4 cq = *reinterpret_cast<const float4*>(row + DS + 2 * n);
+        y0 = __ffma2_rn(h[n], make_float2(cq.x, cq.y), y0);
+        y1 = __ffma2_rn(h[n + 1], make_float2(cq.z, cq.w), y1);
       }
     }
-    if (more) settle(t + kTok, sp + (b ^ 1) * stage);
+    const float2 sum = __fadd2_rn(y0, y1);
+    const float yv = sum.x + sum.y;
+    return gated ? yv * silu_fast(zv) : yv;
+  };
+  settle(0);
+  for (int t = 0, b = 0; t < rows; t += kStage, b ^= 1) {
+    __syncthreads();  // this stage is written, the other one has been read
+    const bool more = t + kStage < rows;
+    if (more) {
+      request(t + kStage);
+      prefetch(t + kStage + kTok);
+    }
+    const int stop = min(kStage, rows - t);
+    int i = 0;
+    for (; i + kTok <= stop; i += kTok) {
+      const int left = rows - t - i - kTok;  // rows behind this step
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        const float d = dn[j], uv = to_f32(un[j]), zv = gated ? to_f32(zn[j]) : 0.0f;
+        if (j < left) request_row(j);
+        const float yv = one_row(sbc[b][i + j], d, uv, zv);
+        if (!SUMMARY && on) y[j * p.y_ld] = from_f32<T>(yv);
+      }
+      advance();
+      y += kTok * p.y_ld;
+      total += sum_dt;
+      sum_dt = 0.0f;
+    }
+    for (; i < stop; ++i) {  // the last rows of the tile, fewer than kTok
+      const float yv = one_row(sbc[b][i], dn[0], to_f32(un[0]), gated ? to_f32(zn[0]) : 0.0f);
+      if (!SUMMARY && on) *y = from_f32<T>(yv);
+      y += p.y_ld;
+#pragma unroll
+      for (int j = 0; j + 1 < kTok; ++j) {
+        dn[j] = dn[j + 1];
+        un[j] = un[j + 1];
+        zn[j] = zn[j + 1];
+      }
+    }
+    total += sum_dt;
+    sum_dt = 0.0f;
+    if (more) settle(b ^ 1);
   }
   if (!on) return;
   auto store = [&](float* to) {
@@ -560,29 +715,51 @@ __global__ void __launch_bounds__(kScanWarps * 32) scan_prompt_kernel(const Scan
 }
 
 // The state that enters each tile of a sequence of several, in place of the
-// tile's own end: one thread per (channel, state) walks the tiles.
+// tile's own end: one thread per channel and kCarryStates states walks the
+// tiles, the next kCarryAhead of them requested at a time.
+constexpr int kCarryStates = 2, kCarryAhead = 4;
 __global__ void __launch_bounds__(128) scan_carry_kernel(const ScanParams p) {
-  const int s = blockIdx.x, n = blockIdx.z;
-  const Seq q = resolve(p.q, s, false);
+  const int s = blockIdx.x, n0 = blockIdx.z * kCarryStates;
+  if (p.q.offsets[s + 1] - p.q.offsets[s] <= p.chunk) return;
+  const Seq q = resolve(p.q, s, false, false);
   const int c = blockIdx.y * 128 + threadIdx.x;
-  if (!q.live || q.len <= p.chunk || c >= p.di) return;
+  if (!q.live || c >= p.di) return;
   const int tiles = (q.len + p.chunk - 1) / p.chunk;
-  float* ws = p.ws + (q.begin / p.chunk + s) * (1 + p.ds) * p.di + c;
-  const float an = p.a[static_cast<long long>(n) * p.di + c] * 1.4426950408889634f;
-  float h = p.state == nullptr || q.fresh ? 0.0f : p.state[q.slot * p.slot_stride + static_cast<long long>(n) * p.di + c];
   const long long step = static_cast<long long>(1 + p.ds) * p.di;
-  for (int k = 0; k < tiles; ++k, ws += step) {
-    float* end = ws + static_cast<long long>(1 + n) * p.di;
-    const bool more = k + 1 < tiles;
-    const float dt = more ? ws[0] : 0.0f, e = more ? *end : 0.0f;
-    *end = h;
-    h = fmaf(ex2_approx(dt * an), h, e);
+  float* ws = p.ws + (q.begin / p.chunk + s) * step + c;
+  float an[kCarryStates], h[kCarryStates];
+#pragma unroll
+  for (int i = 0; i < kCarryStates; ++i) {
+    const long long at = static_cast<long long>(min(n0 + i, p.ds - 1)) * p.di;
+    an[i] = p.a[at + c] * 1.4426950408889634f;
+    h[i] = p.state == nullptr || q.fresh ? 0.0f : p.state[q.slot * p.slot_stride + at + c];
+  }
+  for (int k = 0; k < tiles; k += kCarryAhead) {
+    float dt[kCarryAhead], e[kCarryAhead][kCarryStates];
+#pragma unroll
+    for (int j = 0; j < kCarryAhead; ++j) {
+      const bool more = k + j + 1 < tiles;  // the last tile has no summary
+      dt[j] = more ? ws[j * step] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kCarryStates; ++i)
+        e[j][i] = more && n0 + i < p.ds ? ws[j * step + static_cast<long long>(1 + n0 + i) * p.di] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kCarryAhead; ++j) {
+      if (k + j >= tiles) break;
+#pragma unroll
+      for (int i = 0; i < kCarryStates; ++i) {
+        if (n0 + i < p.ds) ws[j * step + static_cast<long long>(1 + n0 + i) * p.di] = h[i];
+        h[i] = fmaf(ex2_approx(dt[j] * an[i]), h[i], e[j][i]);
+      }
+    }
+    ws += kCarryAhead * step;
   }
 }
 
 // Rows of a tile, a power of two: as many tiles as keep about kFillThreads
 // threads (one per channel) on every SM.
-constexpr int kMinChunk = 16, kMaxChunk = 2048, kFillThreads = 512;
+constexpr int kMinChunk = 16, kMaxChunk = 2048, kFillThreads = 768;
 
 int scan_chunk(long long rows, int di) {
   const long long want = rows * di / (static_cast<long long>(kFillThreads) * current_sm_count());
@@ -603,12 +780,14 @@ int scan_typed(const ScanParams& p, cudaStream_t st) {
     return static_cast<int>(cudaGetLastError());
   }
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
-  const std::size_t smem = 2 * static_cast<std::size_t>(scan_stage(p.dr, DS)) * sizeof(float);
+  if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
   if (p.q.rows > p.chunk) {
-    scan_prompt_kernel<T, DS, true><<<grid, kScanWarps * 32, smem, st>>>(p);
-    scan_carry_kernel<<<dim3(static_cast<unsigned>(p.q.n_seq), cb, static_cast<unsigned>(p.ds)), 128, 0, st>>>(p);
+    scan_prompt_kernel<T, DS, true><<<grid, kScanWarps * 32, 0, st>>>(p);
+    scan_carry_kernel<<<dim3(static_cast<unsigned>(p.q.n_seq), cb,
+                             static_cast<unsigned>((p.ds + kCarryStates - 1) / kCarryStates)),
+                        128, 0, st>>>(p);
   }
-  scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, smem, st>>>(p);
+  scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, 0, st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -666,11 +845,21 @@ int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept {
   return with_dtype(a.dtype, [&](auto t) { return conv_typed<decltype(t)>(p, st); });
 }
 
+namespace {
+
+// Bytes of the rows' steps, a whole number of 256 bytes.
+std::size_t steps_bytes(std::size_t rows, std::size_t d_inner) {
+  return (rows * d_inner * sizeof(float) + 255) / 256 * 256;
+}
+
+}  // namespace
+
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept {
   if (a.offsets == nullptr) return 0;
+  const std::size_t steps = steps_bytes(a.rows, a.d_inner);
   const int chunk = scan_chunk(static_cast<long long>(a.rows), static_cast<int>(a.d_inner));
-  if (a.rows <= static_cast<std::uint64_t>(chunk)) return 0;
-  return (a.rows / static_cast<std::uint64_t>(chunk) + a.n_seq) * (1 + a.d_state) * a.d_inner * sizeof(float);
+  if (a.rows <= static_cast<std::uint64_t>(chunk)) return steps;
+  return steps + (a.rows / static_cast<std::uint64_t>(chunk) + a.n_seq) * (1 + a.d_state) * a.d_inner * sizeof(float);
 }
 
 std::size_t selective_scan_workspace_most(std::size_t rows, std::size_t n_seq, std::size_t d_inner,
@@ -682,15 +871,18 @@ std::size_t selective_scan_workspace_most(std::size_t rows, std::size_t n_seq, s
     if (chunk < kMaxChunk) most = std::min(most, 2 * chunk * kFillThreads * current_sm_count() / d_inner + 1);
     tiles = std::max(tiles, most / chunk);
   }
-  return (tiles + n_seq) * (1 + d_state) * d_inner * sizeof(float);
+  return steps_bytes(rows, d_inner) + (tiles + n_seq) * (1 + d_state) * d_inner * sizeof(float);
 }
 
 int launch_selective_scan(const fe_scan_args& a, void* stream) noexcept {
   ScanParams p{sequences(a.offsets, a.slots, a.fresh, a.status, a.rows, a.n_seq, a.n_slots, a.state != nullptr),
                a.u, a.proj, a.z, a.a, a.d, a.dt_w, a.dt_b, a.y, a.state, static_cast<float*>(a.workspace),
-               a.u_ld, a.proj_ld, a.z_ld, a.y_ld, a.slot_stride, static_cast<int>(a.d_inner),
+               static_cast<float*>(a.workspace), a.u_ld, a.proj_ld, a.z_ld, a.y_ld, a.slot_stride, static_cast<int>(a.d_inner),
                static_cast<int>(a.d_state), static_cast<int>(a.dt_rank), 0};
-  if (a.offsets != nullptr) p.chunk = scan_chunk(p.q.rows, p.di);
+  if (a.offsets != nullptr) {
+    p.chunk = scan_chunk(p.q.rows, p.di);
+    p.ws = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + steps_bytes(a.rows, a.d_inner));
+  }
   const auto st = static_cast<cudaStream_t>(stream);
   return with_dtype(a.dtype, [&](auto t) { return scan_sized<decltype(t)>(p, st); });
 }
