@@ -90,11 +90,13 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
     const int c = (lane + i * p.tpr) * VEC;
     if (c < p.dim) {
       Pack<R, VEC> keep;
+      Pack<float, VEC> pw;
+      if (p.post != nullptr) pw = *reinterpret_cast<const Pack<float, VEC>*>(p.post + c);
       if (!kEarly && gate != nullptr) gv[0] = *reinterpret_cast<const Pack<T, VEC>*>(gate + c);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         float t = to_f32(xv[i].v[e]) * mul;
-        if (p.post != nullptr) t *= p.post[c + e];
+        if (p.post != nullptr) t *= pw.v[e];
         if (gate != nullptr) t *= to_f32(gv[kEarly ? i : 0].v[e]);
         const float v = to_f32(rv[i].v[e]) + t;
         keep.v[e] = from_f32<R>(v);
@@ -111,8 +113,9 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
     const int c = (lane + i * p.tpr) * VEC;
     if (c < p.dim) {
       Pack<T, VEC> o;
+      const Pack<float, VEC> w = *reinterpret_cast<const Pack<float, VEC>*>(p.weight + c);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(y[i][e] * norm * p.weight[c + e]);
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(y[i][e] * norm * w.v[e]);
       *reinterpret_cast<Pack<T, VEC>*>(out + c) = o;
     }
   }
@@ -125,7 +128,7 @@ int norm_typed(NormParams p, cudaStream_t st) {
     return reinterpret_cast<std::uintptr_t>(q) % 16 == 0 && ld * static_cast<long long>(e) % 16 == 0;
   };
   const bool wide = p.dim % kVec == 0 && fits(p.x, p.x_ld, sizeof(T)) && fits(p.out, p.out_ld, sizeof(T)) &&
-                    fits(p.residual, p.residual_ld, sizeof(R)) && (p.gate == nullptr || fits(p.gate, p.gate_ld, sizeof(T)));
+                    fits(p.residual, p.residual_ld, sizeof(R)) && (p.gate == nullptr || fits(p.gate, p.gate_ld, sizeof(T))) && fits(p.weight, 0, 4) && fits(p.post, 0, 4);
   const int vecs = wide ? p.dim / kVec : p.dim;
   // few rows: as many threads to a row as it has vectors; many rows: about
   // two vectors to a thread

@@ -37,7 +37,7 @@ struct SeqParams {
 struct Seq {
   long long begin;
   int len;
-  int slot;
+  int slot, bad;
   bool fresh, live;
 };
 
@@ -60,18 +60,15 @@ __device__ int find_sequence(const SeqParams& q, long long tile, int chunk) {
   }
 }
 
-// Bounds, slot and flags of sequence s; every thread of the CTA calls it.
-// live is false for a sequence that is skipped: a negative slot, or one of the
-// faults that set a status bit (offsets outside the rows, a slot outside the
-// pool, a slot that an earlier sequence of the call has).
-// `distinct` false leaves that last test out, for work on a sequence's own
-// buffers.
-__device__ __forceinline__ Seq resolve(const SeqParams& q, int s, bool report, bool distinct = true) {
+// Bounds, slot and flags of sequence s.  live is false for a sequence that is
+// skipped: a negative slot, or a fault (offsets outside the rows, a slot
+// outside the pool), whose status bits are in bad.
+__device__ __forceinline__ Seq resolve(const SeqParams& q, int s) {
   Seq r;
-  int bad = 0;
+  r.bad = 0;
   if (q.offsets != nullptr) {
     const int b = q.offsets[s], e = q.offsets[s + 1];
-    if (b < 0 || e < b || e > q.rows) bad |= FE_SEQ_BAD_OFFSETS;
+    if (b < 0 || e < b || e > q.rows) r.bad |= FE_SEQ_BAD_OFFSETS;
     r.begin = b;
     r.len = e - b;
   } else {
@@ -79,17 +76,23 @@ __device__ __forceinline__ Seq resolve(const SeqParams& q, int s, bool report, b
     r.len = 1;
   }
   r.slot = q.slots != nullptr ? q.slots[s] : s;
-  if (q.stateful && r.slot >= q.n_slots) bad |= FE_SEQ_BAD_SLOT;
+  if (q.stateful && r.slot >= q.n_slots) r.bad |= FE_SEQ_BAD_SLOT;
   r.fresh = q.fresh != nullptr && q.fresh[s] != 0;
-  int dup = 0;
-  if (distinct && q.stateful && q.slots != nullptr && r.slot >= 0) {
-    for (int i = threadIdx.x; i < s; i += blockDim.x) dup |= q.slots[i] == r.slot;
-    dup = __syncthreads_or(dup);
-  }
-  if (dup) bad |= FE_SEQ_DUPLICATE_SLOT;
-  r.live = bad == 0 && r.slot >= 0;
-  if (report && bad != 0 && q.status != nullptr && threadIdx.x == 0) atomicOr(q.status, bad);
+  r.live = r.bad == 0 && r.slot >= 0;
   return r;
+}
+
+// The last test before anything is written: a sequence whose slot an earlier
+// one of the call has is skipped.  Every thread of the CTA calls it; `report`
+// writes the sequence's faults to the status.
+__device__ __forceinline__ bool writes(const SeqParams& q, int s, Seq& r, bool report) {
+  if (q.stateful && q.slots != nullptr && r.slot >= 0) {
+    int dup = 0;
+    for (int i = threadIdx.x; i < s; i += blockDim.x) dup |= q.slots[i] == r.slot;
+    if (__syncthreads_or(dup)) r.bad |= FE_SEQ_DUPLICATE_SLOT;
+  }
+  if (report && r.bad != 0 && q.status != nullptr && threadIdx.x == 0) atomicOr(q.status, r.bad);
+  return r.bad == 0 && r.slot >= 0;
 }
 
 // The first CTA of a grid also reports offsets that no tile can be found by:
@@ -103,125 +106,6 @@ __device__ void report_offsets(const SeqParams& q) {
   }
   if (bad) atomicOr(q.status, FE_SEQ_BAD_OFFSETS);
 }
-
-// --- causal convolution -------------------------------------------------------
-
-struct ConvParams {
-  SeqParams q;
-  const void* x;
-  const float* w;  // [di][dc]
-  const float* b;  // [di]
-  void* u;
-  float* window;  // [slot][di][dc], the last dc inputs, newest last
-  long long x_ld, u_ld, slot_stride;
-  int di, dc, chunk;
-};
-
-// One thread per (token, channel): shift the window, append x, dot, SiLU.
-// Bound by the window's bytes.
-template <typename T>
-__global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
-  const int s = blockIdx.x;
-  const Seq q = resolve(p.q, s, blockIdx.y == 0);
-  const int c = blockIdx.y * blockDim.x + threadIdx.x;
-  if (!q.live || c >= p.di) return;
-  const float xv = to_f32(static_cast<const T*>(p.x)[s * p.x_ld + c]);
-  const float* w = p.w + static_cast<long long>(c) * p.dc;
-  float* win = p.window == nullptr ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * p.dc;
-  float acc = p.b[c];
-  for (int k = 0; k + 1 < p.dc; ++k) {
-    const float v = win == nullptr || q.fresh ? 0.0f : win[k + 1];
-    if (win != nullptr) win[k] = v;
-    acc = fmaf(w[k], v, acc);
-  }
-  if (win != nullptr) win[p.dc - 1] = xv;
-  acc = fmaf(w[p.dc - 1], xv, acc);
-  static_cast<T*>(p.u)[s * p.u_ld + c] = from_f32<T>(silu_f(acc));
-}
-
-// One thread per channel walks the tile's rows with the last DC inputs in
-// registers (right-aligned: taps before the first of dc carry weight zero).
-// The first tile of a sequence reads the old window and writes the new one
-// from the sequence's last rows, so no other tile touches it.
-template <typename T, int DC>
-__global__ void __launch_bounds__(128) conv_prompt_kernel(const ConvParams p) {
-  report_offsets(p.q);
-  const int s = find_sequence(p.q, blockIdx.x, p.chunk);
-  if (s < 0) return;
-  const Seq q = resolve(p.q, s, blockIdx.y == 0);
-  const long long k = blockIdx.x - (q.begin / p.chunk + s);
-  const int c = blockIdx.y * blockDim.x + threadIdx.x;
-  if (!q.live || c >= p.di || (k > 0 && k * p.chunk >= q.len)) return;
-  const int t0 = static_cast<int>(k * p.chunk);
-  const T* x = static_cast<const T*>(p.x) + q.begin * p.x_ld + c;
-  T* u = static_cast<T*>(p.u) + q.begin * p.u_ld + c;
-  float* win = p.window == nullptr ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * p.dc;
-  float wk[DC], in[DC];
-#pragma unroll
-  for (int j = 0; j < DC; ++j) {
-    const int tap = j - (DC - p.dc);
-    wk[j] = tap >= 0 ? p.w[static_cast<long long>(c) * p.dc + tap] : 0.0f;
-    const int t = t0 - DC + j;  // the input that slot j holds before row t0
-    in[j] = 0.0f;
-    if (t >= 0)
-      in[j] = to_f32(x[t * p.x_ld]);
-    else if (win != nullptr && !q.fresh && p.dc + t >= 0)
-      in[j] = win[p.dc + t];
-  }
-  const float bias = p.b[c];
-  if (k == 0 && win != nullptr) {
-    for (int j = 0; j < p.dc; ++j) {
-      const int t = q.len - p.dc + j;
-      win[j] = t >= 0 ? to_f32(x[t * p.x_ld]) : (q.fresh ? 0.0f : win[p.dc + t]);
-    }
-  }
-  const int t1 = min(t0 + p.chunk, q.len);
-  constexpr int kAhead = 8;
-  for (int t = t0; t < t1; t += kAhead) {
-    float v[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = t + i < t1 ? to_f32(x[(t + i) * p.x_ld]) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-#pragma unroll
-      for (int j = 0; j + 1 < DC; ++j) in[j] = in[j + 1];
-      in[DC - 1] = v[i];
-      float acc = bias;
-#pragma unroll
-      for (int j = 0; j < DC; ++j) acc = fmaf(wk[j], in[j], acc);
-      if (t + i < t1) u[(t + i) * p.u_ld] = from_f32<T>(silu_f(acc));
-    }
-  }
-}
-
-template <typename T>
-int conv_typed(const ConvParams& p, cudaStream_t st) {
-  const unsigned cb = static_cast<unsigned>((p.di + 127) / 128);
-  if (p.q.offsets == nullptr) {
-    conv_token_kernel<T><<<dim3(static_cast<unsigned>(p.q.n_seq), cb), 128, 0, st>>>(p);
-    return static_cast<int>(cudaGetLastError());
-  }
-  const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
-  if (p.dc <= 4)
-    conv_prompt_kernel<T, 4><<<grid, 128, 0, st>>>(p);
-  else
-    conv_prompt_kernel<T, 8><<<grid, 128, 0, st>>>(p);
-  return static_cast<int>(cudaGetLastError());
-}
-
-// --- selective scan -----------------------------------------------------------
-
-struct ScanParams {
-  SeqParams q;
-  const void *u, *proj, *z;
-  const float *a, *d, *dt_w, *dt_b;  // a [ds][di], dt_w [dr][di]
-  void* y;
-  float* state;  // [slot][ds][di]
-  float* steps;  // [rows][di], dt of every row (prompts)
-  float* ws;     // [tile][1 + ds][di]: sum of dt, then the tile's state (its end from zero; later its start)
-  long long u_ld, proj_ld, z_ld, y_ld, slot_stride;
-  int di, ds, dr, chunk;
-};
 
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
@@ -240,6 +124,249 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// SiLU of a pair: x / (1 + 2^(-x log2 e)) by the hardware's power and
+// reciprocal (relative error a few steps of fp32, and one more for every unit
+// of |x|; -0 below -88, the limit)
+__device__ __forceinline__ float2 silu2(float2 x) {
+  const float2 t = __fmul2_rn(x, splat(-1.4426950408889634f));
+  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), splat(1.0f));
+  return __fmul2_rn(x, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+__device__ __forceinline__ float silu1(float x) {
+  return x * rcp_approx(1.0f + ex2_approx(x * -1.4426950408889634f));
+}
+
+// --- causal convolution -------------------------------------------------------
+
+struct ConvParams {
+  SeqParams q;
+  const void* x;
+  const float* w;  // [di][dc]
+  const float* b;  // [di]
+  void* u;
+  float* window;  // [slot][di][dc], the last dc inputs, newest last
+  long long x_ld, u_ld, slot_stride;
+  int di, dc, chunk;
+};
+
+// One thread per (token, channel): shift the window, append x, dot, SiLU.
+// Bound by the window's bytes.  FOUR: four taps and windows on 16-byte
+// boundaries, one load and one store each.
+template <typename T, bool FOUR>
+__global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
+  const int s = blockIdx.x;
+  Seq q = resolve(p.q, s);
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool on = c < p.di && q.live;
+  float* win = p.window == nullptr || !on ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * p.dc;
+  const bool held = win != nullptr && !q.fresh;
+  const int dc = FOUR ? 4 : p.dc;
+  float v[8], xv = 0.0f;  // v[j]: tap j's input, the newest (x) last
+  if constexpr (FOUR) {
+    const float4 o = held ? *reinterpret_cast<const float4*>(win) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    v[0] = o.y;
+    v[1] = o.z;
+    v[2] = o.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = held && j + 1 < dc ? win[j + 1] : 0.0f;
+  }
+  if (on) xv = to_f32(static_cast<const T*>(p.x)[s * p.x_ld + c]);
+  if (!writes(p.q, s, q, blockIdx.y == 0) || !on) return;
+  const float* w = p.w + static_cast<long long>(c) * dc;
+  float acc = p.b[c];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= dc) break;
+    if (j == dc - 1) v[j] = xv;
+    acc = fmaf(w[j], v[j], acc);
+  }
+  static_cast<T*>(p.u)[s * p.u_ld + c] = from_f32<T>(silu1(acc));
+  if (win == nullptr) return;
+  if constexpr (FOUR) {
+    *reinterpret_cast<float4*>(win) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < dc) win[j] = v[j];
+  }
+}
+
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T v[V];
+};
+
+// One thread walks V channels of a tile's rows, two and two (V 1: a pair with
+// an idle half), with their last DC inputs in registers (right-aligned: taps
+// before the first of dc carry weight zero), kAhead rows requested before
+// their arithmetic.  The first tile of a sequence reads the old window and
+// writes the new one from the sequence's last rows, so no other tile touches
+// it.  Bound by x and u, read and written once (a tile reads DC - 1 rows
+// before its own again, from L2).
+template <typename T, int DC, int V>
+__global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p) {
+  constexpr int kPairs = (V + 1) / 2, kAhead = 8;
+  constexpr int kLines = (32 * V * static_cast<int>(sizeof(T)) + 127) / 128;  // of a row, for a warp
+  const int lane = threadIdx.x & 31;
+  report_offsets(p.q);
+  const int s = find_sequence(p.q, blockIdx.x, p.chunk);
+  if (s < 0) return;
+  Seq q = resolve(p.q, s);
+  const long long k = blockIdx.x - (q.begin / p.chunk + s);
+  if (!q.live && q.bad == 0) return;                         // a padded sequence
+  if (q.bad == 0 && k > 0 && k * p.chunk >= q.len) return;  // no such tile
+  const int t0 = static_cast<int>(k * p.chunk);
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const bool on = c < p.di && q.live;
+  const T* x = static_cast<const T*>(p.x) + q.begin * p.x_ld + c;
+  float* win = p.window == nullptr ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * p.dc;
+  const int t1 = on ? min(t0 + p.chunk, q.len) : t0;
+  using Row = Vec<T, V>;
+  auto pair = [](const Row& r, int e) {
+    return make_float2(to_f32(r.v[2 * e]), 2 * e + 1 < V ? to_f32(r.v[V > 1 ? 2 * e + 1 : 0]) : 0.0f);
+  };
+  Row ahead[kAhead];
+  const T* next = x + t0 * p.x_ld;
+  auto request = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (t + i < t1) ahead[i] = *reinterpret_cast<const Row*>(next + i * p.x_ld);
+    next += kAhead * p.x_ld;
+  };
+  request(t0);
+  // the rows after these into L2: a lane one line of one row
+  for (int e = lane; e < (t1 - t0 - kAhead) * kLines; e += 32) {
+    const int at = c + (e % kLines * (128 / static_cast<int>(sizeof(T))) - lane * V);
+    if (at < p.di) prefetch_l2(static_cast<const T*>(p.x) + (q.begin + t0 + kAhead + e / kLines) * p.x_ld + at);
+  }
+  float2 wk[DC][kPairs], in[DC][kPairs], bias[kPairs];
+  float w[DC][2 * kPairs];
+  if (on) {
+#pragma unroll
+    for (int e = 0; e < 2 * kPairs; ++e) {
+      const int ce = e < V ? c + e : c;
+      const float* src = p.w + static_cast<long long>(ce) * p.dc;
+      (e & 1 ? bias[e / 2].y : bias[e / 2].x) = p.b[ce];
+      if constexpr (V > 1 && DC == 4) {
+        if (p.dc == 4) {  // on 16 bytes (conv_prompts)
+          const float4 w4 = *reinterpret_cast<const float4*>(src);
+          w[0][e] = w4.x;
+          w[1][e] = w4.y;
+          w[2][e] = w4.z;
+          w[3][e] = w4.w;
+          continue;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < DC; ++j) w[j][e] = j >= DC - p.dc ? src[j - (DC - p.dc)] : 0.0f;
+    }
+  }
+  Row halo[DC];
+#pragma unroll
+  for (int j = 1; j < DC; ++j)
+    if (on && t0 >= DC) halo[j] = *reinterpret_cast<const Row*>(x + (t0 - DC + j) * p.x_ld);
+  // every request is on its way: only now the test that waits
+  if (!writes(p.q, s, q, blockIdx.y == 0) || !on) return;
+#pragma unroll
+  for (int j = 0; j < DC; ++j) {
+    const int t = t0 - DC + j;  // the input that place j holds before row t0; place 0 is shifted out unused
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) {
+      wk[j][e] = make_float2(w[j][2 * e], w[j][2 * e + 1]);
+      in[j][e] = j > 0 && t0 >= DC ? pair(halo[j], e) : splat(0.0f);
+    }
+    // (a tile's first row is a multiple of the chunk, so that t0 is 0 or at least DC)
+    if (j > 0 && t0 == 0 && win != nullptr && !q.fresh && p.dc + t >= 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) (e & 1 ? in[j][e / 2].y : in[j][e / 2].x) = win[e * p.dc + p.dc + t];
+    }
+  }
+  if (k == 0 && win != nullptr) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      for (int j = 0; j < p.dc; ++j) {
+        const int t = q.len - p.dc + j;
+        win[e * p.dc + j] = t >= 0 ? to_f32(x[t * p.x_ld + e]) : (q.fresh ? 0.0f : win[e * p.dc + p.dc + t]);
+      }
+  }
+  T* u = static_cast<T*>(p.u) + (q.begin + t0) * p.u_ld + c;
+  for (int t = t0; t < t1; t += kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t + i >= t1) break;
+      Row out;
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) {
+#pragma unroll
+        for (int j = 0; j + 1 < DC; ++j) in[j][e] = in[j + 1][e];
+        in[DC - 1][e] = pair(ahead[i], e);
+        float2 acc = bias[e];
+#pragma unroll
+        for (int j = 0; j < DC; ++j) acc = __ffma2_rn(wk[j][e], in[j][e], acc);
+        acc = silu2(acc);
+        out.v[2 * e] = from_f32<T>(acc.x);
+        if (2 * e + 1 < V) out.v[V > 1 ? 2 * e + 1 : 0] = from_f32<T>(acc.y);
+      }
+      *reinterpret_cast<Row*>(u + i * p.u_ld) = out;
+    }
+    u += kAhead * p.u_ld;
+    request(t + kAhead);
+  }
+}
+
+template <typename T, int DC>
+int conv_prompts(ConvParams p, cudaStream_t st) {
+  // 16 bytes of a row to a thread where its rows allow it (at most four
+  // channels, and two of eight taps, which take the registers)
+  constexpr int kVec = DC > 4 ? 2 : 4;
+  const auto fits = [&](const void* q, long long ld) {
+    return reinterpret_cast<std::uintptr_t>(q) % (kVec * sizeof(T)) == 0 && ld % kVec == 0;
+  };
+  const bool wide = p.di % kVec == 0 && fits(p.x, p.x_ld) && fits(p.u, p.u_ld) &&
+                    reinterpret_cast<std::uintptr_t>(p.w) % 16 == 0;
+  const int threads = wide ? p.di / kVec : p.di;  // for a row
+  const unsigned block = static_cast<unsigned>(std::min(128, (threads + 31) / 32 * 32));
+  const long long across = (threads + block - 1) / block;
+  // rows to a tile: as few as let every tile be resident at once (five CTAs to
+  // an SM; half of the sequences' last tiles are extra), from 8 to 64.
+  // Measured at 96 prompts of 12289 rows x 1024: 16 rows 25.0 us, 24 23.8,
+  // 40 (this rule) 21.1, 64 25.8
+  const long long resident = std::max(1LL, 5LL * current_sm_count() / across - p.q.n_seq / 2);
+  p.chunk = static_cast<int>(std::clamp((p.q.rows / resident + 7) / 8 * 8, 8LL, 64LL));
+  const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), static_cast<unsigned>(across));
+  if (wide)
+    conv_prompt_kernel<T, DC, kVec><<<grid, block, 0, st>>>(p);
+  else
+    conv_prompt_kernel<T, DC, 1><<<grid, block, 0, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int conv_typed(const ConvParams& p, cudaStream_t st) {
+  if (p.q.offsets != nullptr) return p.dc <= 4 ? conv_prompts<T, 4>(p, st) : conv_prompts<T, 8>(p, st);
+  const dim3 grid(static_cast<unsigned>(p.q.n_seq), static_cast<unsigned>((p.di + 127) / 128));
+  if (p.dc == 4 && reinterpret_cast<std::uintptr_t>(p.window) % 16 == 0 && p.slot_stride % 4 == 0)
+    conv_token_kernel<T, true><<<grid, 128, 0, st>>>(p);
+  else
+    conv_token_kernel<T, false><<<grid, 128, 0, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// --- selective scan -----------------------------------------------------------
+
+struct ScanParams {
+  SeqParams q;
+  const void *u, *proj, *z;
+  const float *a, *d, *dt_w, *dt_b;  // a [ds][di], dt_w [dr][di]
+  void* y;
+  float* state;  // [slot][ds][di]
+  float* steps;  // [rows][di], dt of every row (prompts)
+  float* ws;     // [tile][1 + ds][di]: sum of dt, then the tile's state (its end from zero; later its start)
+  long long u_ld, proj_ld, z_ld, y_ld, slot_stride;
+  int di, ds, dr, chunk;
+};
 
 // softplus of a pair to a few ulp of the result: e = exp(-|x|) with the
 // rounding error of |x| log2(e) carried into the exponential, log(1 + e) =
@@ -266,15 +393,17 @@ __device__ __forceinline__ float2 softplus_rel2(float2 x) {
 }
 __device__ __forceinline__ float softplus_rel(float x) { return softplus_rel2(splat(x)).x; }
 
-// One token for each of up to RT sequences, one thread per channel.  The dt
-// projection's weights are read once for the RT tokens; then each sequence's
-// ds states are read, stepped and written (the kernel's bytes).
-template <typename T, int DS, int RT>
+// One token for each of up to RT sequences; a thread has V neighbouring
+// channels, as a pair (V 1: the second is idle).  The dt projection's weights
+// are read once for the RT tokens; then each sequence's ds states are read,
+// stepped and written, which are the kernel's bytes.  Arithmetic on the two
+// channels at once (FFMA2).
+template <typename T, int DS, int RT, int V>
 __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
-  extern __shared__ float sp[];  // [RT][dr + 2 ds]
+  extern __shared__ __align__(16) float sp[];  // dt_in [dr][RT], then per row [B (DS) | C (DS)], zero behind ds
   __shared__ int sdup;
-  const int s0 = blockIdx.x * RT, c = blockIdx.y * 128 + threadIdx.x;
-  const int wd = p.dr + 2 * p.ds;
+  const int s0 = blockIdx.x * RT, c = (blockIdx.y * 128 + threadIdx.x) * V;
+  const int ds = p.ds, dr = p.dr, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int slot[RT], bad[RT];
   bool fresh[RT];
 #pragma unroll
@@ -285,10 +414,26 @@ __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
     bad[j] = p.q.stateful && slot[j] >= p.q.n_slots ? FE_SEQ_BAD_SLOT : 0;
   }
   if (threadIdx.x == 0) sdup = 0;
-  for (int i = threadIdx.x; i < RT * wd; i += 128) {
-    const int j = i / wd;
-    if (s0 + j < p.q.n_seq)
-      sp[i] = to_f32(static_cast<const T*>(p.proj)[(s0 + j) * p.proj_ld + (i - j * wd)]);
+  // the states of all RT tokens into L2 while the projection runs: a lane one
+  // line of 32 of the warp's 32 V channels
+  if (p.state != nullptr)
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+      if (slot[j] >= 0 && bad[j] == 0 && !fresh[j])
+        for (int e = lane; e < ds * V; e += 32) {
+          const int at = c - lane * V + e % V * 32;
+          if (at < p.di) prefetch_l2(p.state + slot[j] * p.slot_stride + static_cast<long long>(e / V) * p.di + at);
+        }
+  float* const sbc = sp + (dr * RT + 3) / 4 * 4;  // on 16 bytes
+  for (int j = RT == 1 ? 0 : warp; j < RT; j += 4) {
+    const T* row = static_cast<const T*>(p.proj) + static_cast<long long>(s0 + j) * p.proj_ld;
+    const bool have = s0 + j < p.q.n_seq;
+    const int first = RT == 1 ? threadIdx.x : lane, step = RT == 1 ? 128 : 32;
+    for (int e = first; e < dr; e += step) sp[e * RT + j] = have ? to_f32(row[e]) : 0.0f;
+    for (int e = first; e < 2 * DS; e += step) {
+      const int n = e % DS;
+      sbc[j * 2 * DS + e] = have && n < ds ? to_f32(row[dr + (e < DS ? n : ds + n)]) : 0.0f;
+    }
   }
   __syncthreads();
   if (p.q.stateful && p.q.slots != nullptr) {
@@ -309,43 +454,88 @@ __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
     if (bad[j] != 0) slot[j] = -1;
   }
   if (c >= p.di) return;
-  float acc[RT];
+  auto load2 = [](const float* at) {
+    if constexpr (V == 2)
+      return *reinterpret_cast<const float2*>(at);
+    else
+      return make_float2(*at, 0.0f);
+  };
+  auto read2 = [](const void* base, long long at) {
+    const T* q = static_cast<const T*>(base) + at;
+    if constexpr (V == 2) {
+      const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(q);
+      return make_float2(to_f32(v.v[0]), to_f32(v.v[1]));
+    } else {
+      return make_float2(to_f32(*q), 0.0f);
+    }
+  };
+  float2 acc[RT];
+  const float2 bdt = load2(p.dt_b + c);
 #pragma unroll
-  for (int j = 0; j < RT; ++j) acc[j] = 0.0f;
+  for (int j = 0; j < RT; ++j) acc[j] = bdt;
+  const float* w = p.dt_w + c;
 #pragma unroll 8
-  for (int r = 0; r < p.dr; ++r) {
-    const float w = p.dt_w[static_cast<long long>(r) * p.di + c];
-#pragma unroll
-    for (int j = 0; j < RT; ++j) acc[j] = fmaf(sp[j * wd + r], w, acc[j]);
+  for (int r = 0; r < dr; ++r, w += p.di) {
+    const float2 wv = load2(w);
+    if constexpr (RT == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(sp + r * 4);
+      acc[0] = __ffma2_rn(wv, splat(v.x), acc[0]);
+      acc[1] = __ffma2_rn(wv, splat(v.y), acc[1]);
+      acc[2] = __ffma2_rn(wv, splat(v.z), acc[2]);
+      acc[3] = __ffma2_rn(wv, splat(v.w), acc[3]);
+    } else {
+      acc[0] = __ffma2_rn(wv, splat(sp[r]), acc[0]);
+    }
   }
-  float an[DS];
+  float2 an[DS];
+  {
+    const float* a = p.a + c;
 #pragma unroll
-  for (int n = 0; n < DS; ++n) an[n] = n < p.ds ? p.a[static_cast<long long>(n) * p.di + c] * 1.4426950408889634f : 0.0f;
-  const float bdt = p.dt_b[c], dk = p.d[c];
+    for (int n = 0; n < DS; ++n, a += p.di) an[n] = n < ds ? __fmul2_rn(load2(a), splat(1.4426950408889634f)) : splat(0.0f);
+  }
+  const float2 dk = load2(p.d + c);
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     if (slot[j] < 0) continue;
-    float* st = p.state == nullptr ? nullptr : p.state + slot[j] * p.slot_stride + c;
-    float h[DS];
+    float* const st = p.state == nullptr ? nullptr : p.state + slot[j] * p.slot_stride + c;
+    const bool held = st != nullptr && !fresh[j];
+    float2 h[DS];
+    const float* from = st;
 #pragma unroll
-    for (int n = 0; n < DS; ++n)
-      h[n] = st != nullptr && !fresh[j] && n < p.ds ? st[static_cast<long long>(n) * p.di] : 0.0f;
-    const float uv = to_f32(static_cast<const T*>(p.u)[(s0 + j) * p.u_ld + c]);
-    const float dt = softplus_rel(acc[j] + bdt), dtu = dt * uv;
-    const float* row = sp + j * wd + p.dr;
-    float y = dk * uv;
-#pragma unroll
-    for (int n = 0; n < DS; ++n) {
-      if (n >= p.ds) break;
-      h[n] = fmaf(ex2_approx(dt * an[n]), h[n], dtu * row[n]);
-      y = fmaf(h[n], row[p.ds + n], y);
-      if (st != nullptr) st[static_cast<long long>(n) * p.di] = h[n];
-    }
+    for (int n = 0; n < DS; ++n, from += p.di) h[n] = held && n < ds ? load2(from) : splat(0.0f);
+    const float2 uv = read2(p.u, (s0 + j) * p.u_ld + c);
+    float2 gate = splat(1.0f);
     if (p.z != nullptr) {
-      const float zv = to_f32(static_cast<const T*>(p.z)[(s0 + j) * p.z_ld + c]);
-      y *= silu_f(zv);
+      const float2 zv = read2(p.z, (s0 + j) * p.z_ld + c);
+      gate = silu2(zv);
     }
-    static_cast<T*>(p.y)[(s0 + j) * p.y_ld + c] = from_f32<T>(y);
+    const float2 dt = softplus_rel2(acc[j]), dtu = __fmul2_rn(dt, uv);
+    float2 y = __fmul2_rn(dk, uv);
+    float* to = st;
+#pragma unroll
+    for (int n = 0; n < DS; n += 4) {
+      const float4 bq = *reinterpret_cast<const float4*>(sbc + j * 2 * DS + n);
+      const float4 cq = *reinterpret_cast<const float4*>(sbc + j * 2 * DS + DS + n);
+      const float bn[4] = {bq.x, bq.y, bq.z, bq.w}, cn[4] = {cq.x, cq.y, cq.z, cq.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i, to += p.di) {
+        const float2 e = __fmul2_rn(dt, an[n + i]);
+        const float2 hn = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), h[n + i], __fmul2_rn(dtu, splat(bn[i])));
+        y = __ffma2_rn(hn, splat(cn[i]), y);
+        if (st != nullptr && n + i < ds) {
+          if constexpr (V == 2)
+            *reinterpret_cast<float2*>(to) = hn;
+          else
+            *to = hn.x;
+        }
+      }
+    }
+    y = __fmul2_rn(y, gate);
+    T* out = static_cast<T*>(p.y) + (s0 + j) * p.y_ld + c;
+    if constexpr (V == 2)
+      *reinterpret_cast<Vec<T, 2>*>(out) = Vec<T, 2>{{from_f32<T>(y.x), from_f32<T>(y.y)}};
+    else
+      *out = from_f32<T>(y.x);
   }
 }
 
@@ -545,8 +735,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
   if (!SUMMARY) report_offsets(p.q);
   const int s = find_sequence(p.q, blockIdx.x, p.chunk);
   if (s < 0) return;
-  const Seq q = resolve(p.q, s, !SUMMARY && blockIdx.y == 0, !SUMMARY);
+  Seq q = resolve(p.q, s);
   const long long k = blockIdx.x - (q.begin / p.chunk + s);
+  // (a summary is its sequence's own, whoever else has the slot)
+  if (!SUMMARY && !writes(p.q, s, q, blockIdx.y == 0)) return;
   if (!q.live || (k > 0 && k * p.chunk >= q.len)) return;
   const int t0 = static_cast<int>(k * p.chunk);
   const bool last = t0 + p.chunk >= q.len;
@@ -657,7 +849,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
     }
     const float2 sum = __fadd2_rn(y0, y1);
     const float yv = sum.x + sum.y;
-    return gated ? yv * silu_fast(zv) : yv;
+    return gated ? yv * silu1(zv) : yv;
   };
   settle(0);
   for (int t = 0, b = 0; t < rows; t += kStage, b ^= 1) {
@@ -721,7 +913,7 @@ constexpr int kCarryStates = 2, kCarryAhead = 4;
 __global__ void __launch_bounds__(128) scan_carry_kernel(const ScanParams p) {
   const int s = blockIdx.x, n0 = blockIdx.z * kCarryStates;
   if (p.q.offsets[s + 1] - p.q.offsets[s] <= p.chunk) return;
-  const Seq q = resolve(p.q, s, false, false);
+  const Seq q = resolve(p.q, s);
   const int c = blockIdx.y * 128 + threadIdx.x;
   if (!q.live || c >= p.di) return;
   const int tiles = (q.len + p.chunk - 1) / p.chunk;
@@ -768,16 +960,33 @@ int scan_chunk(long long rows, int di) {
   return chunk;
 }
 
+// Pairs of channels where the matrices and slots allow it, and four tokens to
+// a CTA (one reading of dt_w) once that leaves four CTAs for every SM.
+template <typename T, int DS>
+int scan_tokens(const ScanParams& p, cudaStream_t st) {
+  const auto even = [](const void* q, long long ld, std::size_t e) {
+    return reinterpret_cast<std::uintptr_t>(q) % (2 * e) == 0 && ld % 2 == 0;
+  };
+  const bool pairs = p.di % 2 == 0 && even(p.u, p.u_ld, sizeof(T)) && even(p.y, p.y_ld, sizeof(T)) &&
+                     even(p.z, p.z_ld, sizeof(T)) && even(p.state, p.slot_stride, 4) && even(p.a, 0, 4) &&
+                     even(p.d, 0, 4) && even(p.dt_w, 0, 4) && even(p.dt_b, 0, 4);
+  const unsigned cb = static_cast<unsigned>((p.di + (pairs ? 255 : 127)) / (pairs ? 256 : 128));
+  const bool four = (p.q.n_seq + 3LL) / 4 * cb >= 4LL * current_sm_count();
+  const dim3 grid(static_cast<unsigned>(four ? (p.q.n_seq + 3) / 4 : p.q.n_seq), cb);
+  const std::size_t rt = four ? 4 : 1;
+  const std::size_t smem = ((p.dr * rt + 3) / 4 * 4 + 2 * DS * rt) * sizeof(float);
+  if (four)
+    pairs ? scan_token_kernel<T, DS, 4, 2><<<grid, 128, smem, st>>>(p) : scan_token_kernel<T, DS, 4, 1><<<grid, 128, smem, st>>>(p);
+  else
+    pairs ? scan_token_kernel<T, DS, 1, 2><<<grid, 128, smem, st>>>(p) : scan_token_kernel<T, DS, 1, 1><<<grid, 128, smem, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
 template <typename T, int DS>
 int scan_typed(const ScanParams& p, cudaStream_t st) {
   const unsigned cb = static_cast<unsigned>((p.di + 127) / 128);
-  const std::size_t row = static_cast<std::size_t>(p.dr + 2 * p.ds) * sizeof(float);
   if (p.q.offsets == nullptr) {
-    if (static_cast<long long>(p.q.n_seq) * cb >= 8LL * current_sm_count())
-      scan_token_kernel<T, DS, 4><<<dim3(static_cast<unsigned>((p.q.n_seq + 3) / 4), cb), 128, 4 * row, st>>>(p);
-    else
-      scan_token_kernel<T, DS, 1><<<dim3(static_cast<unsigned>(p.q.n_seq), cb), 128, row, st>>>(p);
-    return static_cast<int>(cudaGetLastError());
+    return scan_tokens<T, DS>(p, st);
   }
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
   if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
@@ -840,7 +1049,7 @@ int current_sm_count() noexcept {
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept {
   ConvParams p{sequences(a.offsets, a.slots, a.fresh, a.status, a.rows, a.n_seq, a.n_slots, a.window != nullptr),
                a.x, a.w, a.b, a.u, a.window, a.x_ld, a.u_ld, a.slot_stride, static_cast<int>(a.d_inner),
-               static_cast<int>(a.d_conv), 32};
+               static_cast<int>(a.d_conv), 0};
   const auto st = static_cast<cudaStream_t>(stream);
   return with_dtype(a.dtype, [&](auto t) { return conv_typed<decltype(t)>(p, st); });
 }
