@@ -10,8 +10,8 @@
 // terms that add up to its 24 bits (fp32).
 //
 // Bound by the weights' bytes for few rows; a warp reads 16 weight rows x 64
-// bytes per step, and the k range is split over the warps of a CTA where there
-// are too few rows of weights to fill the GPU.
+// bytes per block of k, and the blocks are dealt out to several warps where
+// there are too few rows of weights to fill the GPU.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,7 +25,6 @@
 namespace feb {
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kBlock = 128;  // elements of a packed block of 64 bytes
 
 struct W4Params {
@@ -78,6 +77,18 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&v)[4]) {
 template <typename T, int TERMS>
 __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0, int blocks, unsigned short* sx, int stride) {
   const int width = blocks * kBlock, first = b0 * kBlock;
+  if constexpr (TERMS == 1) {
+    // whole 16 bytes as they are, where rows start on them and k ends there
+    if (p.k % 8 == 0 && p.x_ld % 8 == 0 && reinterpret_cast<std::uintptr_t>(p.x) % 16 == 0) {
+      for (int i = threadIdx.x; i < n * (width / 8); i += blockDim.x) {
+        const int r = i / (width / 8), c = (i - r * (width / 8)) * 8;
+        const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first + c;
+        const uint4 v = first + c < p.k ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(sx + r * stride + c) = v;
+      }
+      return;
+    }
+  }
   for (int i = threadIdx.x; i < n * (width / 2); i += blockDim.x) {
     const int r = i / (width / 2), c = (i - r * (width / 2)) * 2;
     const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first + c;
@@ -105,83 +116,120 @@ __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0
 // that the eight rows of a fragment fall into different banks
 __host__ __device__ constexpr int stage_stride(int blocks) { return blocks * kBlock + 32; }
 
+// A CTA has 4 or 8 warps: p.kw of them share a tile of 16 weight rows, each with
+// a run of the blocks of k, and join their sums through shared memory in
+// order.  A warp has kSet blocks in its arithmetic and the next kSet on their
+// way; a last odd block and one whose last groups do not exist come one by one.
 template <typename T, int NT, int GROUP>
-__global__ void __launch_bounds__(kWarps * 32) w4_matvec_kernel(const W4Params p) {
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) w4_matvec_kernel(const W4Params p) {
   constexpr bool kBf16 = !std::is_same_v<T, __half>;
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
+  constexpr int kPer = kBlock / GROUP, kPieces = 4 / kPer;  // groups of a block, 32-element pieces of a group
+  constexpr int kSet = NT == 1 ? 2 : 1;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int rw = kWarps / p.kw, wk = warp % p.kw, wr = warp / p.kw;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rw = warps / p.kw, wk = warp % p.kw, wr = warp / p.kw;
   const int m0 = (blockIdx.x * rw + wr) * 16;
   const int r0 = blockIdx.y * NT * 8, n = min(NT * 8, p.rows - r0);
   unsigned short* sx = reinterpret_cast<unsigned short*>(smem);
   const int stride = stage_stride(p.stage);
-  // rows behind the last read the last one and are not written
+  // weight rows behind the last read the last one, columns of x behind the
+  // last the last one: their sums are not written
   const int ra = min(m0 + g, p.m - 1), rb = min(m0 + g + 8, p.m - 1);
-  const uint4* wa = p.packed + static_cast<long long>(ra) * p.blocks * 4 + t;
-  const uint4* wb = p.packed + static_cast<long long>(rb) * p.blocks * 4 + t;
-  const __half* sa = p.scales + static_cast<long long>(ra) * p.groups;
-  const __half* sb = p.scales + static_cast<long long>(rb) * p.groups;
   float acc[NT][4] = {};
-  constexpr int kPer = kBlock / GROUP;  // groups of a block
+  struct Block {
+    uint4 a, b;
+    __half sa[kPer], sb[kPer];
+  };
   for (int b0 = 0; b0 < p.blocks; b0 += p.stage) {
-    const int nb = min(p.stage, p.blocks - b0);
-    if (b0 > 0) __syncthreads();
-    stage_x<T, kTerms>(p, r0, n, b0, nb, sx, stride);
-    __syncthreads();
-    constexpr int kAhead = 4;
-    for (int b = wk; b < nb; b += p.kw * kAhead) {
-      uint4 qa[kAhead], qb[kAhead];
-      __half ha[kAhead][kPer], hb[kAhead][kPer];
+    // this warp's blocks of the stage: [first, end), with all of their groups up to `whole`
+    const int nb = min(p.stage, p.blocks - b0), share = (nb + p.kw - 1) / p.kw;
+    const int first = min(wk * share, nb), end = min(first + share, nb);
+    const int whole = max(first, min(end, p.groups / kPer - b0));
+    const uint4* wa = p.packed + (static_cast<long long>(ra) * p.blocks + b0 + first) * 4 + t;
+    const uint4* wb = p.packed + (static_cast<long long>(rb) * p.blocks + b0 + first) * 4 + t;
+    const __half* sa = p.scales + static_cast<long long>(ra) * p.groups + (b0 + first) * kPer;
+    const __half* sb = p.scales + static_cast<long long>(rb) * p.groups + (b0 + first) * kPer;
+    auto request = [&](Block& blk, int i, int groups) {  // block i from the pointers
+      blk.a = __ldg(wa + i * 4);
+      blk.b = __ldg(wb + i * 4);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int blk = b0 + min(b + i * p.kw, nb - 1);
-        qa[i] = __ldg(wa + blk * 4);
-        qb[i] = __ldg(wb + blk * 4);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int grp = min(blk * kPer + j, p.groups - 1);
-          ha[i][j] = sa[grp];
-          hb[i][j] = sb[grp];
-        }
+      for (int j = 0; j < kPer; ++j) {
+        blk.sa[j] = j < groups ? sa[i * kPer + j] : __half(0.0f);
+        blk.sb[j] = j < groups ? sb[i * kPer + j] : __half(0.0f);
       }
+    };
+    const unsigned short* xs[NT];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (b + i * p.kw >= nb) break;
-        const uint32_t ua[4] = {qa[i].x, qa[i].y, qa[i].z, qa[i].w}, ub[4] = {qb[i].x, qb[i].y, qb[i].z, qb[i].w};
-        const unsigned short* xs = sx + (b + i * p.kw) * kBlock + t * 8;
-        float part[NT][4];
+    for (int q = 0; q < NT; ++q) xs[q] = sx + min(q * 8 + g, n - 1) * stride + first * kBlock + t * 8;
+    auto consume = [&](const Block& blk, int i) {
+      const uint32_t ua[4] = {blk.a.x, blk.a.y, blk.a.z, blk.a.w}, ub[4] = {blk.b.x, blk.b.y, blk.b.z, blk.b.w};
+      // the leading terms' sums and those of the rest, apart: the latter's
+      // roundings are then 2^-8 of the former's
+      float part[NT][4], rest[NT][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j % (4 / kPer) == 0)
-#pragma unroll
-            for (int q = 0; q < NT; ++q)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) part[q][e] = 0.0f;
-          uint32_t va[4], vb[4];
-          unpack8<kBf16>(ua[j], va);
-          unpack8<kBf16>(ub[j], vb);
+      for (int j = 0; j < 4; ++j) {
+        if (j % kPieces == 0)
 #pragma unroll
           for (int q = 0; q < NT; ++q)
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term) {
-              uint4 xb = make_uint4(0u, 0u, 0u, 0u);
-              if (q * 8 + g < n) xb = *reinterpret_cast<const uint4*>(xs + (term * n + q * 8 + g) * stride + j * 32);
-              mma_16816<kBf16>(part[q], va[0], vb[0], va[1], vb[1], xb.x, xb.y);
-              mma_16816<kBf16>(part[q], va[2], vb[2], va[3], vb[3], xb.z, xb.w);
-            }
-          if (j % (4 / kPer) == 4 / kPer - 1) {
-            const float fa = __half2float(ha[i][j / (4 / kPer)]), fb = __half2float(hb[i][j / (4 / kPer)]);
+            for (int e = 0; e < 4; ++e) part[q][e] = rest[q][e] = 0.0f;
+        uint32_t va[4], vb[4];
+        unpack8<kBf16>(ua[j], va);
+        unpack8<kBf16>(ub[j], vb);
 #pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              acc[q][0] = fmaf(fa, part[q][0], acc[q][0]);
-              acc[q][1] = fmaf(fa, part[q][1], acc[q][1]);
-              acc[q][2] = fmaf(fb, part[q][2], acc[q][2]);
-              acc[q][3] = fmaf(fb, part[q][3], acc[q][3]);
-            }
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term) {
+            const uint4 xb = *reinterpret_cast<const uint4*>(xs[q] + term * n * stride + i * kBlock + j * 32);
+            float(&sum)[4] = term == 0 ? part[q] : rest[q];
+            mma_16816<kBf16>(sum, va[0], vb[0], va[1], vb[1], xb.x, xb.y);
+            mma_16816<kBf16>(sum, va[2], vb[2], va[3], vb[3], xb.z, xb.w);
           }
+        if (j % kPieces == kPieces - 1) {
+          const float fa = __half2float(blk.sa[j / kPieces]), fb = __half2float(blk.sb[j / kPieces]);
+#pragma unroll
+          for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[q][e] = fmaf(e < 2 ? fa : fb, kTerms > 1 ? part[q][e] + rest[q][e] : part[q][e], acc[q][e]);
         }
       }
+    };
+    auto advance = [&](int blocks) {
+      wa += blocks * 4;
+      wb += blocks * 4;
+      sa += blocks * kPer;
+      sb += blocks * kPer;
+#pragma unroll
+      for (int q = 0; q < NT; ++q) xs[q] += blocks * kBlock;
+    };
+    Block one[kSet], two[kSet];
+    int sets = (whole - first) / kSet;
+    if (sets > 0)
+#pragma unroll
+      for (int i = 0; i < kSet; ++i) request(one[i], i, kPer);
+    if (b0 > 0) __syncthreads();
+    stage_x<T, kTerms>(p, r0, n, b0, nb, sx, stride);
+    __syncthreads();
+    for (; sets > 0; sets -= 2) {
+      if (sets > 1)
+#pragma unroll
+        for (int i = 0; i < kSet; ++i) request(two[i], kSet + i, kPer);
+#pragma unroll
+      for (int i = 0; i < kSet; ++i) consume(one[i], i);
+      if (sets > 2)
+#pragma unroll
+        for (int i = 0; i < kSet; ++i) request(one[i], 2 * kSet + i, kPer);
+      if (sets > 1)
+#pragma unroll
+        for (int i = 0; i < kSet; ++i) consume(two[i], kSet + i);
+      advance(min(sets, 2) * kSet);
+    }
+    for (int b = first + (whole - first) / kSet * kSet; b < end; ++b) {
+      request(one[0], 0, min(kPer, p.groups - (b0 + b) * kPer));
+      consume(one[0], 0);
+      advance(1);
     }
   }
   // the warps' parts of k, joined in order: [warp][16][NT * 8 + 1]
@@ -211,18 +259,19 @@ template <typename T, int NT, int GROUP>
 int matvec_launch(W4Params p, cudaStream_t st) {
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
   const int n = std::min(p.rows, NT * 8);
-  // warps over k until there are about 16 on every SM, of 16 weight rows each
+  // warps over k until there are about 12 on every SM, of 16 weight rows each;
+  // small CTAs, so that all of them are resident and share the SMs evenly
   const int tiles = (p.m + 15) / 16;
   p.kw = 1;
-  while (p.kw < kWarps && p.kw * 2 <= p.blocks && tiles * p.kw < 16 * current_sm_count()) p.kw *= 2;
-  // x in shared memory: at most 48 KB, so that several CTAs share an SM
-  const int room = 48 * 1024 / (kTerms * n * 2);
+  while (p.kw < 8 && p.kw * 2 <= p.blocks && tiles * p.kw < 12 * current_sm_count()) p.kw *= 2;
+  const int warps = std::max(4, p.kw), rw = warps / p.kw;
+  // x in shared memory: at most 32 KB, so that several CTAs share an SM
+  const int room = 32 * 1024 / (kTerms * n * 2);
   p.stage = std::max(1, std::min(p.blocks, (room - 32) / kBlock));
   const std::size_t xs = static_cast<std::size_t>(kTerms) * n * stage_stride(p.stage) * 2;
-  const std::size_t rs = static_cast<std::size_t>(kWarps) * 16 * (NT * 8 + 1) * 4;
-  const int rw = kWarps / p.kw;
+  const std::size_t rs = static_cast<std::size_t>(warps) * 16 * (NT * 8 + 1) * 4;
   const dim3 grid(static_cast<unsigned>((tiles + rw - 1) / rw), static_cast<unsigned>((p.rows + NT * 8 - 1) / (NT * 8)));
-  w4_matvec_kernel<T, NT, GROUP><<<grid, kWarps * 32, std::max(xs, rs), st>>>(p);
+  w4_matvec_kernel<T, NT, GROUP><<<grid, static_cast<unsigned>(warps * 32), std::max(xs, rs), st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
