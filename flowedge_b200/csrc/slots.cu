@@ -137,6 +137,11 @@ __device__ __forceinline__ float silu1(float x) {
   return x * rcp_approx(1.0f + ex2_approx(x * -1.4426950408889634f));
 }
 
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T v[V];
+};
+
 // --- causal convolution -------------------------------------------------------
 
 struct ConvParams {
@@ -192,11 +197,6 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
       if (j < dc) win[j] = v[j];
   }
 }
-
-template <typename T, int V>
-struct alignas(V * sizeof(T)) Vec {
-  T v[V];
-};
 
 // One thread walks V channels of a tile's rows, two and two (V 1: a pair with
 // an idle half), with their last DC inputs in registers (right-aligned: taps
@@ -562,13 +562,13 @@ __device__ __forceinline__ float2 exp2_neg2(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
-// Lets a kernel have `bytes` of shared memory (always the same limit, so that
-// calls on several threads do not change each other's).
+// Lets a kernel have `bytes` of shared memory, at most 200 KB (always the same
+// limit, so that calls on several threads do not change each other's).
 template <typename K>
 cudaError_t allow_smem(K kernel, int bytes) {
   if (bytes <= 48 * 1024) return cudaSuccess;
   return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              227 * 1024);
+                              200 * 1024);
 }
 
 // --- the steps dt of a prompt call's rows --------------------------------------
@@ -598,20 +598,25 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A warp takes 16 rows x COLS channels at a time and walks the rows; dt_in goes
-// from memory into fragments, the weights' terms sit in shared memory for the
-// whole kernel: [term][16 of dt_rank][t][channel][2], t and the pair being the
-// fragment's, a lane's two words side by side and the lanes of a half warp on
-// different banks.
+// A warp takes 16 rows x COLS channels at a time and walks the rows; dt_in goes from memory into fragments (the next 16 columns asked for before
+// the products), the weights' terms sit in shared memory for the whole kernel:
+// [term][16 of dt_rank][t][channel][2], t and the pair being the fragment's, a
+// lane's two words side by side and the lanes of a half warp on different
+// banks.  (Two row tiles a warp, to read the weights' fragments half as often,
+// take the registers of a third CTA: 425 against 422 us for the whole scan of
+// 16384 rows x 2048 in bf16, 188 against 186 for 96 prompts x 1024 in fp32.)
 constexpr int kDtWarps = 8;
 constexpr int dt_stride(int cols) { return 2 * cols + 8; }
+constexpr int kDtRows = 16, kDtCtas = 3;  // rows of a warp, CTAs resident on an SM
 
 template <typename T, int COLS>
-__global__ void __launch_bounds__(kDtWarps * 32) scan_steps_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(const ScanParams p) {
   constexpr int kTerms = kDtTerms<T>, kStride = dt_stride(COLS);
   extern __shared__ __align__(16) uint32_t sb[];
+  __shared__ float sbias[COLS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int c0 = blockIdx.y * COLS, nk = (p.dr + 15) / 16;
+  const bool pairs = p.di % 2 == 0;
   for (int i = threadIdx.x; i < nk * 8 * COLS; i += kDtWarps * 32) {
     const int n = i % COLS, k2 = i / COLS, r = 2 * k2, c = c0 + n;
     float a = c < p.di && r < p.dr ? p.dt_w[static_cast<long long>(r) * p.di + c] : 0.0f;
@@ -620,89 +625,105 @@ __global__ void __launch_bounds__(kDtWarps * 32) scan_steps_kernel(const ScanPar
     for (int m = 0; m < 3; ++m)
       sb[((m * nk + k2 / 8) * 4 + k2 % 4) * kStride + 2 * n + k2 % 8 / 4] = take_bf16(a, b);
   }
+  for (int n = threadIdx.x; n < COLS; n += kDtWarps * 32) sbias[n] = c0 + n < p.di ? p.dt_b[c0 + n] : 0.0f;
   __syncthreads();
-  const long long step = static_cast<long long>(gridDim.x) * kDtWarps * 16;
-  for (long long row0 = (static_cast<long long>(blockIdx.x) * kDtWarps + warp) * 16; row0 < p.q.rows; row0 += step) {
-    float acc[COLS / 8][4] = {};
-    const bool lo = row0 + g < p.q.rows, hi = row0 + g + 8 < p.q.rows;
-    const T* ra = static_cast<const T*>(p.proj) + (row0 + g) * p.proj_ld;
-    const T* rb = ra + 8 * p.proj_ld;
-    T raw[8];  // rows g, g + 8 x columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the next 16
+  griddep_launch();
+  // two neighbours of a row in one load, where rows start on such pairs
+  const bool even = p.proj_ld % 2 == 0 && reinterpret_cast<std::uintptr_t>(p.proj) % (2 * sizeof(T)) == 0;
+  const long long step = static_cast<long long>(gridDim.x) * kDtWarps * kDtRows;
+  for (long long row0 = (static_cast<long long>(blockIdx.x) * kDtWarps + warp) * kDtRows; row0 < p.q.rows; row0 += step) {
+    float acc[COLS / 8][4];
+    const T* base = static_cast<const T*>(p.proj) + (row0 + g) * p.proj_ld + 2 * t;
+    const int have = static_cast<int>(min(static_cast<long long>(kDtRows), p.q.rows - row0)) - g;  // rows g + 8 i, 8 i < have
+    Vec<T, 2> raw[4];  // fragment words: (g, 2t), (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
     auto request = [&](int k) {
+      const bool whole = even && 16 * (k + 1) <= p.dr;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 16 * k + 2 * t + (i & 1) + (i & 2) * 4;
-        raw[i] = from_f32<T>(0.0f);
-        if (r < p.dr && (i < 4 ? lo : hi)) raw[i] = (i < 4 ? ra : rb)[r];
+      for (int w = 0; w < 4; ++w) {
+        const int row = 8 * (w & 1), r = 16 * k + 4 * (w & 2);
+        const T* src = base + row * p.proj_ld + r;
+        raw[w] = Vec<T, 2>{{from_f32<T>(0.0f), from_f32<T>(0.0f)}};
+        if (whole) {
+          if (row < have) raw[w] = *reinterpret_cast<const Vec<T, 2>*>(src);
+        } else {
+          const int more = row < have ? p.dr - r - 2 * t : 0;  // columns of dt_in from here on
+          if (more > 0) raw[w].v[0] = src[0];
+          if (more > 1) raw[w].v[1] = src[1];
+        }
       }
     };
     request(0);
+#pragma unroll
+    for (int n = 0; n < COLS / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][e] = sbias[8 * n + 2 * t + (e & 1)];
     for (int k = 0; k < nk; ++k) {
       uint32_t fa[kTerms][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // fragment words: (g, 2t), (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
-        const int at = (i & 1) * 4 + (i & 2);
-        float a = to_f32(raw[at]), b = to_f32(raw[at + 1]);
+      for (int w = 0; w < 4; ++w) {
+        float a = to_f32(raw[w].v[0]), b = to_f32(raw[w].v[1]);
 #pragma unroll
-        for (int q = 0; q < kTerms; ++q) fa[q][i] = take_bf16(a, b);
+        for (int q = 0; q < kTerms; ++q) fa[q][w] = take_bf16(a, b);
       }
       if (k + 1 < nk) request(k + 1);
-      // eight tiles at a time, so that the products in flight have sums of their own
+      // several tiles at a time, so that the products in flight have sums of their own
+      constexpr int kTogether = COLS / 8 < 8 ? COLS / 8 : 8;
 #pragma unroll
-      for (int n0 = 0; n0 < COLS / 8; n0 += 8) {
+      for (int n0 = 0; n0 < COLS / 8; n0 += kTogether) {
 #pragma unroll
         for (int m = 2; m >= 0; --m) {
-          uint2 b[8];
+          uint2 b[kTogether];
 #pragma unroll
-          for (int n = 0; n < 8; ++n)
+          for (int n = 0; n < kTogether; ++n)
             b[n] = *reinterpret_cast<const uint2*>(sb + ((m * nk + k) * 4 + t) * kStride + 2 * (8 * (n0 + n) + g));
 #pragma unroll
           for (int q = kTerms - 1; q >= 0; --q)
             if (q + m <= 2)
 #pragma unroll
-              for (int n = 0; n < 8; ++n) mma_bf16(acc[n0 + n], fa[q], b[n].x, b[n].y);
+              for (int n = 0; n < kTogether; ++n) mma_bf16(acc[n0 + n], fa[q], b[n].x, b[n].y);
         }
       }
     }
-    float* to = p.steps + (row0 + g) * p.di;
+    float* to = p.steps + (row0 + g) * p.di + c0 + 2 * t;
+    const long long below = 8LL * p.di;
 #pragma unroll
-    for (int n = 0; n < COLS / 8; ++n) {
+    for (int n = 0; n < COLS / 8; ++n, to += 8) {
       const int c = c0 + 8 * n + 2 * t;
-      const float b0 = c < p.di ? p.dt_b[c] : 0.0f, b1 = c + 1 < p.di ? p.dt_b[c + 1] : 0.0f;
+      const bool c_lo = c < p.di, c_hi = c + 1 < p.di;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 v = softplus_rel2(make_float2(acc[n][2 * i] + b0, acc[n][2 * i + 1] + b1));
-        if (!(i ? hi : lo)) continue;
-        float* at = to + static_cast<long long>(8 * i) * p.di + c;
-        if (c + 1 < p.di && p.di % 2 == 0) {
-          *reinterpret_cast<float2*>(at) = v;
+        const float2 v = softplus_rel2(make_float2(acc[n][2 * i], acc[n][2 * i + 1]));
+        float* at = to + i * below;
+        if (pairs) {
+          if (8 * i < have && c_hi) *reinterpret_cast<float2*>(at) = v;
         } else {
-          if (c < p.di) at[0] = v.x;
-          if (c + 1 < p.di) at[1] = v.y;
+          if (8 * i < have && c_lo) at[0] = v.x;
+          if (8 * i < have && c_hi) at[1] = v.y;
         }
       }
     }
   }
 }
 
+// Channels to a CTA: 64 (sums and fragments then leave room for three CTAs to
+// an SM), or 32 where the weights' terms of 64 do not fit the shared memory
+// (dt_rank above 256).
 template <typename T, int COLS>
 int steps_launch_cols(const ScanParams& p, cudaStream_t st) {
   const int smem = 4 * 3 * ((p.dr + 15) / 16) * 4 * dt_stride(COLS);
   if (const cudaError_t rc = allow_smem(scan_steps_kernel<T, COLS>, smem); rc != cudaSuccess) return static_cast<int>(rc);
-  const long long tiles = (p.q.rows + 15) / 16, cols = (p.di + COLS - 1) / COLS;
-  // two CTAs on every SM, or the row tiles that there are
-  const long long ctas = std::max(1LL, std::min((tiles + kDtWarps - 1) / kDtWarps, 2LL * current_sm_count() / cols));
+  const long long tiles = (p.q.rows + kDtRows - 1) / kDtRows, cols = (p.di + COLS - 1) / COLS;
+  const long long ctas =
+      std::max(1LL, std::min((tiles + kDtWarps - 1) / kDtWarps, static_cast<long long>(kDtCtas) * current_sm_count() / cols));
   scan_steps_kernel<T, COLS><<<dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(cols)), kDtWarps * 32,
                                static_cast<std::size_t>(smem), st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
-// 128 channels to a CTA, or 64 where the weights' terms of 128 do not fit the
-// shared memory (dt_rank above 256).
 template <typename T>
 int steps_launch(const ScanParams& p, cudaStream_t st) {
   if (p.q.rows == 0) return 0;
-  return p.dr <= 256 ? steps_launch_cols<T, 128>(p, st) : steps_launch_cols<T, 64>(p, st);
+  return p.dr <= 256 ? steps_launch_cols<T, 64>(p, st) : steps_launch_cols<T, 32>(p, st);
 }
 
 // --- the scan of prompts ----------------------------------------------------------
@@ -710,13 +731,15 @@ int steps_launch(const ScanParams& p, cudaStream_t st) {
 constexpr int kScanWarps = 4;  // warps of a CTA, 32 channels each
 constexpr int kStage = 16;     // rows whose B and C are in shared memory at a time
 constexpr int kTok = 4;        // rows whose dt, u and z are requested ahead
-// State pairs whose exponentials go to the FMA pipe: one of eight, the first
-// (where a grows with n, as it does at the start of training, the slowest
-// states).  Measured at 16384 rows x 2048 channels, DS 16: none 466 us, one
-// 472, two 490, three 523 (issue slots and the MUFU unit are then level); the
-// one is kept for its exactness near 1.
-template <int DS>
-constexpr int kPolyPairs = DS / 16;
+// State pairs whose exponentials go to the FMA pipe, the first ones (where a
+// grows with n, as it does at the start of training, the slowest states, which
+// gain from its exactness near 1).  A row's exponentials take the MUFU unit 8
+// cycles each, the FMA pipe 18 a pair beside 6 (summary) or 8 for the pair's
+// products: two pairs of eight in the summary, one where y is made too.
+// Measured for the latter at 16384 rows x 2048 channels, DS 16, both passes
+// alike: none 466 us, one 472, two 490, three 523.
+template <int DS, bool SUMMARY>
+constexpr int kPolyPairs = SUMMARY ? DS / 8 : DS / 16;
 
 // One thread per channel, the states in registers, over the rows of one tile.
 // SUMMARY: the tile's sum of dt and its state from a zero start, for the tiles
@@ -733,13 +756,17 @@ template <typename T, int DS, bool SUMMARY>
 __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt_kernel(const ScanParams p) {
   __shared__ __align__(16) float sbc[2][kStage][2 * DS];
   if (!SUMMARY) report_offsets(p.q);
+  // (the call's own inputs may be read before the kernel it waits for is
+  // done; every thread passes the wait, so that the kernels follow in order)
   const int s = find_sequence(p.q, blockIdx.x, p.chunk);
-  if (s < 0) return;
-  Seq q = resolve(p.q, s);
-  const long long k = blockIdx.x - (q.begin / p.chunk + s);
+  Seq q = resolve(p.q, s < 0 ? 0 : s);
   // (a summary is its sequence's own, whoever else has the slot)
-  if (!SUMMARY && !writes(p.q, s, q, blockIdx.y == 0)) return;
-  if (!q.live || (k > 0 && k * p.chunk >= q.len)) return;
+  const bool mine = SUMMARY ? q.live : writes(p.q, s < 0 ? 0 : s, q, s >= 0 && blockIdx.y == 0);
+  griddep_launch();
+  griddep_wait();
+  if (s < 0 || !mine) return;
+  const long long k = blockIdx.x - (q.begin / p.chunk + s);
+  if (k > 0 && k * p.chunk >= q.len) return;
   const int t0 = static_cast<int>(k * p.chunk);
   const bool last = t0 + p.chunk >= q.len;
   if (SUMMARY && last) return;
@@ -831,24 +858,26 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
   auto one_row = [&](const float* row, float d, float uv, float zv) {
     const float dtu = d * uv;
     const float2 d2 = splat(d), dtu2 = splat(dtu);
-    float2 y0 = make_float2(dk * uv, 0.0f), y1 = splat(0.0f);
+    float2 y0, y1;
     if (SUMMARY) sum_dt += d;
 #pragma unroll
     for (int n = 0; n < DS / 2; n += 2) {
       const float4 bq = *reinterpret_cast<const float4*>(row + 2 * n);
       const float2 e0 = __fmul2_rn(d2, an[n]), e1 = __fmul2_rn(d2, an[n + 1]);
-      const float2 a0 = n < kPolyPairs<DS> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
-      const float2 a1 = n + 1 < kPolyPairs<DS> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
+      const float2 a0 = n < kPolyPairs<DS, SUMMARY> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
+      const float2 a1 = n + 1 < kPolyPairs<DS, SUMMARY> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
       h[n] = __ffma2_rn(a0, h[n], __fmul2_rn(dtu2, make_float2(bq.x, bq.y)));
       h[n + 1] = __ffma2_rn(a1, h[n + 1], __fmul2_rn(dtu2, make_float2(bq.z, bq.w)));
       if (!SUMMARY) {
         const float4 cq = *reinterpret_cast<const float4*>(row + DS + 2 * n);
-        y0 = __ffma2_rn(h[n], make_float2(cq.x, cq.y), y0);
-        y1 = __ffma2_rn(h[n + 1], make_float2(cq.z, cq.w), y1);
+        const float2 c0 = make_float2(cq.x, cq.y), c1 = make_float2(cq.z, cq.w);
+        y0 = n == 0 ? __fmul2_rn(h[n], c0) : __ffma2_rn(h[n], c0, y0);
+        y1 = n == 0 ? __fmul2_rn(h[n + 1], c1) : __ffma2_rn(h[n + 1], c1, y1);
       }
     }
+    if (SUMMARY) return 0.0f;
     const float2 sum = __fadd2_rn(y0, y1);
-    const float yv = sum.x + sum.y;
+    const float yv = fmaf(dk, uv, sum.x + sum.y);
     return gated ? yv * silu1(zv) : yv;
   };
   settle(0);
@@ -909,13 +938,14 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
 // The state that enters each tile of a sequence of several, in place of the
 // tile's own end: one thread per channel and kCarryStates states walks the
 // tiles, the next kCarryAhead of them requested at a time.
-constexpr int kCarryStates = 2, kCarryAhead = 4;
-__global__ void __launch_bounds__(128) scan_carry_kernel(const ScanParams p) {
+constexpr int kCarryStates = 2, kCarryAhead = 8, kCarryThreads = 256;
+__global__ void __launch_bounds__(kCarryThreads) scan_carry_kernel(const ScanParams p) {
   const int s = blockIdx.x, n0 = blockIdx.z * kCarryStates;
-  if (p.q.offsets[s + 1] - p.q.offsets[s] <= p.chunk) return;
   const Seq q = resolve(p.q, s);
-  const int c = blockIdx.y * 128 + threadIdx.x;
-  if (!q.live || c >= p.di) return;
+  griddep_launch();
+  griddep_wait();
+  const int c = blockIdx.y * kCarryThreads + threadIdx.x;
+  if (!q.live || q.len <= p.chunk || c >= p.di) return;
   const int tiles = (q.len + p.chunk - 1) / p.chunk;
   const long long step = static_cast<long long>(1 + p.ds) * p.di;
   float* ws = p.ws + (q.begin / p.chunk + s) * step + c;
@@ -991,12 +1021,16 @@ int scan_typed(const ScanParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
   if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
   if (p.q.rows > p.chunk) {
-    scan_prompt_kernel<T, DS, true><<<grid, kScanWarps * 32, 0, st>>>(p);
-    scan_carry_kernel<<<dim3(static_cast<unsigned>(p.q.n_seq), cb,
-                             static_cast<unsigned>((p.ds + kCarryStates - 1) / kCarryStates)),
-                        128, 0, st>>>(p);
+    launch_pdl(scan_prompt_kernel<T, DS, true>, grid, dim3(kScanWarps * 32), 0, st, p);
+    launch_pdl(scan_carry_kernel,
+               dim3(static_cast<unsigned>(p.q.n_seq), static_cast<unsigned>((p.di + kCarryThreads - 1) / kCarryThreads),
+                    static_cast<unsigned>((p.ds + kCarryStates - 1) / kCarryStates)),
+               dim3(kCarryThreads), 0, st, p);
   }
-  scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, 0, st>>>(p);
+  if (p.q.rows > 0)
+    launch_pdl(scan_prompt_kernel<T, DS, false>, grid, dim3(kScanWarps * 32), 0, st, p);
+  else  // behind no kernel of this call: the caller's writes have to be seen
+    scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, 0, st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
