@@ -40,50 +40,67 @@ def _refuse(message: str):
     raise FlowEdgeError(1, message)
 
 
-def _check(rc: int):
-    if rc != 0:
-        raise FlowEdgeError(rc, load_library().fe_engine_last_error().decode())
+def _failed(rc: int):
+    raise FlowEdgeError(rc, load_library().fe_engine_last_error().decode())
 
 
-def _tensor(t, name: str, dtype, device):
+# The checks below take the plain case in a few attribute reads (a call of small
+# sizes costs little more than its checks); _explain goes through the same
+# conditions again and names the one that failed.  `device` is a CUDA index.
+
+
+def _explain(t, name: str, shape, dtype, device: int):
     if not isinstance(t, torch.Tensor):
         _refuse(f"{name} is a tensor")
     if t.dtype != dtype:
         _refuse(f"{name} is {dtype}, not {t.dtype}")
-    if t.device != device:
-        _refuse(f"{name} is on {t.device}, not {device}")
+    if not t.is_cuda or t.get_device() != device:
+        _refuse(f"{name} is on {t.device}, not cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name} requires a gradient: this operator has none")
+    if t.layout != torch.strided or t.shape != shape:
+        _refuse(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
 
 
-def _matrix(t, name: str, rows: int, width: int, dtype, device) -> int:
+def _matrix(t, name: str, shape: tuple, dtype, device: int) -> int:
     """Checks a matrix with contiguous rows and returns the distance of its rows."""
-    _tensor(t, name, dtype, device)
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
-        _refuse(f"{name} has shape {tuple(t.shape)}, not {(rows, width)}")
+    try:
+        plain = t.dtype is dtype and t.get_device() == device and t.shape == shape and not t.requires_grad
+    except (AttributeError, RuntimeError):
+        plain = False
+    if not plain:
+        _explain(t, name, shape, dtype, device)
     ld, inner = t.stride()
+    rows, width = shape
     if inner != 1 and width > 1:
         _refuse(f"{name} has rows that are not contiguous")
-    return ld if rows > 1 else max(ld, width)
+    return ld if rows > 1 or ld > width else width
 
 
-def _flat(t, name: str, shape: tuple, dtype, device):
+def _flat(t, name: str, shape: tuple, dtype, device: int):
     """Checks a contiguous tensor of the given shape."""
-    _tensor(t, name, dtype, device)
-    if t.shape != shape or not t.is_contiguous():
-        _refuse(f"{name} is a contiguous tensor of shape {tuple(shape)}, not {tuple(t.shape)}")
+    try:
+        if (t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous()
+                and not t.requires_grad):
+            return
+    except (AttributeError, RuntimeError):
+        pass
+    _explain(t, name, shape, dtype, device)
+    if not t.is_contiguous():
+        _refuse(f"{name} is a contiguous tensor of shape {tuple(shape)}")
 
 
 def _first(x, name: str):
-    """Checks the matrix that the other arguments go by."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _DTYPES:
+    """Checks the matrix that the other arguments go by: (shape, dtype, device)."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES or x.dim() != 2:
         _refuse(f"{name} is a matrix of float32, bfloat16 or float16")
-    if not x.is_cuda:
+    device = x.get_device() if x.is_cuda else -1
+    if device < 0:
         _refuse(f"{name} is on {x.device}, not on a GPU")
-    return x.shape[0], x.shape[1], x.dtype, x.device
+    return x.shape, x.dtype, device
 
 
-def _sequences(rows: int, offsets, slots, fresh, status, device) -> int:
+def _sequences(rows: int, offsets, slots, fresh, status, device: int) -> int:
     """Checks the sequences' description and returns their number."""
     n_seq = rows
     if offsets is not None:
@@ -94,34 +111,29 @@ def _sequences(rows: int, offsets, slots, fresh, status, device) -> int:
     if slots is not None:
         _flat(slots, "slots", (n_seq,), torch.int32, device)
     if fresh is not None:
-        _tensor(fresh, "fresh", torch.bool if getattr(fresh, "dtype", None) == torch.bool else torch.uint8, device)
-        if fresh.shape != (n_seq,) or not fresh.is_contiguous():
-            _refuse(f"fresh is a contiguous tensor of shape {(n_seq,)}, not {tuple(fresh.shape)}")
+        _flat(fresh, "fresh", (n_seq,), torch.bool if getattr(fresh, "dtype", None) is torch.bool else torch.uint8, device)
     if status is not None:
         _flat(status, "status", (1,), torch.int32, device)
     return n_seq
 
 
-def _pool(state, name: str, inner: tuple, device) -> tuple:
+def _pool(state, name: str, inner: tuple, device: int) -> tuple:
     """Checks a pool of slot states and returns (slots, distance of two slots)."""
-    _tensor(state, name, torch.float32, device)
-    if state.dim() != 3 or state.shape[1:] != inner:
-        _refuse(f"{name} has shape {tuple(state.shape)}, not {('slots',) + inner}")
-    per = inner[0] * inner[1]
+    if not isinstance(state, torch.Tensor) or state.dim() != 3:
+        _refuse(f"{name} is a tensor of shape {('slots',) + inner}")
+    n_slots = state.shape[0]
+    if (state.dtype is not torch.float32 or state.get_device() != device or state.shape != (n_slots, *inner)
+            or state.requires_grad):
+        _explain(state, name, (n_slots, *inner), torch.float32, device)
     outer, mid, last = state.stride()
     if (mid != inner[1] and inner[0] > 1) or (last != 1 and inner[1] > 1):
         _refuse(f"{name} has slots that are not contiguous")
-    return state.shape[0], outer if state.shape[0] > 1 else max(outer, per)
+    per = inner[0] * inner[1]
+    return n_slots, outer if n_slots > 1 or outer > per else per
 
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
-
-
-def _out(out, like_rows: int, width: int, dtype, device) -> tuple:
-    if out is None:
-        return torch.empty((like_rows, width), dtype=dtype, device=device), width
-    return out, _matrix(out, "out", like_rows, width, dtype, device)
 
 
 def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, status=None, out=None):
@@ -131,8 +143,9 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     float32, d_conv 1 to 8.  `window` [slots, d_inner, d_conv] float32 holds each slot's last inputs, newest last; a
     sequence reads the inputs before its first row there and leaves its own last ones.  Returns u like x.
     """
-    rows, di, dtype, device = _first(x, "x")
-    x_ld = _matrix(x, "x", rows, di, dtype, device)
+    shape, dtype, device = _first(x, "x")
+    rows, di = shape
+    x_ld = _matrix(x, "x", shape, dtype, device)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         _refuse("weight is a tensor of shape (d_inner, d_conv)")
     dc = weight.shape[1]
@@ -140,12 +153,16 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     _flat(bias, "bias", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
     n_slots, stride = (0, 0) if window is None else _pool(window, "window", (di, dc), device)
-    u, u_ld = _out(out, rows, di, dtype, device)
-    args = _CONV.pack(_CONV.size, device.index, _DTYPES[dtype], dc, rows, di, n_seq, n_slots, x_ld, u_ld, stride,
-                      x.data_ptr(), weight.data_ptr(), bias.data_ptr(), u.data_ptr(), _ptr(window), _ptr(offsets),
+    if out is None:
+        out = torch.empty_like(x)
+    u_ld = _matrix(out, "out", shape, dtype, device)
+    args = _CONV.pack(_CONV.size, device, _DTYPES[dtype], dc, rows, di, n_seq, n_slots, x_ld, u_ld, stride,
+                      x.data_ptr(), weight.data_ptr(), bias.data_ptr(), out.data_ptr(), _ptr(window), _ptr(offsets),
                       _ptr(slots), _ptr(fresh), _ptr(status))
-    _check(load_library().fe_causal_conv_device(args, _raw_stream(device.index)))
-    return u
+    rc = load_library().fe_causal_conv_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
+    return out
 
 
 def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=None, fresh=None, status=None,
@@ -158,35 +175,40 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     dt_w [dt_rank, d_inner] and dt_b [d_inner] float32, d_state 1 to 32, dt_rank 1 to 512.  `state` [slots, d_state,
     d_inner] float32.  Returns y like u.
     """
-    rows, di, dtype, device = _first(u, "u")
-    u_ld = _matrix(u, "u", rows, di, dtype, device)
+    shape, dtype, device = _first(u, "u")
+    rows, di = shape
+    u_ld = _matrix(u, "u", shape, dtype, device)
     if not isinstance(a, torch.Tensor) or a.dim() != 2 or not isinstance(dt_w, torch.Tensor) or dt_w.dim() != 2:
         _refuse("a is a tensor of shape (d_state, d_inner) and dt_w one of shape (dt_rank, d_inner)")
     ds, dr = a.shape[0], dt_w.shape[0]
-    proj_ld = _matrix(proj, "proj", rows, dr + 2 * ds, dtype, device)
-    z_ld = 0 if z is None else _matrix(z, "z", rows, di, dtype, device)
+    proj_ld = _matrix(proj, "proj", (rows, dr + 2 * ds), dtype, device)
+    z_ld = 0 if z is None else _matrix(z, "z", shape, dtype, device)
     _flat(a, "a", (ds, di), torch.float32, device)
     _flat(d, "d", (di,), torch.float32, device)
     _flat(dt_w, "dt_w", (dr, di), torch.float32, device)
     _flat(dt_b, "dt_b", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
     n_slots, stride = (0, 0) if state is None else _pool(state, "state", (ds, di), device)
-    y, y_ld = _out(out, rows, di, dtype, device)
+    if out is None:
+        out = torch.empty_like(u)
+    y_ld = _matrix(out, "out", shape, dtype, device)
     lib = load_library()
-
-    def pack(workspace, size):
-        return _SCAN.pack(_SCAN.size, device.index, _DTYPES[dtype], ds, rows, di, dr, n_seq, n_slots, u_ld, proj_ld,
-                          z_ld, y_ld, stride, u.data_ptr(), proj.data_ptr(), _ptr(z), a.data_ptr(), d.data_ptr(),
-                          dt_w.data_ptr(), dt_b.data_ptr(), y.data_ptr(), _ptr(state), _ptr(offsets), _ptr(slots),
-                          _ptr(fresh), _ptr(status), workspace, size)
-
-    workspace, size = None, 0
+    workspace, size = 0, 0
     if offsets is not None:
-        size = lib.fe_selective_scan_workspace(pack(0, 0))
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    _check(lib.fe_selective_scan_device(pack(_ptr(workspace), size), _raw_stream(device.index)))
-    return y
+        # the sizes alone decide; the tensor returns to torch's allocator in stream order
+        size = lib.fe_selective_scan_workspace(_SCAN.pack(_SCAN.size, device, _DTYPES[dtype], ds, rows, di, dr, n_seq,
+                                                          n_slots, u_ld, proj_ld, z_ld, y_ld, stride, 0, 0, 0, 0, 0, 0,
+                                                          0, 0, 0, offsets.data_ptr(), 0, 0, 0, 0, 0))
+        held = u.new_empty(size, dtype=torch.uint8)
+        workspace = held.data_ptr()
+    args = _SCAN.pack(_SCAN.size, device, _DTYPES[dtype], ds, rows, di, dr, n_seq, n_slots, u_ld, proj_ld, z_ld, y_ld,
+                      stride, u.data_ptr(), proj.data_ptr(), _ptr(z), a.data_ptr(), d.data_ptr(), dt_w.data_ptr(),
+                      dt_b.data_ptr(), out.data_ptr(), _ptr(state), _ptr(offsets), _ptr(slots), _ptr(fresh),
+                      _ptr(status), workspace, size)
+    rc = lib.fe_selective_scan_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
+    return out
 
 
 def _w4_shapes(m: int, k: int, group: int) -> tuple:
@@ -201,18 +223,21 @@ def w4_quantize(weight, group: int = 64) -> tuple:
     packed is uint8 [m, ceil(k / 128) * 64] in the layout of include/flowedge_b200.h (fe_w4_args), scales
     [m, ceil(k / group)].
     """
-    m, k, dtype, device = _first(weight, "weight")
-    ld = _matrix(weight, "weight", m, k, dtype, device)
+    shape, dtype, device = _first(weight, "weight")
+    m, k = shape
+    ld = _matrix(weight, "weight", shape, dtype, device)
     packed_shape, scales_shape = _w4_shapes(m, k, group)
-    packed = torch.empty(packed_shape, dtype=torch.uint8, device=device)
-    scales = torch.empty(scales_shape, dtype=torch.float16, device=device)
-    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, 0, m, k, ld, 0, weight.data_ptr(),
-                    packed.data_ptr(), scales.data_ptr(), 0)
-    _check(load_library().fe_w4_quantize_device(args, _raw_stream(device.index)))
+    packed = weight.new_empty(packed_shape, dtype=torch.uint8)
+    scales = weight.new_empty(scales_shape, dtype=torch.float16)
+    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, 0, m, k, ld, 0, weight.data_ptr(), packed.data_ptr(),
+                    scales.data_ptr(), 0)
+    rc = load_library().fe_w4_quantize_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
     return packed, scales
 
 
-def _w4_weight(packed, scales, k: int, group: int, device) -> int:
+def _w4_weight(packed, scales, k: int, group: int, device: int) -> int:
     """Checks a packed weight of k columns and returns its rows."""
     if not isinstance(packed, torch.Tensor) or packed.dim() != 2:
         _refuse("packed is a tensor of shape (m, ceil(k / 128) * 64)")
@@ -227,14 +252,16 @@ def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float3
     """The matrix [m, k] that a packed weight stands for, rounded to `dtype`."""
     if dtype not in _DTYPES:
         _refuse("dtype is float32, bfloat16 or float16")
-    device = getattr(packed, "device", None)
+    if not isinstance(packed, torch.Tensor) or not packed.is_cuda:
+        _refuse("packed is a tensor on a GPU")
+    device = packed.get_device()
     m = _w4_weight(packed, scales, k, group, device)
-    if not packed.is_cuda:
-        _refuse(f"packed is on {device}, not on a GPU")
-    weight = torch.empty((m, k), dtype=dtype, device=device)
-    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, 0, m, k, 0, k, 0, packed.data_ptr(),
-                    scales.data_ptr(), weight.data_ptr())
-    _check(load_library().fe_w4_dequantize_device(args, _raw_stream(device.index)))
+    weight = packed.new_empty((m, k), dtype=dtype)
+    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, 0, m, k, 0, k, 0, packed.data_ptr(), scales.data_ptr(),
+                    weight.data_ptr())
+    rc = load_library().fe_w4_dequantize_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
     return weight
 
 
@@ -243,14 +270,20 @@ def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
 
     float32, bfloat16 or float16 x and result; sums in float32, the weight exact.
     """
-    rows, k, dtype, device = _first(x, "x")
-    x_ld = _matrix(x, "x", rows, k, dtype, device)
+    shape, dtype, device = _first(x, "x")
+    rows, k = shape
+    x_ld = _matrix(x, "x", shape, dtype, device)
     m = _w4_weight(packed, scales, k, group, device)
-    y, y_ld = _out(out, rows, m, dtype, device)
-    args = _W4.pack(_W4.size, device.index, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(),
-                    packed.data_ptr(), scales.data_ptr(), y.data_ptr())
-    _check(load_library().fe_w4_matvec_device(args, _raw_stream(device.index)))
-    return y
+    if out is None:
+        out, y_ld = x.new_empty((rows, m)), m
+    else:
+        y_ld = _matrix(out, "out", (rows, m), dtype, device)
+    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(), packed.data_ptr(),
+                    scales.data_ptr(), out.data_ptr())
+    rc = load_library().fe_w4_matvec_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
+    return out
 
 
 def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-5, out=None):
@@ -260,21 +293,26 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
     float32 or the same; weights [dim] float32, dim 1 to 16384.  Without post_weight x is added as it is.  The returned
     norm is taken before the residual is rounded to its type.
     """
-    rows, dim, dtype, device = _first(x, "x")
-    x_ld = _matrix(x, "x", rows, dim, dtype, device)
-    r_dtype = getattr(residual, "dtype", None)
-    r_ld = _matrix(residual, "residual", rows, dim, dtype if r_dtype == dtype else torch.float32, device)
+    shape, dtype, device = _first(x, "x")
+    rows, dim = shape
+    x_ld = _matrix(x, "x", shape, dtype, device)
+    r_dtype = dtype if getattr(residual, "dtype", None) is dtype else torch.float32
+    r_ld = _matrix(residual, "residual", shape, r_dtype, device)
     _flat(weight, "weight", (dim,), torch.float32, device)
     if post_weight is not None:
         _flat(post_weight, "post_weight", (dim,), torch.float32, device)
     gate_ld = 0
     if gate is not None:
         one = isinstance(gate, torch.Tensor) and gate.dim() == 2 and gate.shape[0] == 1
-        gate_ld = _matrix(gate, "gate", 1 if one else rows, dim, dtype, device)
+        gate_ld = _matrix(gate, "gate", (1, dim) if one else shape, dtype, device)
         gate_ld = 0 if one else gate_ld
-    y, y_ld = _out(out, rows, dim, dtype, device)
-    args = _NORM.pack(_NORM.size, device.index, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
+    if out is None:
+        out = torch.empty_like(x)
+    y_ld = _matrix(out, "out", shape, dtype, device)
+    args = _NORM.pack(_NORM.size, device, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
                       x.data_ptr(), _ptr(post_weight), _ptr(gate), residual.data_ptr(), weight.data_ptr(),
-                      y.data_ptr(), scale, eps)
-    _check(load_library().fe_residual_norm_device(args, _raw_stream(device.index)))
-    return y
+                      out.data_ptr(), scale, eps)
+    rc = load_library().fe_residual_norm_device(args, _raw_stream(device))
+    if rc:
+        _failed(rc)
+    return out
