@@ -393,152 +393,6 @@ __device__ __forceinline__ float2 softplus_rel2(float2 x) {
 }
 __device__ __forceinline__ float softplus_rel(float x) { return softplus_rel2(splat(x)).x; }
 
-// One token for each of up to RT sequences; a thread has V neighbouring
-// channels, as a pair (V 1: the second is idle).  The dt projection's weights
-// are read once for the RT tokens; then each sequence's ds states are read,
-// stepped and written, which are the kernel's bytes.  Arithmetic on the two
-// channels at once (FFMA2).
-template <typename T, int DS, int RT, int V>
-__global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
-  extern __shared__ __align__(16) float sp[];  // dt_in [dr][RT], then per row [B (DS) | C (DS)], zero behind ds
-  __shared__ int sdup;
-  const int s0 = blockIdx.x * RT, c = (blockIdx.y * 128 + threadIdx.x) * V;
-  const int ds = p.ds, dr = p.dr, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int slot[RT], bad[RT];
-  bool fresh[RT];
-#pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const int s = s0 + j;
-    slot[j] = s >= p.q.n_seq ? -1 : (p.q.slots != nullptr ? p.q.slots[s] : s);
-    fresh[j] = s < p.q.n_seq && p.q.fresh != nullptr && p.q.fresh[s] != 0;
-    bad[j] = p.q.stateful && slot[j] >= p.q.n_slots ? FE_SEQ_BAD_SLOT : 0;
-  }
-  if (threadIdx.x == 0) sdup = 0;
-  // the states of all RT tokens into L2 while the projection runs: a lane one
-  // line of 32 of the warp's 32 V channels
-  if (p.state != nullptr)
-#pragma unroll
-    for (int j = 0; j < RT; ++j)
-      if (slot[j] >= 0 && bad[j] == 0 && !fresh[j])
-        for (int e = lane; e < ds * V; e += 32) {
-          const int at = c - lane * V + e % V * 32;
-          if (at < p.di) prefetch_l2(p.state + slot[j] * p.slot_stride + static_cast<long long>(e / V) * p.di + at);
-        }
-  float* const sbc = sp + (dr * RT + 3) / 4 * 4;  // on 16 bytes
-  for (int j = RT == 1 ? 0 : warp; j < RT; j += 4) {
-    const T* row = static_cast<const T*>(p.proj) + static_cast<long long>(s0 + j) * p.proj_ld;
-    const bool have = s0 + j < p.q.n_seq;
-    const int first = RT == 1 ? threadIdx.x : lane, step = RT == 1 ? 128 : 32;
-    for (int e = first; e < dr; e += step) sp[e * RT + j] = have ? to_f32(row[e]) : 0.0f;
-    for (int e = first; e < 2 * DS; e += step) {
-      const int n = e % DS;
-      sbc[j * 2 * DS + e] = have && n < ds ? to_f32(row[dr + (e < DS ? n : ds + n)]) : 0.0f;
-    }
-  }
-  __syncthreads();
-  if (p.q.stateful && p.q.slots != nullptr) {
-    int dup = 0;
-    for (int i = threadIdx.x; i < min(s0 + RT, p.q.n_seq); i += 128) {
-      const int v = p.q.slots[i];
-#pragma unroll
-      for (int j = 0; j < RT; ++j)
-        if (i < s0 + j && v == slot[j] && v >= 0) dup |= 1 << j;
-    }
-    if (dup != 0) atomicOr(&sdup, dup);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    if (sdup >> j & 1) bad[j] |= FE_SEQ_DUPLICATE_SLOT;
-    if (bad[j] != 0 && p.q.status != nullptr && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(p.q.status, bad[j]);
-    if (bad[j] != 0) slot[j] = -1;
-  }
-  if (c >= p.di) return;
-  auto load2 = [](const float* at) {
-    if constexpr (V == 2)
-      return *reinterpret_cast<const float2*>(at);
-    else
-      return make_float2(*at, 0.0f);
-  };
-  auto read2 = [](const void* base, long long at) {
-    const T* q = static_cast<const T*>(base) + at;
-    if constexpr (V == 2) {
-      const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(q);
-      return make_float2(to_f32(v.v[0]), to_f32(v.v[1]));
-    } else {
-      return make_float2(to_f32(*q), 0.0f);
-    }
-  };
-  float2 acc[RT];
-  const float2 bdt = load2(p.dt_b + c);
-#pragma unroll
-  for (int j = 0; j < RT; ++j) acc[j] = bdt;
-  const float* w = p.dt_w + c;
-#pragma unroll 8
-  for (int r = 0; r < dr; ++r, w += p.di) {
-    const float2 wv = load2(w);
-    if constexpr (RT == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(sp + r * 4);
-      acc[0] = __ffma2_rn(wv, splat(v.x), acc[0]);
-      acc[1] = __ffma2_rn(wv, splat(v.y), acc[1]);
-      acc[2] = __ffma2_rn(wv, splat(v.z), acc[2]);
-      acc[3] = __ffma2_rn(wv, splat(v.w), acc[3]);
-    } else {
-      acc[0] = __ffma2_rn(wv, splat(sp[r]), acc[0]);
-    }
-  }
-  float2 an[DS];
-  {
-    const float* a = p.a + c;
-#pragma unroll
-    for (int n = 0; n < DS; ++n, a += p.di) an[n] = n < ds ? __fmul2_rn(load2(a), splat(1.4426950408889634f)) : splat(0.0f);
-  }
-  const float2 dk = load2(p.d + c);
-#pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    if (slot[j] < 0) continue;
-    float* const st = p.state == nullptr ? nullptr : p.state + slot[j] * p.slot_stride + c;
-    const bool held = st != nullptr && !fresh[j];
-    float2 h[DS];
-    const float* from = st;
-#pragma unroll
-    for (int n = 0; n < DS; ++n, from += p.di) h[n] = held && n < ds ? load2(from) : splat(0.0f);
-    const float2 uv = read2(p.u, (s0 + j) * p.u_ld + c);
-    float2 gate = splat(1.0f);
-    if (p.z != nullptr) {
-      const float2 zv = read2(p.z, (s0 + j) * p.z_ld + c);
-      gate = silu2(zv);
-    }
-    const float2 dt = softplus_rel2(acc[j]), dtu = __fmul2_rn(dt, uv);
-    float2 y = __fmul2_rn(dk, uv);
-    float* to = st;
-#pragma unroll
-    for (int n = 0; n < DS; n += 4) {
-      const float4 bq = *reinterpret_cast<const float4*>(sbc + j * 2 * DS + n);
-      const float4 cq = *reinterpret_cast<const float4*>(sbc + j * 2 * DS + DS + n);
-      const float bn[4] = {bq.x, bq.y, bq.z, bq.w}, cn[4] = {cq.x, cq.y, cq.z, cq.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i, to += p.di) {
-        const float2 e = __fmul2_rn(dt, an[n + i]);
-        const float2 hn = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), h[n + i], __fmul2_rn(dtu, splat(bn[i])));
-        y = __ffma2_rn(hn, splat(cn[i]), y);
-        if (st != nullptr && n + i < ds) {
-          if constexpr (V == 2)
-            *reinterpret_cast<float2*>(to) = hn;
-          else
-            *to = hn.x;
-        }
-      }
-    }
-    y = __fmul2_rn(y, gate);
-    T* out = static_cast<T*>(p.y) + (s0 + j) * p.y_ld + c;
-    if constexpr (V == 2)
-      *reinterpret_cast<Vec<T, 2>*>(out) = Vec<T, 2>{{from_f32<T>(y.x), from_f32<T>(y.y)}};
-    else
-      *out = from_f32<T>(y.x);
-  }
-}
-
 // 2^x for a pair of x <= 0 on the FMA pipe.  x = k + r with k whole and r in
 // [-1/2, 1/2] (k by adding and taking away 1.5 * 2^23), 2^r = 1 + r q(r) with
 // q the degree-5 Chebyshev interpolant of (2^r - 1) / r, 2^k added to the
@@ -724,6 +578,127 @@ template <typename T>
 int steps_launch(const ScanParams& p, cudaStream_t st) {
   if (p.q.rows == 0) return 0;
   return p.dr <= 256 ? steps_launch_cols<T, 64>(p, st) : steps_launch_cols<T, 32>(p, st);
+}
+
+// --- the scan of single tokens -----------------------------------------------------
+
+// One token for a sequence.  DS / 8 threads of a warp share V neighbouring
+// channels (a pair; V 1: the second is idle), eight of their states each: a
+// thread requests its states first, which are the kernel's bytes; the rest of
+// its work comes while they do.  Arithmetic on the two channels at once
+// (FFMA2).  GIVEN: dt is in the workspace (many sequences: dt_w would be read
+// again for every one of them), else the CTA makes it.
+constexpr int kTokenStates = 8;  // of a thread
+
+template <typename T, int DS, int V, bool GIVEN>
+__global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
+  constexpr int kSplit = DS / kTokenStates, kPairs = 32 / kSplit;  // threads of a channel pair, pairs of a warp
+  extern __shared__ float sdt[];                  // dt_in [dr], not GIVEN
+  __shared__ __align__(16) float sbc[2 * DS];     // [B (DS) | C (DS)], zero behind ds
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kPairs;
+  const int s = blockIdx.x, c = ((blockIdx.y * 4 + warp) * kPairs + lane % kPairs) * V;
+  const int ds = p.ds, dr = p.dr, n0 = sub * kTokenStates;
+  const bool on = c < p.di;
+  const int cc = on ? c : 0;
+  auto load2 = [](const float* at) {
+    if constexpr (V == 2)
+      return *reinterpret_cast<const float2*>(at);
+    else
+      return make_float2(*at, 0.0f);
+  };
+  auto read2 = [](const void* base, long long at) {
+    const T* q = static_cast<const T*>(base) + at;
+    if constexpr (V == 2) {
+      const Vec<T, 2> v = *reinterpret_cast<const Vec<T, 2>*>(q);
+      return make_float2(to_f32(v.v[0]), to_f32(v.v[1]));
+    } else {
+      return make_float2(to_f32(*q), 0.0f);
+    }
+  };
+  Seq q = resolve(p.q, s);
+  float* const st = q.live && p.state != nullptr ? p.state + q.slot * p.slot_stride + static_cast<long long>(n0) * p.di + cc
+                                                 : nullptr;
+  const bool held = st != nullptr && !q.fresh;
+  float2 h[kTokenStates];
+  {
+    const float* from = st;
+#pragma unroll
+    for (int n = 0; n < kTokenStates; ++n, from += p.di) h[n] = held && n0 + n < ds ? load2(from) : splat(0.0f);
+  }
+  const float2 uv = read2(p.u, s * p.u_ld + cc);
+  const float2 zv = p.z != nullptr && sub == 0 ? read2(p.z, s * p.z_ld + cc) : splat(0.0f);
+  const T* row = static_cast<const T*>(p.proj) + s * p.proj_ld;
+  if (!GIVEN)
+    for (int e = threadIdx.x; e < dr; e += 128) sdt[e] = to_f32(row[e]);
+  for (int e = threadIdx.x; e < 2 * DS; e += 128) {
+    const int n = e % DS;
+    sbc[e] = n < ds ? to_f32(row[dr + (e < DS ? n : ds + n)]) : 0.0f;
+  }
+  float2 an[kTokenStates];
+  {
+    const float* a = p.a + static_cast<long long>(n0) * p.di + cc;
+#pragma unroll
+    for (int n = 0; n < kTokenStates; ++n, a += p.di)
+      an[n] = n0 + n < ds ? __fmul2_rn(load2(a), splat(1.4426950408889634f)) : splat(0.0f);
+  }
+  const float2 dk = load2(p.d + cc);
+  const bool runs = writes(p.q, s, q, blockIdx.y == 0);
+  if constexpr (GIVEN) griddep_wait();
+  __syncthreads();  // dt_in, B and C
+  auto across = [](float2 v) {  // summed over the channels' threads, the same in each
+#pragma unroll
+    for (int off = kPairs; off < 32; off *= 2) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+    }
+    return v;
+  };
+  float2 dt;
+  if constexpr (GIVEN) {
+    dt = load2(p.steps + static_cast<long long>(s) * p.di + cc);
+  } else {
+    // every kSplit-th term here, the rest in the channels' other threads
+    float2 acc = sub == 0 ? load2(p.dt_b + cc) : splat(0.0f);
+    const float* w = p.dt_w + static_cast<long long>(sub) * p.di + cc;
+#pragma unroll 8
+    for (int r = sub; r < dr; r += kSplit, w += static_cast<long long>(kSplit) * p.di)
+      acc = __ffma2_rn(load2(w), splat(sdt[r]), acc);
+    dt = softplus_rel2(across(acc));
+  }
+  const float2 dtu = __fmul2_rn(dt, uv);
+  float2 y = sub == 0 ? __fmul2_rn(dk, uv) : splat(0.0f);
+#pragma unroll
+  for (int n = 0; n < kTokenStates; n += 4) {
+    const float4 bq = *reinterpret_cast<const float4*>(sbc + n0 + n);
+    const float4 cq = *reinterpret_cast<const float4*>(sbc + DS + n0 + n);
+    const float bn[4] = {bq.x, bq.y, bq.z, bq.w}, cn[4] = {cq.x, cq.y, cq.z, cq.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 e = __fmul2_rn(dt, an[n + i]);
+      h[n + i] = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), h[n + i], __fmul2_rn(dtu, splat(bn[i])));
+      y = __ffma2_rn(h[n + i], splat(cn[i]), y);
+    }
+  }
+  y = across(y);
+  if (!runs || !on) return;
+  if (st != nullptr) {
+    float* to = st;
+#pragma unroll
+    for (int n = 0; n < kTokenStates; ++n, to += p.di)
+      if (n0 + n < ds) {
+        if constexpr (V == 2)
+          *reinterpret_cast<float2*>(to) = h[n];
+        else
+          *to = h[n].x;
+      }
+  }
+  if (sub != 0) return;  // one of the channels' threads writes the row
+  if (p.z != nullptr) y = __fmul2_rn(y, silu2(zv));
+  T* out = static_cast<T*>(p.y) + s * p.y_ld + c;
+  if constexpr (V == 2)
+    *reinterpret_cast<Vec<T, 2>*>(out) = Vec<T, 2>{{from_f32<T>(y.x), from_f32<T>(y.y)}};
+  else
+    *out = from_f32<T>(y.x);
 }
 
 // --- the scan of prompts ----------------------------------------------------------
@@ -990,25 +965,31 @@ int scan_chunk(long long rows, int di) {
   return chunk;
 }
 
-// Pairs of channels where the matrices and slots allow it, and four tokens to
-// a CTA (one reading of dt_w) once that leaves four CTAs for every SM.
+// Whether dt of single tokens is made for all of them beforehand: from as many
+// as fill the GPU.  Fewer take dt_w from L2 faster than another kernel starts.
+bool tokens_given(long long n_seq, long long di) { return n_seq * di >= 512LL * current_sm_count() && n_seq >= 16; }
+
 template <typename T, int DS>
 int scan_tokens(const ScanParams& p, cudaStream_t st) {
   const auto even = [](const void* q, long long ld, std::size_t e) {
     return reinterpret_cast<std::uintptr_t>(q) % (2 * e) == 0 && ld % 2 == 0;
   };
+  // pairs of channels where the matrices and slots allow it
   const bool pairs = p.di % 2 == 0 && even(p.u, p.u_ld, sizeof(T)) && even(p.y, p.y_ld, sizeof(T)) &&
                      even(p.z, p.z_ld, sizeof(T)) && even(p.state, p.slot_stride, 4) && even(p.a, 0, 4) &&
                      even(p.d, 0, 4) && even(p.dt_w, 0, 4) && even(p.dt_b, 0, 4);
-  const unsigned cb = static_cast<unsigned>((p.di + (pairs ? 255 : 127)) / (pairs ? 256 : 128));
-  const bool four = (p.q.n_seq + 3LL) / 4 * cb >= 4LL * current_sm_count();
-  const dim3 grid(static_cast<unsigned>(four ? (p.q.n_seq + 3) / 4 : p.q.n_seq), cb);
-  const std::size_t rt = four ? 4 : 1;
-  const std::size_t smem = ((p.dr * rt + 3) / 4 * 4 + 2 * DS * rt) * sizeof(float);
-  if (four)
-    pairs ? scan_token_kernel<T, DS, 4, 2><<<grid, 128, smem, st>>>(p) : scan_token_kernel<T, DS, 4, 1><<<grid, 128, smem, st>>>(p);
-  else
-    pairs ? scan_token_kernel<T, DS, 1, 2><<<grid, 128, smem, st>>>(p) : scan_token_kernel<T, DS, 1, 1><<<grid, 128, smem, st>>>(p);
+  const int channels = 128 / (DS / kTokenStates) * (pairs ? 2 : 1);  // of a CTA
+  const dim3 grid(static_cast<unsigned>(p.q.n_seq), static_cast<unsigned>((p.di + channels - 1) / channels));
+  const dim3 block(128);
+  if (tokens_given(p.q.n_seq, p.di)) {
+    if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
+    pairs ? launch_pdl(scan_token_kernel<T, DS, 2, true>, grid, block, 0, st, p)
+          : launch_pdl(scan_token_kernel<T, DS, 1, true>, grid, block, 0, st, p);
+  } else {
+    const std::size_t smem = static_cast<std::size_t>(p.dr) * sizeof(float);
+    pairs ? scan_token_kernel<T, DS, 2, false><<<grid, block, smem, st>>>(p)
+          : scan_token_kernel<T, DS, 1, false><<<grid, block, smem, st>>>(p);
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1098,8 +1079,9 @@ std::size_t steps_bytes(std::size_t rows, std::size_t d_inner) {
 }  // namespace
 
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept {
-  if (a.offsets == nullptr) return 0;
   const std::size_t steps = steps_bytes(a.rows, a.d_inner);
+  if (a.offsets == nullptr)
+    return tokens_given(static_cast<long long>(a.n_seq), static_cast<long long>(a.d_inner)) ? steps : 0;
   const int chunk = scan_chunk(static_cast<long long>(a.rows), static_cast<int>(a.d_inner));
   if (a.rows <= static_cast<std::uint64_t>(chunk)) return steps;
   return steps + (a.rows / static_cast<std::uint64_t>(chunk) + a.n_seq) * (1 + a.d_state) * a.d_inner * sizeof(float);

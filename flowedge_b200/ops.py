@@ -194,13 +194,14 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     y_ld = _matrix(out, "out", shape, dtype, device)
     lib = load_library()
     workspace, size = 0, 0
-    if offsets is not None:
+    if offsets is not None or n_seq >= 16:  # fewer single tokens need none
         # the sizes alone decide; the tensor returns to torch's allocator in stream order
         size = lib.fe_selective_scan_workspace(_SCAN.pack(_SCAN.size, device, _DTYPES[dtype], ds, rows, di, dr, n_seq,
                                                           n_slots, u_ld, proj_ld, z_ld, y_ld, stride, 0, 0, 0, 0, 0, 0,
-                                                          0, 0, 0, offsets.data_ptr(), 0, 0, 0, 0, 0))
-        held = u.new_empty(size, dtype=torch.uint8)
-        workspace = held.data_ptr()
+                                                          0, 0, 0, _ptr(offsets), 0, 0, 0, 0, 0))
+        if size:
+            held = u.new_empty(size, dtype=torch.uint8)
+            workspace = held.data_ptr()
     args = _SCAN.pack(_SCAN.size, device, _DTYPES[dtype], ds, rows, di, dr, n_seq, n_slots, u_ld, proj_ld, z_ld, y_ld,
                       stride, u.data_ptr(), proj.data_ptr(), _ptr(z), a.data_ptr(), d.data_ptr(), dt_w.data_ptr(),
                       dt_b.data_ptr(), out.data_ptr(), _ptr(state), _ptr(offsets), _ptr(slots), _ptr(fresh),

@@ -479,10 +479,11 @@ int fe_causal_conv_device(const fe_conv_args* args, void* stream);
  *   y[t][c] = (d[c] u[t][c] + sum_n h_n C_n) SiLU(z[t][c])    (no z: no gate)
  * u, proj, z and y are `dtype`; weights, states ([d_state][d_inner] per slot)
  * and all sums are fp32.  d_state 1 .. 32, dt_rank 1 .. 512.  y may share no
- * element with u, z or proj.  `workspace` holds prompts' steps dt and the
- * partial states of prompts that are scanned in parallel pieces: at least
- * fe_selective_scan_workspace(args) bytes (0 for single tokens), 16-byte
- * aligned, in use until the call's work completes. */
+ * element with u, z or proj.  `workspace` holds the rows' steps dt (of
+ * prompts, and of many single tokens) and the partial states of prompts that
+ * are scanned in parallel pieces: at least fe_selective_scan_workspace(args)
+ * bytes (0 for few single tokens), 16-byte aligned, in use until the call's
+ * work completes. */
 typedef struct fe_scan_args {
   uint32_t struct_size; /* sizeof(fe_scan_args) */
   int32_t device;
