@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
   const bool even = p.proj_ld % 2 == 0 && reinterpret_cast<std::uintptr_t>(p.proj) % (2 * sizeof(T)) == 0;
   const long long step = static_cast<long long>(gridDim.x) * kDtWarps * kDtRows;
   for (long long row0 = (static_cast<long long>(blockIdx.x) * kDtWarps + warp) * kDtRows; row0 < p.q.rows; row0 += step) {
-    float acc[COLS / 8][4];
+    float acc[COLS / 8][4] = {};
     const T* base = static_cast<const T*>(p.proj) + (row0 + g) * p.proj_ld + 2 * t;
     const int have = static_cast<int>(min(static_cast<long long>(kDtRows), p.q.rows - row0)) - g;  // rows g + 8 i, 8 i < have
     Vec<T, 2> raw[4];  // fragment words: (g, 2t), (g + 8, 2t), (g, 2t + 8), (g + 8, 2t + 8)
@@ -507,10 +507,6 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
       }
     };
     request(0);
-#pragma unroll
-    for (int n = 0; n < COLS / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][e] = sbias[8 * n + 2 * t + (e & 1)];
     for (int k = 0; k < nk; ++k) {
       uint32_t fa[kTerms][4];
 #pragma unroll
@@ -544,9 +540,12 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
     for (int n = 0; n < COLS / 8; ++n, to += 8) {
       const int c = c0 + 8 * n + 2 * t;
       const bool c_lo = c < p.di, c_hi = c + 1 < p.di;
+      const float2 bias = make_float2(sbias[8 * n + 2 * t], sbias[8 * n + 2 * t + 1]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 v = softplus_rel2(make_float2(acc[n][2 * i], acc[n][2 * i + 1]));
+        // (the bias joins here: the instruction's sums drop bits below the
+        // largest term's last, and the bias is the largest)
+        const float2 v = softplus_rel2(make_float2(acc[n][2 * i] + bias.x, acc[n][2 * i + 1] + bias.y));
         float* at = to + i * below;
         if (pairs) {
           if (8 * i < have && c_hi) *reinterpret_cast<float2*>(at) = v;

@@ -121,7 +121,7 @@ __host__ __device__ constexpr int stage_stride(int blocks) { return blocks * kBl
 // order.  A warp has kSet blocks in its arithmetic and the next kSet on their
 // way; a last odd block and one whose last groups do not exist come one by one.
 template <typename T, int NT, int GROUP>
-__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) w4_matvec_kernel(const W4Params p) {
+__global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
   constexpr bool kBf16 = !std::is_same_v<T, __half>;
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
   constexpr int kPer = kBlock / GROUP, kPieces = 4 / kPer;  // groups of a block, 32-element pieces of a group
