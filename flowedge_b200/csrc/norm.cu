@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "convert.cuh"
@@ -47,7 +48,7 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float* red) {
 }
 
 template <typename T, typename R, int VEC, int NV>
-__global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(512, 1) residual_norm_kernel(const NormParams p) {
   __shared__ float red[32];
   const long long row = blockIdx.x * static_cast<long long>(blockDim.x / p.tpr) + threadIdx.x / p.tpr;
   const int lane = threadIdx.x & (p.tpr - 1);
@@ -59,64 +60,93 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
   T* out = static_cast<T*>(p.out) + rr * p.out_ld;
   // the gate is asked for together with x, but not where that takes the registers of a long row
   constexpr bool kEarly = NV * VEC <= 16;
-  Pack<T, VEC> xv[NV], gv[kEarly ? NV : 1];
-  Pack<R, VEC> rv[NV];
+  float t[NV][VEC], y[NV][VEC], gv[kEarly ? NV : 1][VEC];  // x, then what it adds; the residual
+  const int c0 = lane * VEC, step = p.tpr * VEC;
+  auto read = [](float(&to)[VEC], const auto* from) {
+    using E = std::remove_cv_t<std::remove_pointer_t<decltype(from)>>;
+    const Pack<E, VEC> v = *reinterpret_cast<const Pack<E, VEC>*>(from);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (lane + i * p.tpr) * VEC;
-    if (c < p.dim) {
-      xv[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + c);
-      rv[i] = *reinterpret_cast<const Pack<R, VEC>*>(res + c);
-      if (kEarly && gate != nullptr) gv[kEarly ? i : 0] = *reinterpret_cast<const Pack<T, VEC>*>(gate + c);
+    for (int e = 0; e < VEC; ++e) to[e] = to_f32(v.v[e]);
+  };
+  auto write = [](auto* to, const float(&from)[VEC]) {
+    using E = std::remove_pointer_t<decltype(to)>;
+    Pack<E, VEC> v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v.v[e] = from_f32<E>(from[e]);
+    *reinterpret_cast<Pack<E, VEC>*>(to) = v;
+  };
+  if constexpr (VEC > 2) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + i * step;
+      if (c < p.dim) {
+        read(t[i], x + c);
+        read(y[i], res + c);
+        if (kEarly && gate != nullptr) read(gv[kEarly ? i : 0], gate + c);
+      }
     }
+  } else {
+    // many short requests: all of them first (behind the row's end the last
+    // vector again, so that no branch parts them), only then the conversions,
+    // each of which waits (16384 x 2047 in bf16: 145 us, as above 370)
+    Pack<T, VEC> xr[NV], gr[kEarly ? NV : 1];
+    Pack<R, VEC> rr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = min(c0 + i * step, p.dim - VEC);
+      xr[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + c);
+      rr[i] = *reinterpret_cast<const Pack<R, VEC>*>(res + c);
+      if (kEarly && gate != nullptr) gr[kEarly ? i : 0] = *reinterpret_cast<const Pack<T, VEC>*>(gate + c);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        t[i][e] = to_f32(xr[i].v[e]);
+        y[i][e] = to_f32(rr[i].v[e]);
+        if (kEarly && gate != nullptr) gv[kEarly ? i : 0][e] = to_f32(gr[kEarly ? i : 0].v[e]);
+      }
   }
   float mul = p.scale;
   if (p.post != nullptr) {
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if ((lane + i * p.tpr) * VEC < p.dim)
+      if (c0 + i * step < p.dim)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float v = to_f32(xv[i].v[e]);
-          ss = fmaf(v, v, ss);
-        }
+        for (int e = 0; e < VEC; ++e) ss = fmaf(t[i][e], t[i][e], ss);
     mul = p.scale * rsqrtf(fmaf(row_sum(ss, p.tpr, red), p.inv_dim, p.eps));
   }
-  float y[NV][VEC];
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (lane + i * p.tpr) * VEC;
+    const int c = c0 + i * step;
     if (c < p.dim) {
-      Pack<R, VEC> keep;
-      Pack<float, VEC> pw;
-      if (p.post != nullptr) pw = *reinterpret_cast<const Pack<float, VEC>*>(p.post + c);
-      if (!kEarly && gate != nullptr) gv[0] = *reinterpret_cast<const Pack<T, VEC>*>(gate + c);
+      float pw[VEC];
+      if (p.post != nullptr) read(pw, p.post + c);
+      if (!kEarly && gate != nullptr) read(gv[0], gate + c);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float t = to_f32(xv[i].v[e]) * mul;
-        if (p.post != nullptr) t *= pw.v[e];
-        if (gate != nullptr) t *= to_f32(gv[kEarly ? i : 0].v[e]);
-        const float v = to_f32(rv[i].v[e]) + t;
-        keep.v[e] = from_f32<R>(v);
-        y[i][e] = v;
-        ss = fmaf(v, v, ss);
+        float v = t[i][e] * mul;
+        if (p.post != nullptr) v *= pw[e];
+        if (gate != nullptr) v *= gv[kEarly ? i : 0][e];
+        y[i][e] += v;
+        ss = fmaf(y[i][e], y[i][e], ss);
       }
-      if (live) *reinterpret_cast<Pack<R, VEC>*>(res + c) = keep;
+      if (live) write(res + c, y[i]);
     }
   }
   const float norm = rsqrtf(fmaf(row_sum(ss, p.tpr, red), p.inv_dim, p.eps));
   if (!live) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (lane + i * p.tpr) * VEC;
+    const int c = c0 + i * step;
     if (c < p.dim) {
-      Pack<T, VEC> o;
-      const Pack<float, VEC> w = *reinterpret_cast<const Pack<float, VEC>*>(p.weight + c);
+      float w[VEC];
+      read(w, p.weight + c);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f32<T>(y[i][e] * norm * w.v[e]);
-      *reinterpret_cast<Pack<T, VEC>*>(out + c) = o;
+      for (int e = 0; e < VEC; ++e) w[e] *= y[i][e] * norm;
+      write(out + c, w);
     }
   }
 }
@@ -124,32 +154,44 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
 template <typename T, typename R>
 int norm_typed(NormParams p, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);  // 16 bytes of the 16- or 32-bit matrices
-  const auto fits = [&](const void* q, long long ld, std::size_t e) {
-    return reinterpret_cast<std::uintptr_t>(q) % 16 == 0 && ld * static_cast<long long>(e) % 16 == 0;
+  // rows that start on `vec` elements, up to 16 bytes
+  const auto starts = [&](int vec) {
+    const auto fits = [&](const void* q, long long ld, std::size_t e) {
+      const std::size_t bytes = std::min<std::size_t>(16, vec * e);
+      return reinterpret_cast<std::uintptr_t>(q) % bytes == 0 && ld * e % bytes == 0;
+    };
+    return p.dim % vec == 0 && fits(p.x, p.x_ld, sizeof(T)) && fits(p.out, p.out_ld, sizeof(T)) &&
+           fits(p.residual, p.residual_ld, sizeof(R)) && (p.gate == nullptr || fits(p.gate, p.gate_ld, sizeof(T))) &&
+           fits(p.weight, 0, 4) && fits(p.post, 0, 4);
   };
-  const bool wide = p.dim % kVec == 0 && fits(p.x, p.x_ld, sizeof(T)) && fits(p.out, p.out_ld, sizeof(T)) &&
-                    fits(p.residual, p.residual_ld, sizeof(R)) && (p.gate == nullptr || fits(p.gate, p.gate_ld, sizeof(T))) && fits(p.weight, 0, 4) && fits(p.post, 0, 4);
-  const int vecs = wide ? p.dim / kVec : p.dim;
-  // few rows: as many threads to a row as it has vectors; many rows: about two
-  // vectors to a thread (16384 x 2048 gated in bf16: 84.5 us, one vector 90.2)
-  const int per = p.rows < 2 * current_sm_count() ? 1 : 2;
+  const int vec = starts(kVec) ? kVec : starts(2) ? 2 : 1, vecs = p.dim / vec;
+  // few rows: as many threads to a row as it has vectors; many rows: about 16
+  // elements to a thread, which leaves several rows on an SM at a time (16384 x
+  // 2048 gated in bf16: 84.5 us, 8 elements 90.2; 16384 x 2047 with 512 threads
+  // to a row, one row on an SM: 540 us)
+  const int per = p.rows < 2 * current_sm_count() ? 1 : 16 / vec;
   p.tpr = 32;
   while (p.tpr < 512 && p.tpr * per < vecs) p.tpr *= 2;
   const int threads = std::max(p.tpr, 128), nv = (vecs + p.tpr - 1) / p.tpr;
   const unsigned grid = static_cast<unsigned>((p.rows + threads / p.tpr - 1) / (threads / p.tpr));
-  if (wide) {
-    if (nv <= 1)
-      residual_norm_kernel<T, R, kVec, 1><<<grid, threads, 0, st>>>(p);
-    else if (nv <= 2)
-      residual_norm_kernel<T, R, kVec, 2><<<grid, threads, 0, st>>>(p);
+  // up to 2, 8, 16 or 32 elements to a thread (at most 16384 on 512 threads)
+  const auto launch = [&](auto width) {
+    constexpr int V = decltype(width)::value;
+    if (nv * V <= 2 || nv == 1)
+      residual_norm_kernel<T, R, V, (V < 2 ? 2 : 1)><<<grid, threads, 0, st>>>(p);
+    else if (nv * V <= 8)
+      residual_norm_kernel<T, R, V, (V < 8 ? 8 / V : 1)><<<grid, threads, 0, st>>>(p);
+    else if (nv * V <= 16)
+      residual_norm_kernel<T, R, V, 16 / V><<<grid, threads, 0, st>>>(p);
     else
-      residual_norm_kernel<T, R, kVec, 32 / kVec><<<grid, threads, 0, st>>>(p);  // 32 elements to a thread at most
-  } else {
-    if (nv <= 2)
-      residual_norm_kernel<T, R, 1, 2><<<grid, threads, 0, st>>>(p);
-    else
-      residual_norm_kernel<T, R, 1, 32><<<grid, threads, 0, st>>>(p);
-  }
+      residual_norm_kernel<T, R, V, 32 / V><<<grid, threads, 0, st>>>(p);
+  };
+  if (vec == kVec)
+    launch(std::integral_constant<int, kVec>{});
+  else if (vec == 2)
+    launch(std::integral_constant<int, 2>{});
+  else
+    launch(std::integral_constant<int, 1>{});
   return static_cast<int>(cudaGetLastError());
 }
 
