@@ -74,39 +74,68 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&v)[4]) {
 
 // Stages rows r0 .. r0 + n - 1, columns of `blocks` packed blocks from block
 // b0 on, as TERMS planes of [n][stride] 16-bit values; zero behind column k.
+// A warp a row, a lane four columns at a time (16 or 8 bytes where rows start
+// on as many), kAhead of those requested together.
 template <typename T, int TERMS>
 __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0, int blocks, unsigned short* sx, int stride) {
-  const int width = blocks * kBlock, first = b0 * kBlock;
+  constexpr int kAhead = 4;
   if constexpr (TERMS == 1) {
     // whole 16 bytes as they are, where rows start on them and k ends there
     if (p.k % 8 == 0 && p.x_ld % 8 == 0 && reinterpret_cast<std::uintptr_t>(p.x) % 16 == 0) {
-      for (int i = threadIdx.x; i < n * (width / 8); i += blockDim.x) {
-        const int r = i / (width / 8), c = (i - r * (width / 8)) * 8;
-        const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first + c;
-        const uint4 v = first + c < p.k ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(sx + r * stride + c) = v;
+      const int pieces = blocks * (kBlock / 8);
+      for (int i = threadIdx.x; i < n * pieces; i += blockDim.x) {
+        const int r = i / pieces, c = (i - r * pieces) * 8;
+        const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + b0 * kBlock + c;
+        *reinterpret_cast<uint4*>(sx + r * stride + c) =
+            b0 * kBlock + c < p.k ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
       }
       return;
     }
   }
-  for (int i = threadIdx.x; i < n * (width / 2); i += blockDim.x) {
-    const int r = i / (width / 2), c = (i - r * (width / 2)) * 2;
-    const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first + c;
-    T v0 = first + c < p.k ? src[0] : from_f32<T>(0.0f), v1 = first + c + 1 < p.k ? src[1] : from_f32<T>(0.0f);
-    unsigned short* dst = sx + r * stride + c;
-    if constexpr (TERMS == 1) {
-      *reinterpret_cast<uint32_t*>(dst) = static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v0)) |
-                                          static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(&v1)) << 16;
-    } else {
-      // the leading bits as bf16, then the rest's: 8 + 8 + 8 bits, nothing lost
-      float f0 = v0, f1 = v1;
+  struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+  };
+  const int width = blocks * kBlock, first = b0 * kBlock, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const bool whole = p.x_ld % 4 == 0 && reinterpret_cast<std::uintptr_t>(p.x) % sizeof(Four) == 0;
+  // (few rows: several warps share one, each with a part of its columns)
+  const int share = max(1, warps / n), part = (threadIdx.x >> 5) % share;
+  for (int r = (threadIdx.x >> 5) / share; r < n; r += warps / share) {
+    const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + first;
+    const int have = p.k - first;  // columns of x from here on
+    for (int c0 = 4 * lane + 128 * part; c0 < width; c0 += 128 * share * kAhead) {
+      Four v[kAhead];
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        const float h0 = __uint_as_float(__float_as_uint(f0) & 0xFFFF0000u);
-        const float h1 = __uint_as_float(__float_as_uint(f1) & 0xFFFF0000u);
-        *reinterpret_cast<uint32_t*>(dst + t * n * stride) = __byte_perm(__float_as_uint(h0), __float_as_uint(h1), 0x7632);
-        f0 = isinf(h0) ? 0.0f : f0 - h0;
-        f1 = isinf(h1) ? 0.0f : f1 - h1;
+      for (int i = 0; i < kAhead; ++i) {
+        const int c = c0 + 128 * share * i;
+        if (whole && c + 4 <= have) {
+          v[i] = *reinterpret_cast<const Four*>(src + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i].v[e] = c + e < have ? src[c + e] : from_f32<T>(0.0f);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int c = c0 + 128 * share * i;
+        if (c >= width) break;
+        unsigned short* dst = sx + r * stride + c;
+        if constexpr (TERMS == 1) {
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(&v[i]);
+        } else {
+          // the leading bits as bf16, then the rest's: 8 + 8 + 8 bits, nothing lost
+          float f[4] = {v[i].v[0], v[i].v[1], v[i].v[2], v[i].v[3]};
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) {
+            float h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = __uint_as_float(__float_as_uint(f[e]) & 0xFFFF0000u);
+            *reinterpret_cast<uint2*>(dst + t * n * stride) =
+                make_uint2(__byte_perm(__float_as_uint(h[0]), __float_as_uint(h[1]), 0x7632),
+                           __byte_perm(__float_as_uint(h[2]), __float_as_uint(h[3]), 0x7632));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = isinf(h[e]) ? 0.0f : f[e] - h[e];
+          }
+        }
       }
     }
   }
@@ -260,17 +289,25 @@ int matvec_launch(W4Params p, cudaStream_t st) {
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
   const int n = std::min(p.rows, NT * 8);
   // warps over k until there are about 12 on every SM, of 16 weight rows each;
-  // small CTAs, so that all of them are resident and share the SMs evenly
+  // small CTAs, so that all of them are resident and share the SMs evenly.
+  // Every CTA stages x; more than 8 rows of 16 bits make that dear: then eight
+  // warps, most of them over weight rows, and more of x at a time (16384 x
+  // 8192, group 64: 8 fp32 rows 54 us against 86, 16 bf16 rows 56 against 93).
   const int tiles = (p.m + 15) / 16;
+  const bool dear = n * kTerms > 8;
+  const int fill = dear ? 8 : 12, widest = dear ? 4 : 8, room = (dear ? 96 : 32) * 1024 / (kTerms * n * 2);
   p.kw = 1;
-  while (p.kw < 8 && p.kw * 2 <= p.blocks && tiles * p.kw < 12 * current_sm_count()) p.kw *= 2;
-  const int warps = std::max(4, p.kw), rw = warps / p.kw;
-  // x in shared memory: at most 32 KB, so that several CTAs share an SM
-  const int room = 32 * 1024 / (kTerms * n * 2);
+  while (p.kw < widest && p.kw * 2 <= p.blocks && tiles * p.kw < fill * current_sm_count()) p.kw *= 2;
+  const int warps = dear ? 8 : std::max(4, p.kw), rw = warps / p.kw;
   p.stage = std::max(1, std::min(p.blocks, (room - 32) / kBlock));
   const std::size_t xs = static_cast<std::size_t>(kTerms) * n * stage_stride(p.stage) * 2;
   const std::size_t rs = static_cast<std::size_t>(warps) * 16 * (NT * 8 + 1) * 4;
   const dim3 grid(static_cast<unsigned>((tiles + rw - 1) / rw), static_cast<unsigned>((p.rows + NT * 8 - 1) / (NT * 8)));
+  if (std::max(xs, rs) > 48 * 1024) {
+    const cudaError_t rc = cudaFuncSetAttribute(w4_matvec_kernel<T, NT, GROUP>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (rc != cudaSuccess) return static_cast<int>(rc);
+  }
   w4_matvec_kernel<T, NT, GROUP><<<grid, static_cast<unsigned>(warps * 32), std::max(xs, rs), st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }

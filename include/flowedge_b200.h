@@ -284,7 +284,7 @@ typedef struct fe_engine_options {
   /* 32, 64 or 128: the Mamba in / x / out projections' weights are rounded to
    * 4 bits with one scale per that many inputs (the rule of
    * fe_w4_quantize_device); every Mamba entry point computes with them, the
-   * calls of up to 64 rows over slots from the packed form.  0: off.  A
+   * calls over slots of fewer than 128 rows from the packed form.  0: off.  A
    * structure that ends before this field (struct_size 40) reads as 0. */
   uint32_t weights4_group;
   uint32_t reserved;
