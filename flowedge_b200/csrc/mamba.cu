@@ -824,19 +824,17 @@ __global__ void act16_kernel(const float* in, long long rows, int width, __half*
     store_act16(out, i / width, width, static_cast<int>(i % width), in[i], split);
 }
 
-// Row offsets[s + 1] - 1 (row s without offsets) of every sequence with a slot
-// and at least one row -> out[s]
-__global__ void gather_slots_kernel(const float* hidden, const int* offsets, const int* slots, int n_seq,
+// Row offsets[s + 1] - 1 (row s without offsets) of every sequence that ran and
+// has rows -> out[s]; a CTA per sequence.  A slot outside the pool, or one that
+// an earlier sequence has, did not run (the rule of the operators on slots).
+__global__ void gather_slots_kernel(const float* hidden, const int* offsets, const int* slots, int n_slots,
                                     long long rows, int dm, float* out) {
-  const long long total = static_cast<long long>(n_seq) * dm;
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long q = i / dm;
-    const int c = static_cast<int>(i - q * dm);
-    const long long begin = offsets != nullptr ? offsets[q] : q, end = offsets != nullptr ? offsets[q + 1] : q + 1;
-    if (slots[q] < 0 || begin < 0 || end <= begin || end > rows) continue;
-    out[i] = hidden[(end - 1) * dm + c];
-  }
+  const int q = blockIdx.x, slot = slots[q];
+  const long long begin = offsets != nullptr ? offsets[q] : q, end = offsets != nullptr ? offsets[q + 1] : q + 1;
+  int twice = 0;
+  for (int i = threadIdx.x; i < q; i += blockDim.x) twice |= slots[i] == slot;
+  if (__syncthreads_or(twice) || slot < 0 || slot >= n_slots || begin < 0 || end <= begin || end > rows) return;
+  for (int c = threadIdx.x; c < dm; c += blockDim.x) out[static_cast<long long>(q) * dm + c] = hidden[(end - 1) * dm + c];
 }
 
 // last position of each sequence -> dense [B][dm]
@@ -1893,7 +1891,8 @@ int Mamba::reserve_slots(std::size_t n_slots, std::string& err) noexcept {
     if (!grown.init(room.total(), err)) return 2;
     auto* p = static_cast<float*>(grown.take(bytes));
     if (p == nullptr || cudaMemset(p, 0, bytes) != cudaSuccess ||
-        (kept > 0 && (synchronize_context(*ctx_) != 0 ||
+        // (a call on a stream of the caller's may still write the old pool)
+        (kept > 0 && (cudaDeviceSynchronize() != cudaSuccess ||
                       cudaMemcpy(p, pool_state_, kept, cudaMemcpyDeviceToDevice) != cudaSuccess)) ||
         cudaDeviceSynchronize() != cudaSuccess) {
       err = "slot state set-up failed";
@@ -2098,13 +2097,13 @@ int Mamba::prompt_device(const std::int32_t* tokens, std::size_t rows, const std
     err = "token copy failed";
     return 2;
   }
-  const int dm = static_cast<int>(cfg_.d_model);
   if (!embed_and_run(static_cast<long long>(rows), static_cast<int>(n_seq), offsets, slots, fresh, status, st, err)) {
     if (err.empty()) err = std::string("prompt launch failed: ") + cudaGetErrorString(cudaGetLastError());
     return 2;
   }
-  gather_slots_kernel<<<ew_grid(static_cast<long long>(n_seq) * dm, 256, *ctx_), 256, 0, st>>>(
-      out_, offsets, slots, static_cast<int>(n_seq), static_cast<long long>(rows), dm, last_hidden);
+  gather_slots_kernel<<<static_cast<unsigned>(n_seq), 256, 0, st>>>(
+      out_, offsets, slots, static_cast<int>(n_slots_), static_cast<long long>(rows), static_cast<int>(cfg_.d_model),
+      last_hidden);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 
@@ -2119,7 +2118,7 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
   }
   cudaSetDevice(ctx_->device);
   cudaStream_t st = stream != nullptr ? static_cast<cudaStream_t>(stream) : ctx_->stream;
-  const int rows = static_cast<int>(n), dm = static_cast<int>(cfg_.d_model);
+  const int rows = static_cast<int>(n);
   if ((tokens != tokens_ && cudaMemcpyAsync(tokens_, tokens, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess) ||
       (slots != slot_ids_ && cudaMemcpyAsync(slot_ids_, slots, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess)) {
     err = "token copy failed";
@@ -2163,8 +2162,8 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
       return 2;
     }
   }
-  gather_slots_kernel<<<ew_grid(static_cast<long long>(n) * dm, 256, *ctx_), 256, 0, st>>>(
-      out_, nullptr, slot_ids_, rows, rows, dm, out);
+  gather_slots_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(out_, nullptr, slot_ids_, static_cast<int>(n_slots_),
+                                                               rows, static_cast<int>(cfg_.d_model), out);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 

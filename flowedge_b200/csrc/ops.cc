@@ -145,6 +145,7 @@ int check_w4(const fe_w4_args* args, const char* call, bool reads_x, bool writes
   c.need(a.device >= -1, "unknown device");
   c.need(a.group == 32 || a.group == 64 || a.group == 128, "group is 32, 64 or 128");
   c.need(a.m >= 1 && a.m <= kMaxWidth && a.k >= 1 && a.k <= kMaxWidth, "m and k are from 1 to 2^20");
+  c.need(a.m * a.k <= std::uint64_t(1) << 38, "m k is at most 2^38");
   c.need(!per_row || a.rows <= kMaxWidth, "rows is at most 2^20");
   c.need(a.packed != nullptr && aligned(a.packed, 16), "packed is required, 16-byte aligned");
   c.need(a.scales != nullptr && aligned(a.scales, 2), "scales are required, aligned to their elements");

@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -1049,15 +1050,15 @@ DeviceScope::~DeviceScope() {
 const char* cuda_error_text(int code) noexcept { return cudaGetErrorString(static_cast<cudaError_t>(code)); }
 
 int current_sm_count() noexcept {
-  static int counts[64];
+  static std::atomic<int> counts[64];
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 148;
-  if (counts[device] == 0) {
-    int v = 0;
+  int v = counts[device].load(std::memory_order_relaxed);
+  if (v == 0) {
     if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || v <= 0) return 148;
-    counts[device] = v;
+    counts[device].store(v, std::memory_order_relaxed);
   }
-  return counts[device];
+  return v;
 }
 
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept {

@@ -441,7 +441,9 @@ uint64_t fe_engine_kernel_launches(const fe_engine* engine);
  * outside the rows, whose slot is n_slots or more, or whose slot an earlier
  * sequence of the call has, is skipped, and the FE_SEQ_* bit is set in
  * *status (an int32 in device memory that the call only adds bits to; may be
- * NULL).
+ * NULL).  Offsets that decrease set the bit too; which of the call's other
+ * sequences run is then undefined, as is what rows and slots of sequences that
+ * overlap hold, but nothing outside the call's buffers is touched.
  */
 enum { FE_DTYPE_F32 = 0, FE_DTYPE_BF16 = 1, FE_DTYPE_F16 = 2 };
 

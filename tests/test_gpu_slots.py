@@ -100,7 +100,8 @@ def test_conv_prompts(dtype, lengths, di, dc, extra, fresh):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,di,ds,dr,extra", [(1, 64, 16, 8, 0), (6, 1, 1, 1, 3), (9, 200, 4, 5, 1), (33, 129, 16, 32, 2),
-                                                 (3, 40, 32, 64, 0), (70, 1200, 12, 17, 0), (5, 100, 20, 130, 4)])
+                                                 (3, 40, 32, 64, 0), (70, 1200, 12, 17, 0), (5, 100, 20, 130, 4),
+                                                 (19, 4099, 16, 300, 0), (300, 300, 8, 512, 0), (2, 30, 9, 512, 0)])
 def test_scan_tokens(dtype, rows, di, ds, dr, extra):
     case, slots = _scan_case(rows + di, rows, di, ds, dr, dtype, rows, rows + 3, extra)
     if rows > 2:
@@ -112,7 +113,8 @@ def test_scan_tokens(dtype, rows, di, ds, dr, extra):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lengths,di,ds,dr,extra", [([1], 64, 16, 8, 0), ([0, 3, 0, 1, 70, 2, 33, 0], 136, 16, 32, 2),
                                                     ([15, 16, 17, 1, 32], 129, 8, 4, 1), ([130], 40, 32, 9, 0),
-                                                    ([300, 7], 70, 5, 3, 5), ([9, 40], 24, 16, 130, 0)])
+                                                    ([300, 7], 70, 5, 3, 5), ([9, 40], 24, 16, 130, 0),
+                                                    ([50, 1, 20], 66, 17, 300, 1), ([700], 2050, 16, 7, 0)])
 def test_scan_prompts(dtype, lengths, di, ds, dr, extra):
     n, rows = len(lengths), sum(lengths)
     case, slots = _scan_case(rows + di, rows + 4, di, ds, dr, dtype, n, n + 2, extra)

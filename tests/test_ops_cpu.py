@@ -73,7 +73,7 @@ def _w4(lib, call="fe_w4_matvec_device", **kw):
 @pytest.mark.parametrize("call", ["fe_w4_matvec_device", "fe_w4_quantize_device", "fe_w4_dequantize_device"])
 @pytest.mark.parametrize("change,said", [
     ({"size": 8}, "size"), ({"dtype": 7}, "dtype"), ({"group": 16}, "group"), ({"m": 0}, "m and k"),
-    ({"k": 2 ** 21}, "m and k"), ({"packed": 72}, "packed"), ({"scales": 0}, "scales"), ({"device": -3}, "device")])
+    ({"k": 2 ** 21}, "m and k"), ({"m": 2 ** 20, "k": 2 ** 19}, "2^38"), ({"packed": 72}, "packed"), ({"scales": 0}, "scales"), ({"device": -3}, "device")])
 def test_w4_refusals(lib, call, change, said):
     assert _w4(lib, call, **change) == 1
     text = lib.fe_engine_last_error().decode()
