@@ -386,6 +386,7 @@ int check_tokens(const fe_engine* e, const std::int32_t* tokens, std::size_t n) 
 
 namespace feb {
 void set_last_error(std::string message) { set_error(std::move(message)); }
+void set_last_error_text(const char* message) noexcept { set_error(message); }
 void clear_last_error() noexcept { clear_error(); }
 }  // namespace feb
 
@@ -1059,9 +1060,14 @@ int fe_engine_reserve_slots(fe_engine* engine, size_t n_slots) {
     set_error("Model has no backbone");
     return FE_STATUS_UNSUPPORTED_MODEL;
   }
-  std::string err;
-  if (engine->mamba->reserve_slots(n_slots, err) != 0) return slots_failed("Slot reservation", err);
-  return FE_STATUS_OK;
+  try {
+    std::string err;
+    if (engine->mamba->reserve_slots(n_slots, err) != 0) return slots_failed("Slot reservation", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_reserve_slots (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
 }
 
 int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n) {
@@ -1070,8 +1076,8 @@ int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n) {
     set_error("Invalid arguments to fe_engine_reset_slots");
     return FE_STATUS_INVALID_ARGUMENT;
   }
-  if (int rc = check_slots_engine(engine, "fe_engine_reset_slots"); rc != 0) return rc;
   try {
+    if (int rc = check_slots_engine(engine, "fe_engine_reset_slots"); rc != 0) return rc;
     if (int rc = check_slot_list(engine, slots, n); rc != 0) return rc;
     std::string err;
     if (engine->mamba->reset_slots(slots, n, err) != 0) return slots_failed("Slot reset", err);
@@ -1090,8 +1096,8 @@ int fe_engine_prompt_batch(fe_engine* engine, const int32_t* tokens, const size_
     set_error("Invalid arguments to fe_engine_prompt_batch");
     return FE_STATUS_INVALID_ARGUMENT;
   }
-  if (int rc = check_slots_engine(engine, "fe_engine_prompt_batch"); rc != 0) return rc;
   try {
+    if (int rc = check_slots_engine(engine, "fe_engine_prompt_batch"); rc != 0) return rc;
     if (int rc = check_slot_list(engine, slots, n_seq); rc != 0) return rc;
     std::size_t rows = 0;
     for (std::size_t s = 0; s < n_seq; ++s) {
@@ -1120,11 +1126,16 @@ int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t row
     set_error("Invalid arguments to fe_engine_prompt_device");
     return FE_STATUS_INVALID_ARGUMENT;
   }
-  if (int rc = check_slots_engine(engine, "fe_engine_prompt_device"); rc != 0) return rc;
-  std::string err;
-  if (engine->mamba->prompt_device(tokens, rows, offsets, slots, fresh, n_seq, last_hidden, status, stream, err) != 0)
-    return slots_failed("Mamba prompt", err);
-  return FE_STATUS_OK;
+  try {
+    if (int rc = check_slots_engine(engine, "fe_engine_prompt_device"); rc != 0) return rc;
+    std::string err;
+    if (engine->mamba->prompt_device(tokens, rows, offsets, slots, fresh, n_seq, last_hidden, status, stream, err) != 0)
+      return slots_failed("Mamba prompt", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_prompt_device (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
 }
 
 int fe_engine_step_batch(fe_engine* engine, const int32_t* tokens, const int32_t* slots, size_t n, float* out) {
@@ -1133,8 +1144,8 @@ int fe_engine_step_batch(fe_engine* engine, const int32_t* tokens, const int32_t
     set_error("Invalid arguments to fe_engine_step_batch");
     return FE_STATUS_INVALID_ARGUMENT;
   }
-  if (int rc = check_slots_engine(engine, "fe_engine_step_batch"); rc != 0) return rc;
   try {
+    if (int rc = check_slots_engine(engine, "fe_engine_step_batch"); rc != 0) return rc;
     if (int rc = check_slot_list(engine, slots, n); rc != 0) return rc;
     if (const int rc = check_tokens(engine, tokens, n); rc != 0) return rc;
     std::string err;
@@ -1153,10 +1164,16 @@ int fe_engine_step_device(fe_engine* engine, const int32_t* tokens, const int32_
     set_error("Invalid arguments to fe_engine_step_device");
     return FE_STATUS_INVALID_ARGUMENT;
   }
-  if (int rc = check_slots_engine(engine, "fe_engine_step_device"); rc != 0) return rc;
-  std::string err;
-  if (engine->mamba->step_device(tokens, slots, n, out, status, stream, err) != 0) return slots_failed("Mamba step", err);
-  return FE_STATUS_OK;
+  try {
+    if (int rc = check_slots_engine(engine, "fe_engine_step_device"); rc != 0) return rc;
+    std::string err;
+    if (engine->mamba->step_device(tokens, slots, n, out, status, stream, err) != 0)
+      return slots_failed("Mamba step", err);
+    return FE_STATUS_OK;
+  } catch (const std::exception&) {
+    set_error("Exception in fe_engine_step_device (likely OOM)");
+    return FE_STATUS_RESOURCE_EXHAUSTED;
+  }
 }
 
 void fe_engine_reset(fe_engine* engine) {

@@ -29,6 +29,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <tuple>
 
@@ -2151,11 +2152,16 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
         if (err.empty()) err = "step graph capture failed";
         return 2;
       }
-      if (slot_graphs_.size() >= 64) {  // a server's few batch sizes; not one graph for every size ever seen
-        cudaDeviceSynchronize();
-        drop_slot_graphs();
+      try {
+        if (slot_graphs_.size() >= 64) {  // a server's few batch sizes; not one graph for every size ever seen
+          cudaDeviceSynchronize();
+          drop_slot_graphs();
+        }
+        it = slot_graphs_.emplace(n, exec).first;
+      } catch (const std::exception&) {
+        cudaGraphExecDestroy(exec);
+        return 2;
       }
-      it = slot_graphs_.emplace(n, exec).first;
     }
     if (cudaGraphLaunch(it->second, st) != cudaSuccess) {
       err = std::string("step launch failed: ") + cudaGetErrorString(cudaGetLastError());

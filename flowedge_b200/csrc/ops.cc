@@ -211,7 +211,7 @@ int guarded(F body) noexcept {
     feb::clear_last_error();
     return body();
   } catch (const std::exception&) {
-    feb::clear_last_error();
+    feb::set_last_error_text("out of host memory");
     return FE_STATUS_RESOURCE_EXHAUSTED;
   }
 }

@@ -30,6 +30,7 @@ int launch_residual_norm(const fe_norm_args& a, void* stream) noexcept;
 
 // Last error of this thread (fe_engine_last_error); defined with the engine.
 void set_last_error(std::string message);
+void set_last_error_text(const char* message) noexcept;  // a literal
 void clear_last_error() noexcept;
 
 // Multiprocessors of the current device (looked up once per device).

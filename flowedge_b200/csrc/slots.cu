@@ -157,8 +157,9 @@ struct ConvParams {
 };
 
 // One thread per (token, channel): shift the window, append x, dot, SiLU.
-// Bound by the window's bytes.  FOUR: four taps and windows on 16-byte
-// boundaries, one load and one store each.
+// Bound by the window's bytes (512 x 2048 in bf16: 8.4 us, 0.70 of the measured
+// copy rate).  FOUR: four taps and windows on 16-byte boundaries, one load and
+// one store each.
 template <typename T, bool FOUR>
 __global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
   const int s = blockIdx.x;
@@ -205,7 +206,9 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
 // their arithmetic.  The first tile of a sequence reads the old window and
 // writes the new one from the sequence's last rows, so no other tile touches
 // it.  Bound by x and u, read and written once (a tile reads DC - 1 rows
-// before its own again, from L2).
+// before its own again, from L2), and in front of that by the chain of a tile:
+// search, slot, rows, stores (96 prompts, 12289 x 1024 in bf16: 21 us, 8 of
+// them the bytes).
 template <typename T, int DC, int V>
 __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p) {
   constexpr int kPairs = (V + 1) / 2, kAhead = 8;
@@ -434,7 +437,8 @@ cudaError_t allow_smem(K kernel, int bytes) {
 // in each of the scan's passes.  The products are those of fp32: every operand
 // is a sum of bf16 terms (dt_w of three; dt_in of one, two or three as it is
 // bf16, fp16 or fp32: 8, 11 or 24 bits), and all pairs of terms are multiplied
-// whose product is above 2^-25 of the whole, smallest first.
+// whose product is above 2^-25 of the whole, smallest first.  16384 x 2048, dt
+// rank 64, bf16: 72 us, the softplus of its 33 million values most of it.
 template <typename T>
 constexpr int kDtTerms = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;
 
@@ -587,7 +591,9 @@ int steps_launch(const ScanParams& p, cudaStream_t st) {
 // thread requests its states first, which are the kernel's bytes; the rest of
 // its work comes while they do.  Arithmetic on the two channels at once
 // (FFMA2).  GIVEN: dt is in the workspace (many sequences: dt_w would be read
-// again for every one of them), else the CTA makes it.
+// again for every one of them), else the CTA makes it.  Bound by the states'
+// bytes and their latency: 475 of 512 x 2048, 16 states, bf16: 38 us with the
+// dt before it, 0.53 of the measured copy rate.
 constexpr int kTokenStates = 8;  // of a thread
 
 template <typename T, int DS, int V, bool GIVEN>
@@ -912,7 +918,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
 
 // The state that enters each tile of a sequence of several, in place of the
 // tile's own end: one thread per channel and kCarryStates states walks the
-// tiles, the next kCarryAhead of them requested at a time.
+// tiles, the next kCarryAhead of them requested at a time (128 tiles x 2048
+// channels: 16 us, a latency chain).
 constexpr int kCarryStates = 2, kCarryAhead = 8, kCarryThreads = 256;
 __global__ void __launch_bounds__(kCarryThreads) scan_carry_kernel(const ScanParams p) {
   const int s = blockIdx.x, n0 = blockIdx.z * kCarryStates;
