@@ -438,7 +438,7 @@ cudaError_t allow_smem(K kernel, int bytes) {
 // is a sum of bf16 terms (dt_w of three; dt_in of one, two or three as it is
 // bf16, fp16 or fp32: 8, 11 or 24 bits), and all pairs of terms are multiplied
 // whose product is above 2^-25 of the whole, smallest first.  16384 x 2048, dt
-// rank 64, bf16: 72 us, the softplus of its 33 million values most of it.
+// rank 64, bf16: 73 us, 21 of them the bytes of dt.
 template <typename T>
 constexpr int kDtTerms = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;
 
@@ -732,7 +732,9 @@ constexpr int kPolyPairs = SUMMARY ? DS / 8 : DS / 16;
 // pipe share, and 4 DS products; dt, u, z and y pass through once.  The rows'
 // B and C sit in shared memory (every channel reads them), the next kStage
 // rows' are requested before the arithmetic; dt, u and z are requested kTok
-// rows ahead.  All arithmetic on pairs (FFMA2): states two and two.
+// rows ahead.  All arithmetic on pairs (FFMA2): states two and two.  16384 rows
+// x 2048, 16 states, bf16: the main pass adds 187 us to the call, the summaries
+// 148.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469.
 template <typename T, int DS, bool SUMMARY>
 __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt_kernel(const ScanParams p) {
   __shared__ __align__(16) float sbc[2][kStage][2 * DS];
@@ -918,8 +920,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
 
 // The state that enters each tile of a sequence of several, in place of the
 // tile's own end: one thread per channel and kCarryStates states walks the
-// tiles, the next kCarryAhead of them requested at a time (128 tiles x 2048
-// channels: 16 us, a latency chain).
+// tiles, the next kCarryAhead of them requested at a time (16384 rows x
+// 2048 channels: adds 12 us, a latency chain).
 constexpr int kCarryStates = 2, kCarryAhead = 8, kCarryThreads = 256;
 __global__ void __launch_bounds__(kCarryThreads) scan_carry_kernel(const ScanParams p) {
   const int s = blockIdx.x, n0 = blockIdx.z * kCarryStates;
