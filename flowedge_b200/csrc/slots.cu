@@ -716,11 +716,12 @@ constexpr int kTok = 4;        // rows whose dt, u and z are requested ahead
 // grows with n, as it does at the start of training, the slowest states, which
 // gain from its exactness near 1).  A row's exponentials take the MUFU unit 8
 // cycles each, the FMA pipe 18 a pair beside 6 (summary) or 8 for the pair's
-// products: two pairs of eight in the summary, one where y is made too.
-// Measured for the latter at 16384 rows x 2048 channels, DS 16, both passes
-// alike: none 466 us, one 472, two 490, three 523.
-template <int DS, bool SUMMARY>
-constexpr int kPolyPairs = SUMMARY ? DS / 8 : DS / 16;
+// products, so few pairs gain.  Measured at 16384 rows x 2048 channels and at 96
+// prompts of 12289 x 1024, DS 16, pairs of eight in the summary and in the main
+// pass: 0, 0 420 and 183 us; 1, 0 418 and 181; 1, 1 416 and 183; 2, 1 421 and
+// 186; 2, 2 440 and 194.
+template <int DS>
+constexpr int kPolyPairs = DS / 16;
 
 // One thread per channel, the states in registers, over the rows of one tile.
 // SUMMARY: the tile's sum of dt and its state from a zero start, for the tiles
@@ -733,8 +734,9 @@ constexpr int kPolyPairs = SUMMARY ? DS / 8 : DS / 16;
 // B and C sit in shared memory (every channel reads them), the next kStage
 // rows' are requested before the arithmetic; dt, u and z are requested kTok
 // rows ahead.  All arithmetic on pairs (FFMA2): states two and two.  16384 rows
-// x 2048, 16 states, bf16: the main pass adds 187 us to the call, the summaries
-// 148.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469.
+// x 2048, 16 states, bf16: the main pass adds 188 us to the call, the summaries
+// 143.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469
+// (with two state pairs on the FMA pipe in the summaries).
 template <typename T, int DS, bool SUMMARY>
 __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt_kernel(const ScanParams p) {
   __shared__ __align__(16) float sbc[2][kStage][2 * DS];
@@ -847,8 +849,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
     for (int n = 0; n < DS / 2; n += 2) {
       const float4 bq = *reinterpret_cast<const float4*>(row + 2 * n);
       const float2 e0 = __fmul2_rn(d2, an[n]), e1 = __fmul2_rn(d2, an[n + 1]);
-      const float2 a0 = n < kPolyPairs<DS, SUMMARY> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
-      const float2 a1 = n + 1 < kPolyPairs<DS, SUMMARY> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
+      const float2 a0 = n < kPolyPairs<DS> ? exp2_neg2(e0) : make_float2(ex2_approx(e0.x), ex2_approx(e0.y));
+      const float2 a1 = n + 1 < kPolyPairs<DS> ? exp2_neg2(e1) : make_float2(ex2_approx(e1.x), ex2_approx(e1.y));
       h[n] = __ffma2_rn(a0, h[n], __fmul2_rn(dtu2, make_float2(bq.x, bq.y)));
       h[n + 1] = __ffma2_rn(a1, h[n + 1], __fmul2_rn(dtu2, make_float2(bq.z, bq.w)));
       if (!SUMMARY) {
