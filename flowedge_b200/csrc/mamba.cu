@@ -1382,6 +1382,10 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
 int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noexcept {
   if (batch == 0) batch = 1;
   if (max_len == 0) max_len = 512;
+  if (batch > (std::size_t(1) << 40) / max_len) {  // (sizes in bytes stay far from 2^64)
+    err = "batch * sequence is too large";
+    return 2;
+  }
   const std::size_t tokens = batch * max_len;
   if (tokens <= cap_tokens_ && batch <= cap_batch_) return 0;
   if (step_graph_ != nullptr) {
@@ -1426,7 +1430,13 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   ws_.release();
   slot_rows_ = 0;  // the slots' calls use these buffers too
   if (!ws_.init(plan.total(), err)) {
-    cap_tokens_ = 0;
+    // back to the buffers that there were, and the decode state
+    const std::size_t old_tokens = cap_tokens_, old_batch = cap_batch_;
+    state_ = nullptr;
+    cap_tokens_ = cap_batch_ = 0;
+    std::string again;
+    if (old_tokens > 0 && reserve(old_batch, old_tokens / old_batch, again) == 0)
+      cudaMemcpy(state_, saved.data(), saved.size() * 4, cudaMemcpyHostToDevice);
     return 2;
   }
   tokens_ = ws_.take_n<int>(rows);
@@ -1475,7 +1485,9 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   if (pinned_floats_ < need) {
     if (pinned_ != nullptr) cudaFreeHost(pinned_);
     pinned_ = nullptr;
+    pinned_floats_ = 0;
     if (counted_host_malloc(reinterpret_cast<void**>(&pinned_), need * 4) != cudaSuccess) {
+      cap_tokens_ = 0;
       err = "pinned host allocation failed";
       return 2;
     }
@@ -1807,6 +1819,10 @@ bool Mamba::record_step(cudaStream_t st, std::string& err) {
 // Streaming decode of one token (mamba.cc:317-382): the conv window and scan
 // state stay on the device; the whole step replays as one CUDA graph.
 int Mamba::step(std::int32_t token, float* out, std::string& err) noexcept {
+  if (cap_tokens_ == 0) {
+    err = "no workspace (an earlier reservation failed)";
+    return 2;
+  }
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
   if (step_graph_ == nullptr) {

@@ -10,7 +10,7 @@ its tensors' device and returns; it keeps nothing.  A refused argument raises
 FlowEdgeError (status 1) before anything is launched.  These are inference
 operators: tensors that require a gradient are refused while gradients are
 being recorded.  Outputs share no element with inputs; states are updated in
-place.  With `out` given, rows of skipped sequences and rows behind the last
+place, which autograd's record of changed tensors does not see.  With `out` given, rows of skipped sequences and rows behind the last
 sequence keep what they held; without it they are undefined.
 """
 
@@ -310,9 +310,12 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
     if out is None:
         out = torch.empty_like(x)
     y_ld = _matrix(out, "out", shape, dtype, device)
-    args = _NORM.pack(_NORM.size, device, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
-                      x.data_ptr(), _ptr(post_weight), _ptr(gate), residual.data_ptr(), weight.data_ptr(),
-                      out.data_ptr(), scale, eps)
+    try:
+        args = _NORM.pack(_NORM.size, device, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
+                          x.data_ptr(), _ptr(post_weight), _ptr(gate), residual.data_ptr(), weight.data_ptr(),
+                          out.data_ptr(), scale, eps)
+    except (struct.error, OverflowError):
+        _refuse("scale and eps are numbers of float32")
     rc = load_library().fe_residual_norm_device(args, _raw_stream(device))
     if rc:
         _failed(rc)

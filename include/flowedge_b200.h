@@ -345,7 +345,10 @@ int fe_engine_run_device(fe_engine* engine, const int32_t* tokens, size_t batch,
  * fe_engine_reserve_slots makes room for slots 0 .. n_slots - 1 (zero states;
  * a larger pool keeps the states of a smaller one) and, together with
  * fe_engine_reserve_batch and max_batch x max_sequence, is what allocates.
- * Slots are apart from the one state of fe_engine_step. */
+ * Slots are apart from the one state of fe_engine_step.  Growth moves buffers:
+ * a graph in which the caller captured one of the calls below is no longer
+ * valid behind it (a prompt_batch or step_batch of more rows than there is
+ * room for grows too). */
 int fe_engine_reserve_slots(fe_engine* engine, size_t n_slots);
 /* Zero states for n slots. */
 int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n);

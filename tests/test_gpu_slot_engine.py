@@ -190,6 +190,25 @@ def test_growth_keeps_states_and_warm_calls_do_not_allocate(engines):
     e.close()
 
 
+def test_growth_beyond_the_device_leaves_everything_usable(engines):
+    """No device holds the batch: the call says so, and the buffers, the single stream's state and the slots' stay."""
+    _, model, path = engines("odd")
+    e = Engine(path, threads=0, device=0, precision="fp32", max_sequence=16)
+    e.reserve_slots(2)
+    tokens = np.random.default_rng(6).integers(0, 17, 24).astype(np.int32)
+    for t in tokens[:5]:
+        e.step(int(t))
+    e.prompt_batch([tokens[:8]], [1])
+    for batch in (1 << 30, 1 << 62):
+        with pytest.raises(FlowEdgeError, match="status 2"):
+            e.reserve_batch(batch)
+    np.testing.assert_allclose(e.step(int(tokens[5])), model.run(tokens[:6])[-1], atol=1e-3)
+    np.testing.assert_allclose(e.step_batch(tokens[8:9], [1])[0], model.run(tokens[:9])[-1], atol=1e-3)
+    np.testing.assert_allclose(e.prompt_batch([tokens], [0])[0], model.run(tokens)[-1], atol=1e-3)  # grows
+    np.testing.assert_allclose(e.step(int(tokens[6])), model.run(tokens[:7])[-1], atol=1e-3)
+    e.close()
+
+
 def test_slot_refusals(engines, golden):
     e, _, path = engines("odd")
     fresh = Engine(path, threads=0, device=0, precision="fp32")

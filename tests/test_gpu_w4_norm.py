@@ -163,3 +163,12 @@ def test_norm_refusals_and_nothing_to_do():
         with pytest.raises(ops.FlowEdgeError, match="status 1"):
             call()
     assert ops.residual_norm(x[:0], r.detach()[:0], w).shape == (0, 64)
+
+
+@pytest.mark.parametrize("scale,eps", [(1e300, 1e-5), (1.0, 1e300), ("1", 1e-5), (1.0, float("nan"))])
+def test_norm_refuses_what_is_no_float32(scale, eps):
+    x, r, w = torch.randn(4, 64, device="cuda"), torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    before = r.clone()
+    with pytest.raises(ops.FlowEdgeError, match="status 1"):
+        ops.residual_norm(x, r, w, scale=scale, eps=eps)
+    assert torch.equal(r, before)
