@@ -3,6 +3,7 @@
 // launch functions of ops.h.  Host C++23, no CUDA headers.
 #include "ops.h"
 
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -177,7 +178,8 @@ int check_norm(const fe_norm_args* args) {
   c.need(a.device >= -1, "unknown device");
   c.need(a.rows <= kMaxRows, "rows is at most 2^30");
   c.need(a.dim >= 1 && a.dim <= 16384, "dim is from 1 to 16384");
-  c.need(a.eps >= 0.0f, "eps is not negative");
+  c.need(std::isfinite(a.scale), "scale is finite");
+  c.need(a.eps >= 0.0f && std::isfinite(a.eps), "eps is finite and not negative");
   c.need(a.weight != nullptr && aligned(a.weight, 4) && aligned(a.post_weight, 4), "weight is required, 4-byte aligned");
   if (int rc = c.done(); rc != 0 || a.rows == 0) return rc;
   c.need(a.x != nullptr && a.residual != nullptr && a.out != nullptr, "x, residual and out are required");

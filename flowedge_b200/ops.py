@@ -10,8 +10,9 @@ its tensors' device and returns; it keeps nothing.  A refused argument raises
 FlowEdgeError (status 1) before anything is launched.  These are inference
 operators: tensors that require a gradient are refused while gradients are
 being recorded.  Outputs share no element with inputs; states are updated in
-place, which autograd's record of changed tensors does not see.  With `out` given, rows of skipped sequences and rows behind the last
-sequence keep what they held; without it they are undefined.
+place, which autograd's record of changed tensors does not see.  With `out`
+given, rows of skipped sequences and rows behind the last sequence keep what
+they held; without it they are undefined.
 """
 
 from __future__ import annotations
@@ -314,8 +315,8 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
         args = _NORM.pack(_NORM.size, device, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
                           x.data_ptr(), _ptr(post_weight), _ptr(gate), residual.data_ptr(), weight.data_ptr(),
                           out.data_ptr(), scale, eps)
-    except (struct.error, OverflowError):
-        _refuse("scale and eps are numbers of float32")
+    except struct.error:
+        _refuse("scale and eps are numbers")
     rc = load_library().fe_residual_norm_device(args, _raw_stream(device))
     if rc:
         _failed(rc)

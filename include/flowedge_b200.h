@@ -556,7 +556,7 @@ int fe_w4_dequantize_device(const fe_w4_args* args, void* stream);
  * x, gate and out are `dtype`, the residual (updated in place) fp32 or
  * `dtype`, weights fp32; sums and the norm's input are fp32, before the
  * residual's rounding.  gate_ld 0 gives every row the same gate.  dim 1 ..
- * 16384.  out, residual, x and gate share no element. */
+ * 16384, scale and eps finite.  out, residual, x and gate share no element. */
 typedef struct fe_norm_args {
   uint32_t struct_size; /* sizeof(fe_norm_args) */
   int32_t device;
