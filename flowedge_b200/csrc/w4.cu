@@ -13,8 +13,7 @@
 // bytes per block of k, and the blocks are dealt out to several warps where
 // there are too few rows of weights to fill the GPU.  16384 x 8192, one bf16
 // row: 27 us, 0.40 of the measured copy rate (a copy without the unpacking
-// took 22 us, so more than that is lost in reading 64-byte pieces of rows);
-// 32 rows 100 us.
+// took 22 us); 32 rows 100 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
