@@ -13,8 +13,7 @@ own = False
 
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 SIZES = {"fp32": 4, "bf16": 2, "fp16": 2}
-# packed 4-bit weights: a row is blocks of 128 elements in 16 words of 32 bits; the word at place 4 t + j of a block holds
-# the eight elements from 32 j + 8 t on, element NIBBLE[i] of them in nibble i
+# nibble i of a 32-bit word of 4-bit weights holds element NIBBLE[i] of the word's eight
 NIBBLE = (0, 2, 4, 6, 1, 3, 5, 7)
 
 
@@ -152,11 +151,12 @@ def prepare(case, seed):
         s["state"] = normal(n_slots, ds, di, scale=0.5)
     elif case["op"] == "w4":
         m, k, group = case["m"], case["k"], case["group"]
-        blocks = (k + 127) // 128
-        q = torch.randint(0, 16, (m, blocks * 128), generator=cg, device="cuda", dtype=torch.uint8)
+        words = (k + 31) // 32 * 4
+        q = torch.randint(0, 16, (m, words * 8), generator=cg, device="cuda", dtype=torch.int64)
         q[:, k:] = 8  # behind the last column: zero
-        q = q.view(m, blocks, 4, 4, 8).transpose(2, 3)[..., list(NIBBLE)]
-        s["packed"] = (q[..., 0::2] | (q[..., 1::2] << 4)).reshape(m, blocks * 64).contiguous()
+        q = q.view(m, words, 8)[:, :, list(NIBBLE)]
+        byte = q[:, :, 0::2] | (q[:, :, 1::2] << 4)
+        s["packed"] = byte.to(torch.uint8).reshape(m, words * 4).contiguous()
         s["scales"] = uniform(m, (k + group - 1) // group, lo=0.5, hi=1.5).mul_(0.2 * k ** -0.5).half()
         s["x"] = normal(case["rows"], k).to(dt)
     else:
@@ -172,9 +172,9 @@ def prepare(case, seed):
 def _unpack(packed, k):
     """Whole numbers 0 .. 15 of packed 4-bit weights, [m][k]."""
     m = packed.shape[0]
-    nib = torch.stack([packed & 15, packed >> 4], -1).view(m, -1, 4, 4, 8)
+    nib = torch.stack([packed & 15, packed >> 4], -1).view(m, -1, 8)
     place = torch.tensor(NIBBLE, device=packed.device).argsort()
-    return nib[..., place].transpose(2, 3).reshape(m, -1)[:, :k]
+    return nib[:, :, place].reshape(m, -1)[:, :k]
 
 
 def _bounds(state, rows):
@@ -338,9 +338,8 @@ def exact(case, seed):
         word = s["packed"].view(torch.int32).long()  # eight elements to a word
         m = word.shape[0]
         w = torch.zeros(m, word.shape[1] * 8, dtype=torch.float64, device="cuda")
-        for p in range(16):  # the words' places in a block of 128
-            for i, place in enumerate(NIBBLE):
-                w[:, p % 4 * 32 + p // 4 * 8 + place::128] = ((word[:, p::16] >> (4 * i)) & 15).double() - 8.0
+        for i, place in enumerate(NIBBLE):
+            w[:, place::8] = ((word >> (4 * i)) & 15).double() - 8.0
         for j in range(s["scales"].shape[1]):
             w[:, j * group:(j + 1) * group] *= s["scales"][:, j:j + 1].double()
         return torch.einsum("rk,mk->rm", x, w[:, :k])
