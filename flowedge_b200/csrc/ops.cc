@@ -4,6 +4,8 @@
 #include "ops.h"
 
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 #include <exception>
 #include <string>
 
@@ -135,11 +137,15 @@ int check_scan(const fe_scan_args* args, const char* call, bool sizes_only) {
   return c.done();
 }
 
-int check_w4(const fe_w4_args* args, const char* call, bool reads_x, bool writes_y, bool per_row) {
+// Reads the caller's structure into `a` (one that ends before the layout has
+// it zero) and checks it.
+int check_w4(const fe_w4_args* args, fe_w4_args& a, const char* call, bool reads_x, bool writes_y, bool per_row) {
+  constexpr std::size_t kFirst = offsetof(fe_w4_args, layout);
   Checks c(call);
-  c.need(args != nullptr && args->struct_size >= sizeof(fe_w4_args), "args are missing or of another size");
+  c.need(args != nullptr && args->struct_size >= kFirst, "args are missing or of another size");
   if (int rc = c.done(); rc != 0) return rc;
-  const fe_w4_args& a = *args;
+  a = {};
+  std::memcpy(&a, args, args->struct_size < sizeof(a) ? kFirst : sizeof(a));
   const std::uint64_t e = dtype_bytes(a.dtype);
   const std::uint64_t x_rows = per_row ? a.rows : a.m, y_rows = per_row ? a.rows : a.m, y_width = per_row ? a.m : a.k;
   c.need(e != 0, "unknown dtype");
@@ -148,6 +154,7 @@ int check_w4(const fe_w4_args* args, const char* call, bool reads_x, bool writes
   c.need(a.m >= 1 && a.m <= kMaxWidth && a.k >= 1 && a.k <= kMaxWidth, "m and k are from 1 to 2^20");
   c.need(a.m * a.k <= std::uint64_t(1) << 38, "m k is at most 2^38");
   c.need(!per_row || a.rows <= kMaxWidth, "rows is at most 2^20");
+  c.need(a.layout <= FE_W4_ROWS && a.reserved == 0, "unknown layout");
   c.need(a.packed != nullptr && aligned(a.packed, 16), "packed is required, 16-byte aligned");
   c.need(a.scales != nullptr && aligned(a.scales, 2), "scales are required, aligned to their elements");
   if (int rc = c.done(); rc != 0) return rc;
@@ -274,25 +281,28 @@ int fe_selective_scan_device(const fe_scan_args* args, void* stream) {
 int fe_w4_matvec_device(const fe_w4_args* args, void* stream) {
   constexpr const char* kCall = "fe_w4_matvec_device";
   return guarded([&] {
-    if (int rc = check_w4(args, kCall, true, true, true); rc != 0) return rc;
-    if (args->rows == 0) return static_cast<int>(FE_STATUS_OK);
-    return on_device(args->device, kCall, [&] { return feb::launch_w4_matvec(*args, stream); });
+    fe_w4_args a;
+    if (int rc = check_w4(args, a, kCall, true, true, true); rc != 0) return rc;
+    if (a.rows == 0) return static_cast<int>(FE_STATUS_OK);
+    return on_device(a.device, kCall, [&] { return feb::launch_w4_matvec(a, stream); });
   });
 }
 
 int fe_w4_quantize_device(const fe_w4_args* args, void* stream) {
   constexpr const char* kCall = "fe_w4_quantize_device";
   return guarded([&] {
-    if (int rc = check_w4(args, kCall, true, false, false); rc != 0) return rc;
-    return on_device(args->device, kCall, [&] { return feb::launch_w4_quantize(*args, stream); });
+    fe_w4_args a;
+    if (int rc = check_w4(args, a, kCall, true, false, false); rc != 0) return rc;
+    return on_device(a.device, kCall, [&] { return feb::launch_w4_quantize(a, stream); });
   });
 }
 
 int fe_w4_dequantize_device(const fe_w4_args* args, void* stream) {
   constexpr const char* kCall = "fe_w4_dequantize_device";
   return guarded([&] {
-    if (int rc = check_w4(args, kCall, false, true, false); rc != 0) return rc;
-    return on_device(args->device, kCall, [&] { return feb::launch_w4_dequantize(*args, stream); });
+    fe_w4_args a;
+    if (int rc = check_w4(args, a, kCall, false, true, false); rc != 0) return rc;
+    return on_device(a.device, kCall, [&] { return feb::launch_w4_dequantize(a, stream); });
   });
 }
 

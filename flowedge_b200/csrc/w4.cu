@@ -9,6 +9,14 @@
 // weight is ever rounded.  x enters as it is (16-bit types) or as three bf16
 // terms that add up to its 24 bits (fp32).
 //
+// Two layouts of the packed words (FE_W4_BLOCKS, FE_W4_ROWS) differ in what a
+// lane reads: a fragment's four lanes must hold words of one group.  In blocks
+// a lane's four words, one of each piece of 32 elements, lie side by side.  In
+// rows it reads as many side by side as a group has pieces (16, 8 or 4 bytes
+// at a time), and the eights of x are staged in the order in which it does.
+// One bf16 row x 16384 x 8192: groups of 128 25 us in either, of 64 27 in
+// blocks and 30 in rows, of 32 34 and 46.
+//
 // Bound by the weights' bytes for few rows; a warp reads 16 weight rows x 64
 // bytes per block of k, and the blocks are dealt out to several warps where
 // there are too few rows of weights to fill the GPU.  16384 x 8192, one bf16
@@ -31,11 +39,12 @@ constexpr int kBlock = 128;  // elements of a packed block of 64 bytes
 
 struct W4Params {
   const void* x;
-  const uint4* packed;  // [m][blocks][4]
+  const uint32_t* packed;  // [m][words]
   const __half* scales;
   void* y;
   long long x_ld, y_ld;
   int rows, m, k, blocks, groups;
+  int words;   // of a row: 16 to a block, or four to every 32 elements (rows)
   int kw;      // warps that share a tile of 16 weight rows, each with part of k
   int stage;   // blocks of x staged in shared memory at a time
 };
@@ -74,13 +83,24 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&v)[4]) {
   }
 }
 
+// Where the eight elements from 8 i on of a block are staged: place 4 j + t for
+// those that lane t multiplies with its word j.
+template <int GROUP, bool ROWS>
+__device__ __forceinline__ int staged_eight(int i) {
+  if constexpr (!ROWS || GROUP == 32) return i;
+  if constexpr (GROUP == 64) return (i & 8) | (i & 1) << 2 | (i >> 1 & 3);
+  return (i & 3) << 2 | i >> 2;
+}
+
 // Stages rows r0 .. r0 + n - 1, columns of `blocks` packed blocks from block
-// b0 on, as TERMS planes of [n][stride] 16-bit values; zero behind column k.
+// b0 on, as TERMS planes of [n][stride] 16-bit values, the eights of a block in
+// their staged order; zero behind column k.
 // A warp a row, a lane four columns at a time (16 or 8 bytes where rows start
 // on as many), kAhead of those requested together.
-template <typename T, int TERMS>
+template <typename T, int TERMS, int GROUP, bool ROWS>
 __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0, int blocks, unsigned short* sx, int stride) {
   constexpr int kAhead = 4;
+  const auto place = [](int c) { return (c & ~(kBlock - 1)) | staged_eight<GROUP, ROWS>(c >> 3 & 15) << 3 | (c & 7); };
   if constexpr (TERMS == 1) {
     // whole 16 bytes as they are, where rows start on them and k ends there
     if (p.k % 8 == 0 && p.x_ld % 8 == 0 && reinterpret_cast<std::uintptr_t>(p.x) % 16 == 0) {
@@ -88,7 +108,7 @@ __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0
       for (int i = threadIdx.x; i < n * pieces; i += blockDim.x) {
         const int r = i / pieces, c = (i - r * pieces) * 8;
         const T* src = static_cast<const T*>(p.x) + (r0 + r) * p.x_ld + b0 * kBlock + c;
-        *reinterpret_cast<uint4*>(sx + r * stride + c) =
+        *reinterpret_cast<uint4*>(sx + r * stride + place(c)) =
             b0 * kBlock + c < p.k ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
       }
       return;
@@ -120,7 +140,7 @@ __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0
       for (int i = 0; i < kAhead; ++i) {
         const int c = c0 + 128 * share * i;
         if (c >= width) break;
-        unsigned short* dst = sx + r * stride + c;
+        unsigned short* dst = sx + r * stride + place(c);
         if constexpr (TERMS == 1) {
           *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(&v[i]);
         } else {
@@ -150,8 +170,9 @@ __host__ __device__ constexpr int stage_stride(int blocks) { return blocks * kBl
 // A CTA has 4 or 8 warps: p.kw of them share a tile of 16 weight rows, each with
 // a run of the blocks of k, and join their sums through shared memory in
 // order.  A warp has kSet blocks in its arithmetic and the next kSet on their
-// way; a last odd block and one whose last groups do not exist come one by one.
-template <typename T, int NT, int GROUP>
+// way; a last odd block and one whose last groups or words do not exist come
+// one by one.
+template <typename T, int NT, int GROUP, bool ROWS>
 __global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
   constexpr bool kBf16 = !std::is_same_v<T, __half>;
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
@@ -173,17 +194,31 @@ __global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
     __half sa[kPer], sb[kPer];
   };
   for (int b0 = 0; b0 < p.blocks; b0 += p.stage) {
-    // this warp's blocks of the stage: [first, end), with all of their groups up to `whole`
+    // this warp's blocks of the stage: [first, end), with all of their groups and words up to `whole`
     const int nb = min(p.stage, p.blocks - b0), share = (nb + p.kw - 1) / p.kw;
     const int first = min(wk * share, nb), end = min(first + share, nb);
-    const int whole = max(first, min(end, p.groups / kPer - b0));
-    const uint4* wa = p.packed + (static_cast<long long>(ra) * p.blocks + b0 + first) * 4 + t;
-    const uint4* wb = p.packed + (static_cast<long long>(rb) * p.blocks + b0 + first) * 4 + t;
+    const int whole = max(first, min(end, min(p.groups / kPer, p.words / 16) - b0));
+    const uint32_t* wa = p.packed + static_cast<long long>(ra) * p.words + (b0 + first) * 16;
+    const uint32_t* wb = p.packed + static_cast<long long>(rb) * p.words + (b0 + first) * 16;
     const __half* sa = p.scales + static_cast<long long>(ra) * p.groups + (b0 + first) * kPer;
     const __half* sb = p.scales + static_cast<long long>(rb) * p.groups + (b0 + first) * kPer;
-    auto request = [&](Block& blk, int i, int groups) {  // block i from the pointers
-      blk.a = __ldg(wa + i * 4);
-      blk.b = __ldg(wb + i * 4);
+    // this lane's words of a block of which `words` exist (a multiple of four); the rest are zero weights
+    auto words_of = [&](const uint32_t* w, int words) {
+      constexpr uint32_t kZero = 0x88888888u;
+      if constexpr (!ROWS || GROUP == 128) {
+        return !ROWS || 4 * t < words ? __ldg(reinterpret_cast<const uint4*>(w) + t) : make_uint4(kZero, kZero, kZero, kZero);
+      } else if constexpr (GROUP == 64) {
+        const uint2 none = make_uint2(kZero, kZero), *at = reinterpret_cast<const uint2*>(w) + t;
+        const uint2 lo = 2 * t < words ? __ldg(at) : none, hi = 8 + 2 * t < words ? __ldg(at + 4) : none;
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+      } else {
+        return make_uint4(__ldg(w + t), 4 < words ? __ldg(w + 4 + t) : kZero, 8 < words ? __ldg(w + 8 + t) : kZero,
+                          12 < words ? __ldg(w + 12 + t) : kZero);
+      }
+    };
+    auto request = [&](Block& blk, int i, int groups, int words) {  // block i from the pointers
+      blk.a = words_of(wa + i * 16, words);
+      blk.b = words_of(wb + i * 16, words);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         blk.sa[j] = j < groups ? sa[i * kPer + j] : __half(0.0f);
@@ -228,8 +263,8 @@ __global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
       }
     };
     auto advance = [&](int blocks) {
-      wa += blocks * 4;
-      wb += blocks * 4;
+      wa += blocks * 16;
+      wb += blocks * 16;
       sa += blocks * kPer;
       sb += blocks * kPer;
 #pragma unroll
@@ -239,26 +274,26 @@ __global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
     int sets = (whole - first) / kSet;
     if (sets > 0)
 #pragma unroll
-      for (int i = 0; i < kSet; ++i) request(one[i], i, kPer);
+      for (int i = 0; i < kSet; ++i) request(one[i], i, kPer, 16);
     if (b0 > 0) __syncthreads();
-    stage_x<T, kTerms>(p, r0, n, b0, nb, sx, stride);
+    stage_x<T, kTerms, GROUP, ROWS>(p, r0, n, b0, nb, sx, stride);
     __syncthreads();
     for (; sets > 0; sets -= 2) {
       if (sets > 1)
 #pragma unroll
-        for (int i = 0; i < kSet; ++i) request(two[i], kSet + i, kPer);
+        for (int i = 0; i < kSet; ++i) request(two[i], kSet + i, kPer, 16);
 #pragma unroll
       for (int i = 0; i < kSet; ++i) consume(one[i], i);
       if (sets > 2)
 #pragma unroll
-        for (int i = 0; i < kSet; ++i) request(one[i], 2 * kSet + i, kPer);
+        for (int i = 0; i < kSet; ++i) request(one[i], 2 * kSet + i, kPer, 16);
       if (sets > 1)
 #pragma unroll
         for (int i = 0; i < kSet; ++i) consume(two[i], kSet + i);
       advance(min(sets, 2) * kSet);
     }
     for (int b = first + (whole - first) / kSet * kSet; b < end; ++b) {
-      request(one[0], 0, min(kPer, p.groups - (b0 + b) * kPer));
+      request(one[0], 0, min(kPer, p.groups - (b0 + b) * kPer), min(16, p.words - (b0 + b) * 16));
       consume(one[0], 0);
       advance(1);
     }
@@ -286,7 +321,7 @@ __global__ void __launch_bounds__(256, 2) w4_matvec_kernel(const W4Params p) {
   }
 }
 
-template <typename T, int NT, int GROUP>
+template <typename T, int NT, int GROUP, bool ROWS>
 int matvec_launch(W4Params p, cudaStream_t st) {
   constexpr int kTerms = std::is_same_v<T, float> ? 3 : 1;
   const int n = std::min(p.rows, NT * 8);
@@ -306,25 +341,38 @@ int matvec_launch(W4Params p, cudaStream_t st) {
   const std::size_t rs = static_cast<std::size_t>(warps) * 16 * (NT * 8 + 1) * 4;
   const dim3 grid(static_cast<unsigned>((tiles + rw - 1) / rw), static_cast<unsigned>((p.rows + NT * 8 - 1) / (NT * 8)));
   if (std::max(xs, rs) > 48 * 1024) {
-    const cudaError_t rc = cudaFuncSetAttribute(w4_matvec_kernel<T, NT, GROUP>,
+    const cudaError_t rc = cudaFuncSetAttribute(w4_matvec_kernel<T, NT, GROUP, ROWS>,
                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (rc != cudaSuccess) return static_cast<int>(rc);
   }
-  w4_matvec_kernel<T, NT, GROUP><<<grid, static_cast<unsigned>(warps * 32), std::max(xs, rs), st>>>(p);
+  w4_matvec_kernel<T, NT, GROUP, ROWS><<<grid, static_cast<unsigned>(warps * 32), std::max(xs, rs), st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, int GROUP>
+template <typename T, int GROUP, bool ROWS>
 int matvec_rows(const W4Params& p, cudaStream_t st) {
-  if (p.rows <= 8) return matvec_launch<T, 1, GROUP>(p, st);
-  if (p.rows <= 16) return matvec_launch<T, 2, GROUP>(p, st);
-  return matvec_launch<T, 4, GROUP>(p, st);
+  if (p.rows <= 8) return matvec_launch<T, 1, GROUP, ROWS>(p, st);
+  if (p.rows <= 16) return matvec_launch<T, 2, GROUP, ROWS>(p, st);
+  return matvec_launch<T, 4, GROUP, ROWS>(p, st);
+}
+
+template <typename T, bool ROWS>
+int matvec_group(const W4Params& p, std::uint32_t group, cudaStream_t st) {
+  if (group == 32) return matvec_rows<T, 32, ROWS>(p, st);
+  if (group == 64) return matvec_rows<T, 64, ROWS>(p, st);
+  return matvec_rows<T, 128, ROWS>(p, st);
+}
+
+// Place in its row of the word that holds element c.
+__device__ __forceinline__ int word_of(int c, bool in_rows) {
+  return in_rows ? c / 8 : c / kBlock * 16 + c % 32 / 8 * 4 + c % kBlock / 32;
 }
 
 // One warp per group: the scale, then the group's words.
 template <typename T>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* __restrict__ w, long long ld, int m, int k, int group,
-                                                          int groups, int blocks, uint32_t* packed, __half* scales) {
+                                                          int groups, int blocks, int words, bool in_rows,
+                                                          uint32_t* packed, __half* scales) {
   const int lane = threadIdx.x & 31;
   const long long id = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) >> 5;
   const int per = kBlock / group;
@@ -350,39 +398,40 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* __restrict__ 
       }
       word |= static_cast<uint32_t>(q) << (4 * ((e >> 1) + (e & 1) * 4));
     }
-    const int at = grp * group + lane * 8, blk = at / kBlock, j = at % kBlock / 32, t = at % 32 / 8;
-    packed[(static_cast<long long>(row) * blocks + blk) * 16 + 4 * t + j] = word;
+    const int at = word_of(grp * group + lane * 8, in_rows);
+    if (at < words) packed[static_cast<long long>(row) * words + at] = word;
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __restrict__ packed,
                                                             const __half* __restrict__ scales, int m, int k, int group,
-                                                            int groups, int blocks, T* w, long long ld) {
+                                                            int groups, int words, bool in_rows, T* w, long long ld) {
   const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
   if (i >= static_cast<long long>(m) * k) return;
   const int row = static_cast<int>(i / k), c = static_cast<int>(i - static_cast<long long>(row) * k);
-  const int blk = c / kBlock, j = c % kBlock / 32, t = c % 32 / 8, e = c % 8;
-  const uint32_t word = packed[(static_cast<long long>(row) * blocks + blk) * 16 + 4 * t + j];
+  const int e = c % 8;
+  const uint32_t word = packed[static_cast<long long>(row) * words + word_of(c, in_rows)];
   const int q = static_cast<int>(word >> (4 * ((e >> 1) + (e & 1) * 4)) & 15u) - 8;
   w[row * ld + c] = from_f32<T>(static_cast<float>(q) * __half2float(scales[static_cast<long long>(row) * groups + c / group]));
 }
 
 int blocks_of(const fe_w4_args& a) { return static_cast<int>((a.k + kBlock - 1) / kBlock); }
+int words_of(const fe_w4_args& a) {
+  return a.layout == FE_W4_ROWS ? static_cast<int>((a.k + 31) / 32 * 4) : blocks_of(a) * 16;
+}
 int groups_of(const fe_w4_args& a) { return static_cast<int>((a.k + a.group - 1) / a.group); }
 
 }  // namespace
 
 int launch_w4_matvec(const fe_w4_args& a, void* stream) noexcept {
-  const W4Params p{a.x, static_cast<const uint4*>(a.packed), static_cast<const __half*>(a.scales), a.y, a.x_ld, a.y_ld,
+  const W4Params p{a.x, static_cast<const uint32_t*>(a.packed), static_cast<const __half*>(a.scales), a.y, a.x_ld, a.y_ld,
                    static_cast<int>(a.rows), static_cast<int>(a.m), static_cast<int>(a.k), blocks_of(a), groups_of(a),
-                   1, 1};
+                   words_of(a), 1, 1};
   const auto st = static_cast<cudaStream_t>(stream);
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.group == 32) return matvec_rows<T, 32>(p, st);
-    if (a.group == 64) return matvec_rows<T, 64>(p, st);
-    return matvec_rows<T, 128>(p, st);
+    return a.layout == FE_W4_ROWS ? matvec_group<T, true>(p, a.group, st) : matvec_group<T, false>(p, a.group, st);
   });
 }
 
@@ -392,7 +441,8 @@ int launch_w4_quantize(const fe_w4_args& a, void* stream) noexcept {
     using T = decltype(t);
     w4_quantize_kernel<T><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const T*>(a.x), a.x_ld, static_cast<int>(a.m), static_cast<int>(a.k), static_cast<int>(a.group),
-        groups_of(a), blocks_of(a), static_cast<uint32_t*>(a.packed), static_cast<__half*>(a.scales));
+        groups_of(a), blocks_of(a), words_of(a), a.layout == FE_W4_ROWS, static_cast<uint32_t*>(a.packed),
+        static_cast<__half*>(a.scales));
     return static_cast<int>(cudaGetLastError());
   });
 }
@@ -403,7 +453,8 @@ int launch_w4_dequantize(const fe_w4_args& a, void* stream) noexcept {
     using T = decltype(t);
     w4_dequantize_kernel<T><<<static_cast<unsigned>((total + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint32_t*>(a.packed), static_cast<const __half*>(a.scales), static_cast<int>(a.m),
-        static_cast<int>(a.k), static_cast<int>(a.group), groups_of(a), blocks_of(a), static_cast<T*>(a.y), a.y_ld);
+        static_cast<int>(a.k), static_cast<int>(a.group), groups_of(a), words_of(a), a.layout == FE_W4_ROWS, static_cast<T*>(a.y),
+        a.y_ld);
     return static_cast<int>(cudaGetLastError());
   });
 }

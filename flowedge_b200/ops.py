@@ -33,7 +33,9 @@ BAD_OFFSETS, BAD_SLOT, DUPLICATE_SLOT = 1, 2, 4
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _CONV = struct.Struct("@IiII4Q3q9P")
 _SCAN = struct.Struct("@IiII5Q5q14PQ")
-_W4 = struct.Struct("@IiII3Q2q4P")
+_W4 = struct.Struct("@IiII3Q2q4P")  # and behind it the layout
+_W4_LAYOUT = {torch.int8: struct.pack("@II", 0, 0), torch.uint8: struct.pack("@II", 1, 0)}
+_W4_SIZE = _W4.size + 8
 _NORM = struct.Struct("@IiII2Q4q6Pff")
 
 
@@ -213,26 +215,36 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     return out
 
 
-def _w4_shapes(m: int, k: int, group: int) -> tuple:
+# Packed 4-bit weights come in two layouts, which their type tells apart: uint8 has a row's words in the order of their
+# elements, int8 has them in blocks of 128 elements in the order in which the products read them.
+
+
+def _w4_shapes(m: int, k: int, group: int, packed_dtype) -> tuple:
     if group not in (32, 64, 128):
         _refuse(f"group is 32, 64 or 128, not {group}")
-    return (m, (k + 127) // 128 * 64), (m, (k + group - 1) // group)
+    width = (k + 31) // 32 * 16 if packed_dtype is torch.uint8 else (k + 127) // 128 * 64
+    return (m, width), (m, (k + group - 1) // group)
 
 
-def w4_quantize(weight, group: int = 64) -> tuple:
+def w4_quantize(weight, group: int = 64, *, layout: str = "blocks") -> tuple:
     """(packed, scales) of a finite weight matrix [m, k]: 4 bits per element, one float16 scale per `group` of k.
 
-    packed is uint8 [m, ceil(k / 128) * 64] in the layout of include/flowedge_b200.h (fe_w4_args), scales
-    [m, ceil(k / group)].
+    packed is int8 [m, ceil(k / 128) * 64] in blocks of 128 elements, or with `layout` "rows" uint8
+    [m, ceil(k / 32) * 16] in the order of the elements (include/flowedge_b200.h, fe_w4_args, has both; products with
+    groups of 32 and 64 read blocks faster); scales [m, ceil(k / group)].  Its type tells the other calls which layout a
+    packed weight has.
     """
     shape, dtype, device = _first(weight, "weight")
     m, k = shape
     ld = _matrix(weight, "weight", shape, dtype, device)
-    packed_shape, scales_shape = _w4_shapes(m, k, group)
-    packed = weight.new_empty(packed_shape, dtype=torch.uint8)
+    if layout not in ("blocks", "rows"):
+        _refuse(f"layout is 'blocks' or 'rows', not {layout!r}")
+    packed_dtype = torch.uint8 if layout == "rows" else torch.int8
+    packed_shape, scales_shape = _w4_shapes(m, k, group, packed_dtype)
+    packed = weight.new_empty(packed_shape, dtype=packed_dtype)
     scales = weight.new_empty(scales_shape, dtype=torch.float16)
-    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, 0, m, k, ld, 0, weight.data_ptr(), packed.data_ptr(),
-                    scales.data_ptr(), 0)
+    args = _W4.pack(_W4_SIZE, device, _DTYPES[dtype], group, 0, m, k, ld, 0, weight.data_ptr(), packed.data_ptr(),
+                    scales.data_ptr(), 0) + _W4_LAYOUT[packed_dtype]
     rc = load_library().fe_w4_quantize_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
@@ -241,17 +253,17 @@ def w4_quantize(weight, group: int = 64) -> tuple:
 
 def _w4_weight(packed, scales, k: int, group: int, device: int) -> int:
     """Checks a packed weight of k columns and returns its rows."""
-    if not isinstance(packed, torch.Tensor) or packed.dim() != 2:
-        _refuse("packed is a tensor of shape (m, ceil(k / 128) * 64)")
+    if not isinstance(packed, torch.Tensor) or packed.dim() != 2 or packed.dtype not in _W4_LAYOUT:
+        _refuse("packed is an int8 tensor of shape (m, ceil(k / 128) * 64) or a uint8 one of shape (m, ceil(k / 32) * 16)")
     m = packed.shape[0]
-    packed_shape, scales_shape = _w4_shapes(m, k, group)
-    _flat(packed, "packed", packed_shape, torch.uint8, device)
+    packed_shape, scales_shape = _w4_shapes(m, k, group, packed.dtype)
+    _flat(packed, "packed", packed_shape, packed.dtype, device)
     _flat(scales, "scales", scales_shape, torch.float16, device)
     return m
 
 
 def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float32):
-    """The matrix [m, k] that a packed weight stands for, rounded to `dtype`."""
+    """The matrix [m, k] that a packed weight of either layout stands for, rounded to `dtype`."""
     if dtype not in _DTYPES:
         _refuse("dtype is float32, bfloat16 or float16")
     if not isinstance(packed, torch.Tensor) or not packed.is_cuda:
@@ -259,8 +271,8 @@ def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float3
     device = packed.get_device()
     m = _w4_weight(packed, scales, k, group, device)
     weight = packed.new_empty((m, k), dtype=dtype)
-    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, 0, m, k, 0, k, 0, packed.data_ptr(), scales.data_ptr(),
-                    weight.data_ptr())
+    args = _W4.pack(_W4_SIZE, device, _DTYPES[dtype], group, 0, m, k, 0, k, 0, packed.data_ptr(), scales.data_ptr(),
+                    weight.data_ptr()) + _W4_LAYOUT[packed.dtype]
     rc = load_library().fe_w4_dequantize_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
@@ -270,7 +282,8 @@ def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float3
 def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
     """x [rows, k] times the transpose of a packed weight [m, k], for a few rows (32 read the weight once).
 
-    float32, bfloat16 or float16 x and result; sums in float32, the weight exact.
+    float32, bfloat16 or float16 x and result; sums in float32, the weight exact.  packed is uint8 with its words in the
+    order of their elements, or int8 in blocks (w4_quantize).
     """
     shape, dtype, device = _first(x, "x")
     rows, k = shape
@@ -280,8 +293,8 @@ def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
         out, y_ld = x.new_empty((rows, m)), m
     else:
         y_ld = _matrix(out, "out", (rows, m), dtype, device)
-    args = _W4.pack(_W4.size, device, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(), packed.data_ptr(),
-                    scales.data_ptr(), out.data_ptr())
+    args = _W4.pack(_W4_SIZE, device, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(), packed.data_ptr(),
+                    scales.data_ptr(), out.data_ptr()) + _W4_LAYOUT[packed.dtype]
     rc = load_library().fe_w4_matvec_device(args, _raw_stream(device))
     if rc:
         _failed(rc)

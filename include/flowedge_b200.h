@@ -518,11 +518,16 @@ size_t fe_selective_scan_workspace(const fe_scan_args* args);
 
 /* Weights of 4 bits with group scales: w[m][k] = (q[m][k] - 8) scales[m][k / group],
  * q from 0 to 15, scales fp16 [m][ceil(k / group)], group 32, 64 or 128.
- * `packed` [m][ceil(k / 128)][64 bytes], 16-byte aligned: the 32-bit word at
- * place 4 t + j (t, j from 0 to 3) of a block of 128 elements holds the eight
- * elements from 32 j + 8 t on; its nibbles 0 .. 7, lowest first, are the
- * elements 0, 2, 4, 6, 1, 3, 5, 7 of the eight (so that one mask takes out two
- * neighbours).  Elements behind the last are 8, that is zero.
+ * `packed` is 16-byte aligned.  A 32-bit word holds eight neighbouring elements;
+ * its nibbles 0 .. 7, lowest first, are the elements 0, 2, 4, 6, 1, 3, 5, 7 of
+ * the eight (so that one mask takes out two neighbours).  Elements behind the
+ * last are 8, that is zero.  The words' order:
+ * FE_W4_ROWS: [m][ceil(k / 32)][16 bytes], the words in the order of their
+ * elements.
+ * FE_W4_BLOCKS: [m][ceil(k / 128)][64 bytes]; the word at place 4 t + j (t, j
+ * from 0 to 3) of a block of 128 elements holds those from 32 j + 8 t on, so
+ * that a thread's words of four groups come in one load.
+ * A structure that ends before `layout` (struct_size 88) reads as FE_W4_BLOCKS.
  *
  * fe_w4_matvec_device: y[r][m] = sum_k x[r][k] w[m][k] for a few rows; x and y
  * are `dtype`, sums fp32 (an fp32 x enters the products unrounded).  Up to 32
@@ -533,6 +538,8 @@ size_t fe_selective_scan_workspace(const fe_scan_args* args);
  * rounded to fp16 (at most 65504), q = round(w / scale) + 8 within 0 .. 15,
  * ties to even (rows is not read).
  * fe_w4_dequantize_device: the weights as `dtype` into y ([m][y_ld]). */
+enum { FE_W4_BLOCKS = 0, FE_W4_ROWS = 1 };
+
 typedef struct fe_w4_args {
   uint32_t struct_size; /* sizeof(fe_w4_args) */
   int32_t device;
@@ -544,6 +551,8 @@ typedef struct fe_w4_args {
   void* packed;
   void* scales;
   void* y;
+  uint32_t layout;   /* FE_W4_* of packed */
+  uint32_t reserved; /* 0 */
 } fe_w4_args;
 int fe_w4_matvec_device(const fe_w4_args* args, void* stream);
 int fe_w4_quantize_device(const fe_w4_args* args, void* stream);
