@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(128) conv_token_kernel(const ConvParams p) {
 }
 
 // One thread walks V channels of a tile's rows, two and two (V 1: a pair with
-// an idle half), with their last DC inputs in registers (right-aligned: taps
-// before the first of dc carry weight zero), kAhead rows requested before
-// their arithmetic.  The first tile of a sequence reads the old window and
+// an idle half), with their last DC (d_conv) inputs in registers, kAhead rows
+// requested before their arithmetic.  Each tap count is a kernel of its own: a
+// surplus tap of weight zero would make NaN of an infinite input.  The first tile of a sequence reads the old window and
 // writes the new one from the sequence's last rows, so no other tile touches
 // it.  Bound by x and u, read and written once (a tile reads DC - 1 rows
 // before its own again, from L2), and in front of that by the chain of a tile:
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p)
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool on = c < p.di && q.live;
   const T* x = static_cast<const T*>(p.x) + q.begin * p.x_ld + c;
-  float* win = p.window == nullptr ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * p.dc;
+  float* win = p.window == nullptr ? nullptr : p.window + q.slot * p.slot_stride + static_cast<long long>(c) * DC;
   const int t1 = on ? min(t0 + p.chunk, q.len) : t0;
   using Row = Vec<T, V>;
   auto pair = [](const Row& r, int e) {
@@ -251,20 +251,18 @@ __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p)
 #pragma unroll
     for (int e = 0; e < 2 * kPairs; ++e) {
       const int ce = e < V ? c + e : c;
-      const float* src = p.w + static_cast<long long>(ce) * p.dc;
+      const float* src = p.w + static_cast<long long>(ce) * DC;
       (e & 1 ? bias[e / 2].y : bias[e / 2].x) = p.b[ce];
-      if constexpr (V > 1 && DC == 4) {
-        if (p.dc == 4) {  // on 16 bytes (conv_prompts)
-          const float4 w4 = *reinterpret_cast<const float4*>(src);
-          w[0][e] = w4.x;
-          w[1][e] = w4.y;
-          w[2][e] = w4.z;
-          w[3][e] = w4.w;
-          continue;
-        }
-      }
+      if constexpr (V > 1 && DC == 4) {  // on 16 bytes (conv_prompts)
+        const float4 w4 = *reinterpret_cast<const float4*>(src);
+        w[0][e] = w4.x;
+        w[1][e] = w4.y;
+        w[2][e] = w4.z;
+        w[3][e] = w4.w;
+      } else {
 #pragma unroll
-      for (int j = 0; j < DC; ++j) w[j][e] = j >= DC - p.dc ? src[j - (DC - p.dc)] : 0.0f;
+        for (int j = 0; j < DC; ++j) w[j][e] = src[j];
+      }
     }
   }
   Row halo[DC];
@@ -275,24 +273,24 @@ __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p)
   if (!writes(p.q, s, q, blockIdx.y == 0) || !on) return;
 #pragma unroll
   for (int j = 0; j < DC; ++j) {
-    const int t = t0 - DC + j;  // the input that place j holds before row t0; place 0 is shifted out unused
+    // place j holds the input t0 - DC + j before row t0; place 0 is shifted out unused
 #pragma unroll
     for (int e = 0; e < kPairs; ++e) {
       wk[j][e] = make_float2(w[j][2 * e], w[j][2 * e + 1]);
       in[j][e] = j > 0 && t0 >= DC ? pair(halo[j], e) : splat(0.0f);
     }
     // (a tile's first row is a multiple of the chunk, so that t0 is 0 or at least DC)
-    if (j > 0 && t0 == 0 && win != nullptr && !q.fresh && p.dc + t >= 0) {
+    if (j > 0 && t0 == 0 && win != nullptr && !q.fresh) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) (e & 1 ? in[j][e / 2].y : in[j][e / 2].x) = win[e * p.dc + p.dc + t];
+      for (int e = 0; e < V; ++e) (e & 1 ? in[j][e / 2].y : in[j][e / 2].x) = win[e * DC + j];
     }
   }
   if (k == 0 && win != nullptr) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      for (int j = 0; j < p.dc; ++j) {
-        const int t = q.len - p.dc + j;
-        win[e * p.dc + j] = t >= 0 ? to_f32(x[t * p.x_ld + e]) : (q.fresh ? 0.0f : win[e * p.dc + p.dc + t]);
+      for (int j = 0; j < DC; ++j) {
+        const int t = q.len - DC + j;
+        win[e * DC + j] = t >= 0 ? to_f32(x[t * p.x_ld + e]) : (q.fresh ? 0.0f : win[e * DC + DC + t]);
       }
   }
   T* u = static_cast<T*>(p.u) + (q.begin + t0) * p.u_ld + c;
@@ -323,7 +321,7 @@ __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p)
 template <typename T, int DC>
 int conv_prompts(ConvParams p, cudaStream_t st) {
   // 16 bytes of a row to a thread where its rows allow it (at most four
-  // channels, and two of eight taps, which take the registers)
+  // channels, and two of more than four taps, which take the registers)
   constexpr int kVec = DC > 4 ? 2 : 4;
   const auto fits = [&](const void* q, long long ld) {
     return reinterpret_cast<std::uintptr_t>(q) % (kVec * sizeof(T)) == 0 && ld % kVec == 0;
@@ -349,7 +347,18 @@ int conv_prompts(ConvParams p, cudaStream_t st) {
 
 template <typename T>
 int conv_typed(const ConvParams& p, cudaStream_t st) {
-  if (p.q.offsets != nullptr) return p.dc <= 4 ? conv_prompts<T, 4>(p, st) : conv_prompts<T, 8>(p, st);
+  if (p.q.offsets != nullptr) {
+    switch (p.dc) {
+      case 1: return conv_prompts<T, 1>(p, st);
+      case 2: return conv_prompts<T, 2>(p, st);
+      case 3: return conv_prompts<T, 3>(p, st);
+      case 4: return conv_prompts<T, 4>(p, st);
+      case 5: return conv_prompts<T, 5>(p, st);
+      case 6: return conv_prompts<T, 6>(p, st);
+      case 7: return conv_prompts<T, 7>(p, st);
+      default: return conv_prompts<T, 8>(p, st);
+    }
+  }
   const dim3 grid(static_cast<unsigned>(p.q.n_seq), static_cast<unsigned>((p.di + 127) / 128));
   if (p.dc == 4 && reinterpret_cast<std::uintptr_t>(p.window) % 16 == 0 && p.slot_stride % 4 == 0)
     conv_token_kernel<T, true><<<grid, 128, 0, st>>>(p);
