@@ -446,8 +446,11 @@ cudaError_t allow_smem(K kernel, int bytes) {
 // in each of the scan's passes.  The products are those of fp32: every operand
 // is a sum of bf16 terms (dt_w of three; dt_in of one, two or three as it is
 // bf16, fp16 or fp32: 8, 11 or 24 bits), and all pairs of terms are multiplied
-// whose product is above 2^-25 of the whole, smallest first.  16384 x 2048, dt
-// rank 64, bf16: 73 us, 21 of them the bytes of dt.
+// whose product is above 2^-25 of the whole, smallest first.  Terms of an
+// infinity or of a value that bf16 rounds to one do not add up to it (infinity
+// times terms of two signs, or of zero, is NaN): a sum that is not finite is
+// made again from the operands.  16384 x 2048, dt rank 64, bf16: 73 us, 21 of
+// them the bytes of dt.
 template <typename T>
 constexpr int kDtTerms = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;
 
@@ -464,6 +467,19 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A row's steps from the operands themselves, for sums that the terms cannot
+// give: columns c, c + 1, c + 8, c + 9 .. below `end`, those of a fragment's lane.
+template <typename T>
+__device__ __noinline__ void step_row(const T* row, const float* dt_w, const float* dt_b, float* to, int dr, int di, int c,
+                                      int end) {
+  for (; c < end; c += c & 1 ? 7 : 1) {
+    float sum = dt_b[c];
+    const float* w = dt_w + c;
+    for (int r = 0; r < dr; ++r, w += di) sum = fmaf(to_f32(row[r]), *w, sum);
+    to[c] = softplus_rel(sum);
+  }
 }
 
 // A warp takes 16 rows x COLS channels at a time and walks the rows; dt_in goes from memory into fragments (the next 16 columns asked for before
@@ -550,6 +566,7 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
     }
     float* to = p.steps + (row0 + g) * p.di + c0 + 2 * t;
     const long long below = 8LL * p.di;
+    float2 finite[2] = {};  // of both rows, zero times every sum: NaN where one is not
 #pragma unroll
     for (int n = 0; n < COLS / 8; ++n, to += 8) {
       const int c = c0 + 8 * n + 2 * t;
@@ -559,7 +576,9 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
       for (int i = 0; i < 2; ++i) {
         // (the bias joins here: the instruction's sums drop bits below the
         // largest term's last, and the bias is the largest)
-        const float2 v = softplus_rel2(make_float2(acc[n][2 * i] + bias.x, acc[n][2 * i + 1] + bias.y));
+        const float2 sum = make_float2(acc[n][2 * i] + bias.x, acc[n][2 * i + 1] + bias.y);
+        finite[i] = __ffma2_rn(sum, splat(0.0f), finite[i]);
+        const float2 v = softplus_rel2(sum);
         float* at = to + i * below;
         if (pairs) {
           if (8 * i < have && c_hi) *reinterpret_cast<float2*>(at) = v;
@@ -568,6 +587,13 @@ __global__ void __launch_bounds__(kDtWarps * 32, kDtCtas) scan_steps_kernel(cons
           if (8 * i < have && c_hi) at[1] = v.y;
         }
       }
+    }
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      if ((i == 0 ? finite[0].x + finite[0].y : finite[1].x + finite[1].y) == 0.0f || 8 * i >= have) continue;
+      const long long row = row0 + g + 8 * i;
+      step_row(static_cast<const T*>(p.proj) + row * p.proj_ld, p.dt_w, p.dt_b, p.steps + row * p.di, p.dr, p.di, c0 + 2 * t,
+               min(p.di, c0 + COLS));
     }
   }
 }

@@ -53,3 +53,66 @@ def test_conv_uses_its_own_taps_alone(dtype, dc, di, form):
     ops.conv(args[0], w, b, window=args[3], offsets=args[4], out=out)
     _same(out, want, bound, "u")
     _same(args[3], win, torch.zeros_like(win), "window")
+
+
+def _scan_case(seed, rows, di, ds, dr, dtype, pool):
+    g = torch.Generator().manual_seed(seed)
+    return {"u": torch.randn(rows, di, generator=g).to(dtype).cuda(), "proj": torch.randn(rows, dr + 2 * ds, generator=g).to(dtype).cuda(),
+            "a": -(torch.rand(ds, di, generator=g) * ds + 0.5).cuda(), "d": torch.randn(di, generator=g).cuda(),
+            "dt_w": (torch.randn(dr, di, generator=g) * 0.5 * dr ** -0.5).cuda(),
+            "dt_b": (torch.rand(di, generator=g) * 4 - 5).cuda(), "z": torch.randn(rows, di, generator=g).to(dtype).cuda(),
+            "state": torch.randn(pool, ds, di, generator=g).cuda()}
+
+
+def _check_scan(case, offsets):
+    out = torch.full_like(case["u"], 7.0)
+    keys = ("u", "proj", "a", "d", "dt_w", "dt_b", "z", "state")
+    y, pool, bound, pool_bound = ref.scan(*(case[k] for k in keys), offsets, None, None, out)
+    ops.scan(*(case[k] for k in keys[:1] + keys[1:6]), z=case["z"], state=case["state"], offsets=offsets, out=out)
+    _same(out, y, bound, "y")
+    _same(case["state"], pool, pool_bound, "state")
+
+
+# sequences, channels: dt of tokens made in the scan, beforehand (from 16 sequences that fill the GPU), and of prompts
+FORMS = [("tokens", 6, 130), ("tokens", 40, 2050), ("prompts", 5, 130), ("prompts", 5, 131)]
+
+
+def _shape(form, n):
+    lengths = [1] * n if form == "tokens" else [3, 1, 12, 9, 16][:n]
+    return sum(lengths), None if form == "tokens" else _offsets(lengths)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form,n,di", FORMS)
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+def test_scan_with_an_infinite_step_input(dtype, form, n, di, value):
+    """dt = softplus(dt_in dt_w + dt_b) of a row with an infinite dt_in: infinite, or zero where the weight's sign makes
+    it minus infinity, and NaN where the weight is zero."""
+    rows, offsets = _shape(form, n)
+    case = _scan_case(1, rows, di, 16, 8, dtype, n)
+    case["dt_w"][3, ::7] = 0.0
+    case["proj"][2, 3] = value
+    case["proj"][5, 7] = value
+    _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("form,n,di", FORMS)
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+def test_scan_with_an_infinite_step_weight(form, n, di, value):
+    rows, offsets = _shape(form, n)
+    case = _scan_case(2, rows, di, 8, 20, torch.float32, n)
+    case["dt_w"][11, 5] = value
+    case["dt_w"][0, 64] = value
+    case["dt_b"][1] = value
+    case["proj"][1, 11] = 0.0
+    _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("form,n,di", FORMS)
+def test_scan_with_a_step_input_at_the_end_of_float32(form, n, di):
+    """A dt_in that bf16 rounds to infinity is finite all the same."""
+    rows, offsets = _shape(form, n)
+    case = _scan_case(3, rows, di, 16, 8, torch.float32, n)
+    case["dt_w"] *= 1e-30
+    case["proj"][2, 3], case["proj"][4, 0] = 3.4e38, -3.4e38
+    _check_scan(case, offsets)
