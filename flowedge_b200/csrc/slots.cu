@@ -626,12 +626,14 @@ int steps_launch(const ScanParams& p, cudaStream_t st) {
 // thread requests its states first, which are the kernel's bytes; the rest of
 // its work comes while they do.  Arithmetic on the two channels at once
 // (FFMA2).  GIVEN: dt is in the workspace (many sequences: dt_w would be read
-// again for every one of them), else the CTA makes it.  Bound by the states'
+// again for every one of them), else the CTA makes it.  PADDED: fewer states
+// than DS; those that do not exist stay out of y (an infinite u or dt makes NaN
+// of them).  Bound by the states'
 // bytes and their latency: 475 of 512 x 2048, 16 states, bf16: 38 us with the
 // dt before it, 0.53 of the measured copy rate.
 constexpr int kTokenStates = 8;  // of a thread
 
-template <typename T, int DS, int V, bool GIVEN>
+template <typename T, int DS, int V, bool GIVEN, bool PADDED>
 __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
   constexpr int kSplit = DS / kTokenStates, kPairs = 32 / kSplit;  // threads of a channel pair, pairs of a warp
   extern __shared__ float sdt[];                  // dt_in [dr], not GIVEN
@@ -717,7 +719,7 @@ __global__ void __launch_bounds__(128) scan_token_kernel(const ScanParams p) {
     for (int i = 0; i < 4; ++i) {
       const float2 e = __fmul2_rn(dt, an[n + i]);
       h[n + i] = __ffma2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), h[n + i], __fmul2_rn(dtu, splat(bn[i])));
-      y = __ffma2_rn(h[n + i], splat(cn[i]), y);
+      if (!PADDED || n0 + n + i < ds) y = __ffma2_rn(h[n + i], splat(cn[i]), y);
     }
   }
   y = across(y);
@@ -771,8 +773,10 @@ constexpr int kPolyPairs = DS / 16;
 // rows ahead.  All arithmetic on pairs (FFMA2): states two and two.  16384 rows
 // x 2048, 16 states, bf16: the main pass adds 188 us to the call, the summaries
 // 143.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469
-// (with two state pairs on the FMA pipe in the summaries).
-template <typename T, int DS, bool SUMMARY>
+// (with two state pairs on the FMA pipe in the summaries).  DS is d_state
+// rounded up to a multiple of four; PADDED: the last states do not exist and
+// stay out of y, as for single tokens.
+template <typename T, int DS, bool SUMMARY, bool PADDED>
 __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt_kernel(const ScanParams p) {
   __shared__ __align__(16) float sbc[2][kStage][2 * DS];
   if (!SUMMARY) report_offsets(p.q);
@@ -891,8 +895,14 @@ __global__ void __launch_bounds__(kScanWarps * 32, DS <= 16 ? 4 : 3) scan_prompt
       if (!SUMMARY) {
         const float4 cq = *reinterpret_cast<const float4*>(row + DS + 2 * n);
         const float2 c0 = make_float2(cq.x, cq.y), c1 = make_float2(cq.z, cq.w);
-        y0 = n == 0 ? __fmul2_rn(h[n], c0) : __ffma2_rn(h[n], c0, y0);
-        y1 = n == 0 ? __fmul2_rn(h[n + 1], c1) : __ffma2_rn(h[n + 1], c1, y1);
+        float2 h0 = h[n], h1 = h[n + 1];
+        if (PADDED && n == DS / 2 - 2) {
+          h0.y = DS - 3 < ds ? h0.y : 0.0f;
+          h1.x = DS - 2 < ds ? h1.x : 0.0f;
+          h1.y = 0.0f;
+        }
+        y0 = n == 0 ? __fmul2_rn(h0, c0) : __ffma2_rn(h0, c0, y0);
+        y1 = n == 0 ? __fmul2_rn(h1, c1) : __ffma2_rn(h1, c1, y1);
       }
     }
     if (SUMMARY) return 0.0f;
@@ -1015,7 +1025,7 @@ int scan_chunk(long long rows, int di) {
 // as fill the GPU.  Fewer take dt_w from L2 faster than another kernel starts.
 bool tokens_given(long long n_seq, long long di) { return n_seq * di >= 512LL * current_sm_count() && n_seq >= 16; }
 
-template <typename T, int DS>
+template <typename T, int DS, bool PADDED>
 int scan_tokens(const ScanParams& p, cudaStream_t st) {
   const auto even = [](const void* q, long long ld, std::size_t e) {
     return reinterpret_cast<std::uintptr_t>(q) % (2 * e) == 0 && ld % 2 == 0;
@@ -1029,43 +1039,53 @@ int scan_tokens(const ScanParams& p, cudaStream_t st) {
   const dim3 block(128);
   if (tokens_given(p.q.n_seq, p.di)) {
     if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
-    pairs ? launch_pdl(scan_token_kernel<T, DS, 2, true>, grid, block, 0, st, p)
-          : launch_pdl(scan_token_kernel<T, DS, 1, true>, grid, block, 0, st, p);
+    pairs ? launch_pdl(scan_token_kernel<T, DS, 2, true, PADDED>, grid, block, 0, st, p)
+          : launch_pdl(scan_token_kernel<T, DS, 1, true, PADDED>, grid, block, 0, st, p);
   } else {
     const std::size_t smem = static_cast<std::size_t>(p.dr) * sizeof(float);
-    pairs ? scan_token_kernel<T, DS, 2, false><<<grid, block, smem, st>>>(p)
-          : scan_token_kernel<T, DS, 1, false><<<grid, block, smem, st>>>(p);
+    pairs ? scan_token_kernel<T, DS, 2, false, PADDED><<<grid, block, smem, st>>>(p)
+          : scan_token_kernel<T, DS, 1, false, PADDED><<<grid, block, smem, st>>>(p);
   }
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, int DS>
-int scan_typed(const ScanParams& p, cudaStream_t st) {
+template <typename T, int DS, bool PADDED>
+int scan_prompts(const ScanParams& p, cudaStream_t st) {
   const unsigned cb = static_cast<unsigned>((p.di + 127) / 128);
-  if (p.q.offsets == nullptr) {
-    return scan_tokens<T, DS>(p, st);
-  }
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), cb);
   if (const int rc = steps_launch<T>(p, st); rc != 0) return rc;
   if (p.q.rows > p.chunk) {
-    launch_pdl(scan_prompt_kernel<T, DS, true>, grid, dim3(kScanWarps * 32), 0, st, p);
+    launch_pdl(scan_prompt_kernel<T, DS, true, false>, grid, dim3(kScanWarps * 32), 0, st, p);
     launch_pdl(scan_carry_kernel,
                dim3(static_cast<unsigned>(p.q.n_seq), static_cast<unsigned>((p.di + kCarryThreads - 1) / kCarryThreads),
                     static_cast<unsigned>((p.ds + kCarryStates - 1) / kCarryStates)),
                dim3(kCarryThreads), 0, st, p);
   }
   if (p.q.rows > 0)
-    launch_pdl(scan_prompt_kernel<T, DS, false>, grid, dim3(kScanWarps * 32), 0, st, p);
+    launch_pdl(scan_prompt_kernel<T, DS, false, PADDED>, grid, dim3(kScanWarps * 32), 0, st, p);
   else  // behind no kernel of this call: the caller's writes have to be seen
-    scan_prompt_kernel<T, DS, false><<<grid, kScanWarps * 32, 0, st>>>(p);
+    scan_prompt_kernel<T, DS, false, PADDED><<<grid, kScanWarps * 32, 0, st>>>(p);
   return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int DS = 4>
+int scan_prompts_sized(const ScanParams& p, cudaStream_t st) {
+  if constexpr (DS < 32)
+    if (p.ds > DS) return scan_prompts_sized<T, DS + 4>(p, st);
+  return p.ds < DS ? scan_prompts<T, DS, true>(p, st) : scan_prompts<T, DS, false>(p, st);
+}
+
+template <typename T, int DS>
+int scan_tokens_sized(const ScanParams& p, cudaStream_t st) {
+  return p.ds < DS ? scan_tokens<T, DS, true>(p, st) : scan_tokens<T, DS, false>(p, st);
 }
 
 template <typename T>
 int scan_sized(const ScanParams& p, cudaStream_t st) {
-  if (p.ds <= 8) return scan_typed<T, 8>(p, st);
-  if (p.ds <= 16) return scan_typed<T, 16>(p, st);
-  return scan_typed<T, 32>(p, st);
+  if (p.q.offsets != nullptr) return scan_prompts_sized<T>(p, st);
+  if (p.ds <= 8) return scan_tokens_sized<T, 8>(p, st);
+  if (p.ds <= 16) return scan_tokens_sized<T, 16>(p, st);
+  return scan_tokens_sized<T, 32>(p, st);
 }
 
 SeqParams sequences(const std::int32_t* offsets, const std::int32_t* slots, const std::uint8_t* fresh,

@@ -116,3 +116,20 @@ def test_scan_with_a_step_input_at_the_end_of_float32(form, n, di):
     case["dt_w"] *= 1e-30
     case["proj"][2, 3], case["proj"][4, 0] = 3.4e38, -3.4e38
     _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form,n,di", FORMS)
+@pytest.mark.parametrize("ds", [1, 5, 8, 12, 15, 16, 20, 31, 32])
+@pytest.mark.parametrize("value", [INF, NAN])
+def test_scan_with_an_infinite_input_and_few_states(dtype, form, n, di, ds, value):
+    """States that the call does not have add nothing, whatever u and dt hold."""
+    rows, offsets = _shape(form, n)
+    case = _scan_case(4, rows, di, ds, 4, dtype, n)
+    case["proj"][:, 4:] = case["proj"][:, 4:].abs() + 0.25  # B and C of one sign: sums of infinities of one sign
+    case["d"] = case["d"].abs() + 0.1
+    case["state"] = case["state"].abs()
+    case["u"][1, ::3] = value
+    case["u"][5, 1] = value
+    case["dt_b"][4] = INF
+    _check_scan(case, offsets)
