@@ -408,14 +408,15 @@ __device__ __forceinline__ float softplus_rel(float x) { return softplus_rel2(sp
 
 // 2^x for a pair of x <= 0 on the FMA pipe.  x = k + r with k whole and r in
 // [-1/2, 1/2] (k by adding and taking away 1.5 * 2^23), 2^r = 1 + r q(r) with
-// q the degree-5 Chebyshev interpolant of (2^r - 1) / r, 2^k added to the
-// exponent field; below 2^-125 the result stays there.  The leading 1 is exact
-// and the error is that of the last addition (at most 7.2e-8, mean 3e-10), so
-// that a decay near 1 keeps its distance from 1 over thousands of steps.
+// q the degree-5 Chebyshev interpolant of (2^r - 1) / r, times 2^k, whose bits
+// are k + 127 in the exponent field (k = -127, which x below it takes too, is
+// 0).  A NaN stays one through the sum.  The leading 1 is exact and the error
+// is that of the last addition (at most 7.2e-8, mean 3e-10), so that a decay
+// near 1 keeps its distance from 1 over thousands of steps.
 __device__ __forceinline__ float2 exp2_neg2(float2 x) {
   constexpr float kRound = 12582912.0f;
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
+  x.x = max_nan(x.x, -127.0f);
+  x.y = max_nan(x.y, -127.0f);
   const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
   const float2 k = __fadd2_rn(t, make_float2(-kRound, -kRound));
   const float2 r = __ffma2_rn(k, make_float2(-1.0f, -1.0f), x);
@@ -425,8 +426,8 @@ __device__ __forceinline__ float2 exp2_neg2(float2 x) {
   p = __ffma2_rn(p, r, make_float2(2.4022651e-1f, 2.4022651e-1f));
   p = __ffma2_rn(p, r, make_float2(6.9314718e-1f, 6.9314718e-1f));
   p = __ffma2_rn(p, r, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  return __fmul2_rn(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000)));
 }
 
 // Lets a kernel have `bytes` of shared memory, at most 200 KB (always the same
@@ -752,11 +753,11 @@ constexpr int kTok = 4;        // rows whose dt, u and z are requested ahead
 // State pairs whose exponentials go to the FMA pipe, the first ones (where a
 // grows with n, as it does at the start of training, the slowest states, which
 // gain from its exactness near 1).  A row's exponentials take the MUFU unit 8
-// cycles each, the FMA pipe 18 a pair beside 6 (summary) or 8 for the pair's
+// cycles each, the FMA pipe 20 a pair beside 6 (summary) or 8 for the pair's
 // products, so few pairs gain.  Measured at 16384 rows x 2048 channels and at 96
-// prompts of 12289 x 1024, DS 16, pairs of eight in the summary and in the main
-// pass: 0, 0 420 and 183 us; 1, 0 418 and 181; 1, 1 416 and 183; 2, 1 421 and
-// 186; 2, 2 440 and 194.
+// prompts of 12289 x 1024, DS 16: no pair 421.6 and 183.8 us, one of eight
+// 417.7 and 184.9; at 64 prompts of 8192 x 1024, DS 32: none 216.8, one of
+// sixteen 218.9, two 213.4.
 template <int DS>
 constexpr int kPolyPairs = DS / 16;
 

@@ -133,3 +133,25 @@ def test_scan_with_an_infinite_input_and_few_states(dtype, form, n, di, ds, valu
     case["u"][5, 1] = value
     case["dt_b"][4] = INF
     _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("form,n,di", FORMS)
+@pytest.mark.parametrize("ds", [4, 16, 24])
+def test_scan_with_a_missing_decay(form, n, di, ds):
+    """A NaN in a spoils its channel, in every form alike; the others keep their values."""
+    rows, offsets = _shape(form, n)
+    case = _scan_case(5, rows, di, ds, 4, torch.float32, n)
+    case["a"][0, 3] = NAN
+    case["a"][1, 9] = NAN
+    case["a"][ds - 1, 20] = NAN
+    _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("form,n,di", FORMS)
+def test_scan_decays_to_nothing(form, n, di):
+    """exp(dt a) far below float32's range takes the old state away, an infinite one too where it is zero in 64 bits."""
+    rows, offsets = _shape(form, n)
+    case = _scan_case(6, rows, di, 16, 4, torch.float32, n)
+    case["a"][:, 5] = -1e30
+    case["state"][:, :, 5] = 3e38
+    _check_scan(case, offsets)
