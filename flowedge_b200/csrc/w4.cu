@@ -144,8 +144,9 @@ __device__ __forceinline__ void stage_x(const W4Params& p, int r0, int n, int b0
         if constexpr (TERMS == 1) {
           *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(&v[i]);
         } else {
-          // the leading bits as bf16, then the rest's: 8 + 8 + 8 bits, nothing lost
-          float f[4] = {v[i].v[0], v[i].v[1], v[i].v[2], v[i].v[3]};
+          // the leading bits as bf16, then the rest's: 8 + 8 + 8 bits, nothing lost (a sum has a NaN's
+          // payload in its leading bits, which alone would read as an infinity where they are zero)
+          float f[4] = {v[i].v[0] + 0.0f, v[i].v[1] + 0.0f, v[i].v[2] + 0.0f, v[i].v[3] + 0.0f};
 #pragma unroll
           for (int t = 0; t < TERMS; ++t) {
             float h[4];
