@@ -31,6 +31,8 @@
 #include <cstring>
 #include <exception>
 #include <map>
+#include <memory>
+#include <new>
 #include <tuple>
 
 #include "ops.h"
@@ -1043,7 +1045,6 @@ class Mamba final : public MambaDevice {
     if (step_graph_ != nullptr) cudaGraphExecDestroy(step_graph_);
     for (auto& [k, g] : fwd_graphs_) cudaGraphExecDestroy(g);
     drop_slot_graphs();
-    if (slot_pinned_ != nullptr) cudaFreeHost(slot_pinned_);
     if (pinned_ != nullptr) cudaFreeHost(pinned_);
   }
   bool load(const TensorTable& t, std::string& err);
@@ -1076,6 +1077,22 @@ class Mamba final : public MambaDevice {
                  std::string& err) noexcept override;
 
  private:
+  // buffers of the calls over slots
+  struct SlotBuffers {
+    DeviceArena arena;
+    std::size_t rows = 0, slots = 0;  // that they hold
+    int *ids = nullptr, *offsets = nullptr;
+    unsigned char* fresh = nullptr;
+    float* proj_out = nullptr;  // [rows][dm]
+    void* scan_ws = nullptr;
+    std::size_t scan_ws_bytes = 0;
+    char* pinned = nullptr;  // a call's description, then from pinned_rows on its result
+    std::size_t pinned_rows = 0;
+    ~SlotBuffers() {
+      if (pinned != nullptr) cudaFreeHost(pinned);
+    }
+  };
+
   // every layer over rows of tokens_ already embedded in hidden_; the final norm's rows to out_
   bool run_slots(long long rows, int n_seq, const int* offsets, const int* slots, const std::uint8_t* fresh,
                  std::int32_t* status, cudaStream_t st, std::string& err);
@@ -1089,9 +1106,14 @@ class Mamba final : public MambaDevice {
     slot_graphs_.clear();
   }
   int finish_slots(cudaStream_t st, std::string& err) noexcept;
+  // rows that a call over slots may have
+  [[nodiscard]] std::size_t slot_rows() const noexcept { return slot_ ? std::min(slot_->rows, cap_tokens_) : 0; }
+  std::unique_ptr<SlotBuffers> make_slot_buffers(std::size_t rows, std::size_t n_slots, std::string& err) noexcept;
+  bool grow_slot_buffers(std::size_t rows, std::size_t n_slots, std::string& err) noexcept;
+  bool place_workspace(std::size_t batch, std::size_t tokens, std::string& err) noexcept;
   // capacity for `rows` tokens, the batch capacity kept
   int make_room(std::size_t rows, std::string& err) noexcept {
-    if (rows <= cap_tokens_) return slot_rows_ >= rows ? 0 : reserve_slots(n_slots_, err);
+    if (rows <= cap_tokens_) return slot_rows() >= rows ? 0 : reserve_slots(n_slots_, err);
     const std::size_t batch = std::max<std::size_t>(cap_batch_, 1);
     return reserve(batch, (rows + batch - 1) / batch, err);
   }
@@ -1124,6 +1146,7 @@ class Mamba final : public MambaDevice {
   std::size_t part_elems_ = 0;
   float* pinned_ = nullptr;
   std::size_t pinned_floats_ = 0;
+  std::vector<float> kept_state_;  // the decode state while the workspace moves
   // the decode step as one graph (token upload, every layer, output download);
   // rebuilt after reserve() moves the buffers
   cudaGraphExec_t step_graph_ = nullptr;
@@ -1136,18 +1159,11 @@ class Mamba final : public MambaDevice {
   bool dec_fused_ = false;
   // slots: a pool of decode states, and buffers for a call's description
   int w4_group_ = 0;
-  DeviceArena pool_, slot_ws_;
+  DeviceArena pool_;
   float* pool_state_ = nullptr;  // [n_slots_][state_floats()]
   std::size_t n_slots_ = 0;
-  int *slot_ids_ = nullptr, *slot_offsets_ = nullptr;
-  unsigned char* slot_fresh_ = nullptr;
-  float* proj_out_ = nullptr;  // [cap_rows_][dm]
-  void* scan_ws_ = nullptr;
-  std::size_t scan_ws_bytes_ = 0;
-  std::size_t slot_rows_ = 0, slot_pool_ = 0;  // rows and slots that the buffers hold
-  char* slot_pinned_ = nullptr;                // a call's description, then from slot_pinned_rows_ on its result
-  std::size_t slot_pinned_bytes_ = 0, slot_pinned_rows_ = 0;
-  // the step of n rows (its tokens and slots in tokens_ and slot_ids_, its
+  std::unique_ptr<SlotBuffers> slot_;
+  // the step of n rows (its tokens and slots in tokens_ and slot_->ids, its
   // rows in out_) as one graph per n
   std::map<std::size_t, cudaGraphExec_t> slot_graphs_;
 };
@@ -1388,6 +1404,42 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   }
   const std::size_t tokens = batch * max_len;
   if (tokens <= cap_tokens_ && batch <= cap_batch_) return 0;
+  // the pinned buffer beside the old one, before anything is given up
+  const std::size_t need = tokens * (cfg_.d_model + 1) + state_floats();
+  float* pinned = nullptr;
+  if (pinned_floats_ < need && counted_host_malloc(reinterpret_cast<void**>(&pinned), need * 4) != cudaSuccess) {
+    cudaGetLastError();
+    err = "pinned host allocation failed";
+    return 2;
+  }
+  // keep the decode state across a re-reserve
+  if (state_ != nullptr) {
+    kept_state_.resize(state_floats());
+    cudaMemcpy(kept_state_.data(), state_, kept_state_.size() * 4, cudaMemcpyDeviceToHost);
+  }
+  const std::size_t old_tokens = cap_tokens_, old_batch = cap_batch_;
+  if (!place_workspace(batch, tokens, err) ||
+      (n_slots_ > 0 && !grow_slot_buffers(tokens, n_slots_, err))) {
+    // back to the buffers that there were
+    if (pinned != nullptr) cudaFreeHost(pinned);
+    std::string again;
+    if (old_tokens > 0 && place_workspace(old_batch, old_tokens, again) && n_slots_ > 0)
+      grow_slot_buffers(old_tokens, n_slots_, again);
+    return 2;
+  }
+  if (pinned != nullptr) {
+    cudaDeviceSynchronize();
+    if (pinned_ != nullptr) cudaFreeHost(pinned_);
+    pinned_ = pinned;
+    pinned_floats_ = need;
+  }
+  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
+}
+
+// The workspace for `tokens` in place of the one that there is, with the decode
+// state in it; where the device does not hold it there is none (capacity 0), and
+// the state waits for the next one.
+bool Mamba::place_workspace(std::size_t batch, std::size_t tokens, std::string& err) noexcept {
   if (step_graph_ != nullptr) {
     cudaGraphExecDestroy(step_graph_);
     step_graph_ = nullptr;
@@ -1395,6 +1447,8 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   for (auto& [k, g] : fwd_graphs_) cudaGraphExecDestroy(g);
   fwd_graphs_.clear();
   drop_slot_graphs();
+  cap_tokens_ = cap_batch_ = 0;
+  state_ = nullptr;
   const std::size_t dm = cfg_.d_model, di = cfg_.d_inner, wd = cfg_.dt_rank + 2 * cfg_.d_state;
   const std::size_t rows = (tokens + 255) / 256 * 256;
   std::size_t nsl = 1;
@@ -1421,24 +1475,8 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   plan.add_n<float>(dm + 2 * di + di + wd + di + di + dm + 64);
   plan.add_n<DecodeLayer>(layers_.size());
   plan.add_n<unsigned>(4);
-  // keep the decode state across a re-reserve
-  std::vector<float> saved;
-  if (state_ != nullptr) {
-    saved.resize(state_floats());
-    cudaMemcpy(saved.data(), state_, saved.size() * 4, cudaMemcpyDeviceToHost);
-  }
   ws_.release();
-  slot_rows_ = 0;  // the slots' calls use these buffers too
-  if (!ws_.init(plan.total(), err)) {
-    // back to the buffers that there were, and the decode state
-    const std::size_t old_tokens = cap_tokens_, old_batch = cap_batch_;
-    state_ = nullptr;
-    cap_tokens_ = cap_batch_ = 0;
-    std::string again;
-    if (old_tokens > 0 && reserve(old_batch, old_tokens / old_batch, again) == 0)
-      cudaMemcpy(state_, saved.data(), saved.size() * 4, cudaMemcpyHostToDevice);
-    return 2;
-  }
+  if (!ws_.init(plan.total(), err)) return false;
   tokens_ = ws_.take_n<int>(rows);
   hidden_ = ws_.take_n<float>(rows * dm);
   xz_ = ws_.take_n<float>(rows * 2 * di);
@@ -1457,8 +1495,7 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
   dec_sync_ = ws_.take_n<unsigned>(4);
   if (ws_.overflowed()) {
     err = "internal error: Mamba workspace arena too small";
-    cap_tokens_ = 0;
-    return 2;
+    return false;
   }
   cudaMemset(tokens_, 0, ws_.used());
   {
@@ -1480,24 +1517,15 @@ int Mamba::reserve(std::size_t batch, std::size_t max_len, std::string& err) noe
     dec_fused_ = oc == cudaSuccess && per_sm >= 1;
     cudaGetLastError();
   }
-  if (!saved.empty()) cudaMemcpy(state_, saved.data(), saved.size() * 4, cudaMemcpyHostToDevice);
-  const std::size_t need = tokens * (dm + 1) + state_floats();
-  if (pinned_floats_ < need) {
-    if (pinned_ != nullptr) cudaFreeHost(pinned_);
-    pinned_ = nullptr;
-    pinned_floats_ = 0;
-    if (counted_host_malloc(reinterpret_cast<void**>(&pinned_), need * 4) != cudaSuccess) {
-      cap_tokens_ = 0;
-      err = "pinned host allocation failed";
-      return 2;
-    }
-    pinned_floats_ = need;
+  if (!kept_state_.empty()) cudaMemcpy(state_, kept_state_.data(), kept_state_.size() * 4, cudaMemcpyHostToDevice);
+  if (cudaDeviceSynchronize() != cudaSuccess) {
+    err = cudaGetErrorString(cudaGetLastError());
+    return false;
   }
   cap_tokens_ = tokens;
   cap_batch_ = batch;
   cap_rows_ = rows;
-  if (n_slots_ > 0 && reserve_slots(n_slots_, err) != 0) return 2;
-  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 2;
+  return true;
 }
 
 bool Mamba::gemm(const Mat& m, const void* in, int in_ld, long long n_tok, float* out, int out_ld, bool accumulate,
@@ -1862,12 +1890,20 @@ int Mamba::step(std::int32_t token, float* out, std::string& err) noexcept {
 }
 
 void Mamba::reset() noexcept {
+  if (state_ == nullptr) {
+    std::fill(kept_state_.begin(), kept_state_.end(), 0.0f);
+    return;
+  }
   cudaSetDevice(ctx_->device);
   cudaMemsetAsync(state_, 0, state_floats() * 4, ctx_->stream);
   cudaStreamSynchronize(ctx_->stream);
 }
 
 int Mamba::read_state(float* dst, std::string& err) noexcept {
+  if (state_ == nullptr && !kept_state_.empty()) {
+    std::copy(kept_state_.begin(), kept_state_.end(), dst);
+    return 0;
+  }
   cudaSetDevice(ctx_->device);
   if (cudaMemcpyAsync(pinned_, state_, state_floats() * 4, cudaMemcpyDeviceToHost, ctx_->stream) != cudaSuccess ||
       cudaStreamSynchronize(ctx_->stream) != cudaSuccess) {
@@ -1879,6 +1915,10 @@ int Mamba::read_state(float* dst, std::string& err) noexcept {
 }
 
 int Mamba::write_state(const float* src, std::string& err) noexcept {
+  if (state_ == nullptr && !kept_state_.empty()) {
+    std::copy(src, src + kept_state_.size(), kept_state_.begin());
+    return 0;
+  }
   cudaSetDevice(ctx_->device);
   std::memcpy(pinned_, src, state_floats() * 4);
   if (cudaMemcpyAsync(state_, pinned_, state_floats() * 4, cudaMemcpyHostToDevice, ctx_->stream) != cudaSuccess ||
@@ -1891,8 +1931,71 @@ int Mamba::write_state(const float* src, std::string& err) noexcept {
 
 // --- many sequences over slots --------------------------------------------------
 
+// Buffers of the calls over slots, or none where they do not fit.
+std::unique_ptr<Mamba::SlotBuffers> Mamba::make_slot_buffers(std::size_t rows, std::size_t n_slots,
+                                                             std::string& err) noexcept {
+  std::unique_ptr<SlotBuffers> b(new (std::nothrow) SlotBuffers);
+  if (!b) {
+    err = "out of host memory";
+    return nullptr;
+  }
+  const std::size_t dm = cfg_.d_model, padded = (rows + 255) / 256 * 256;
+  b->rows = rows;
+  b->slots = n_slots;
+  b->scan_ws_bytes = selective_scan_workspace_most(rows, n_slots, cfg_.d_inner, cfg_.d_state);
+  ArenaPlan plan;
+  plan.add_n<int>(rows);
+  plan.add_n<int>(rows + 1);
+  plan.add(rows);
+  plan.add_n<float>(padded * dm);
+  plan.add(b->scan_ws_bytes);
+  if (!b->arena.init(plan.total(), err)) return nullptr;
+  b->ids = b->arena.take_n<int>(rows);
+  b->offsets = b->arena.take_n<int>(rows + 1);
+  b->fresh = static_cast<unsigned char*>(b->arena.take(rows));
+  b->proj_out = b->arena.take_n<float>(padded * dm);
+  b->scan_ws = b->arena.take(b->scan_ws_bytes);
+  if (b->arena.overflowed()) {
+    err = "internal error: slot workspace arena too small";
+    return nullptr;
+  }
+  b->pinned_rows = (rows * 13 + 19) / 16 * 16;
+  if (counted_host_malloc(reinterpret_cast<void**>(&b->pinned), b->pinned_rows + std::min(n_slots, rows) * dm * 4) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    b->pinned = nullptr;
+    err = "pinned host allocation failed";
+    return nullptr;
+  }
+  return b;
+}
+
+// At least `rows` rows and `n_slots` slots: beside the old buffers, or where
+// there is no room for both without them; they come back if that fails too.
+bool Mamba::grow_slot_buffers(std::size_t rows, std::size_t n_slots, std::string& err) noexcept {
+  if (slot_ && rows <= slot_->rows && n_slots <= slot_->slots) return true;
+  std::unique_ptr<SlotBuffers> next = make_slot_buffers(rows, n_slots, err);
+  if (!next && !slot_) return false;
+  cudaDeviceSynchronize();
+  drop_slot_graphs();
+  if (!next) {
+    const std::size_t old_rows = slot_->rows, old_slots = slot_->slots;
+    slot_.reset();
+    next = make_slot_buffers(rows, n_slots, err);
+    if (!next) {
+      std::string again;
+      slot_ = make_slot_buffers(old_rows, old_slots, again);
+      return false;
+    }
+    err.clear();
+  }
+  slot_ = std::move(next);
+  return true;
+}
+
 // The pool grows and keeps its states; the buffers of a call are sized for
-// the rows that reserve() made room for.
+// the rows that reserve() made room for.  The pool is taken over last, so that
+// a failure leaves it as it was.
 int Mamba::reserve_slots(std::size_t n_slots, std::string& err) noexcept {
   cudaSetDevice(ctx_->device);
   const std::size_t dm = cfg_.d_model;
@@ -1900,13 +2003,18 @@ int Mamba::reserve_slots(std::size_t n_slots, std::string& err) noexcept {
     err = "slots need d_model <= 16384";
     return 2;
   }
+  if (cap_tokens_ == 0) {
+    err = "no workspace (an earlier reservation failed)";
+    return 2;
+  }
+  DeviceArena grown;
+  float* p = nullptr;
   if (n_slots > n_slots_) {
-    DeviceArena grown;
     const std::size_t bytes = n_slots * state_floats() * 4, kept = n_slots_ * state_floats() * 4;
     ArenaPlan room;
     room.add(bytes);
     if (!grown.init(room.total(), err)) return 2;
-    auto* p = static_cast<float*>(grown.take(bytes));
+    p = static_cast<float*>(grown.take(bytes));
     if (p == nullptr || cudaMemset(p, 0, bytes) != cudaSuccess ||
         // (a call on a stream of the caller's may still write the old pool)
         (kept > 0 && (cudaDeviceSynchronize() != cudaSuccess ||
@@ -1915,47 +2023,13 @@ int Mamba::reserve_slots(std::size_t n_slots, std::string& err) noexcept {
       err = "slot state set-up failed";
       return 2;
     }
+  }
+  if (!grow_slot_buffers(cap_tokens_, std::max(n_slots, n_slots_), err)) return 2;
+  if (p != nullptr) {
     drop_slot_graphs();
     pool_.swap(grown);
     pool_state_ = p;
     n_slots_ = n_slots;
-  }
-  if (slot_rows_ < cap_tokens_ || slot_pool_ < n_slots_) {
-    cudaDeviceSynchronize();
-    drop_slot_graphs();
-    slot_rows_ = slot_pool_ = 0;
-    scan_ws_bytes_ = selective_scan_workspace_most(cap_tokens_, n_slots_, cfg_.d_inner, cfg_.d_state);
-    ArenaPlan plan;
-    plan.add_n<int>(cap_tokens_);
-    plan.add_n<int>(cap_tokens_ + 1);
-    plan.add(cap_tokens_);
-    plan.add_n<float>(cap_rows_ * dm);
-    plan.add(scan_ws_bytes_);
-    slot_ws_.release();
-    if (!slot_ws_.init(plan.total(), err)) return 2;
-    slot_ids_ = slot_ws_.take_n<int>(cap_tokens_);
-    slot_offsets_ = slot_ws_.take_n<int>(cap_tokens_ + 1);
-    slot_fresh_ = static_cast<unsigned char*>(slot_ws_.take(cap_tokens_));
-    proj_out_ = slot_ws_.take_n<float>(cap_rows_ * dm);
-    scan_ws_ = slot_ws_.take(scan_ws_bytes_);
-    if (slot_ws_.overflowed()) {
-      err = "internal error: slot workspace arena too small";
-      return 2;
-    }
-    slot_pinned_rows_ = (cap_tokens_ * 13 + 19) / 16 * 16;
-    const std::size_t need = slot_pinned_rows_ + std::min(n_slots_, cap_tokens_) * dm * 4;
-    if (slot_pinned_bytes_ < need) {
-      if (slot_pinned_ != nullptr) cudaFreeHost(slot_pinned_);
-      slot_pinned_ = nullptr;
-      slot_pinned_bytes_ = 0;
-      if (counted_host_malloc(reinterpret_cast<void**>(&slot_pinned_), need) != cudaSuccess) {
-        err = "pinned host allocation failed";
-        return 2;
-      }
-      slot_pinned_bytes_ = need;
-    }
-    slot_rows_ = cap_tokens_;
-    slot_pool_ = n_slots_;
   }
   return 0;
 }
@@ -2053,9 +2127,9 @@ bool Mamba::run_slots(long long rows, int n_seq, const int* offsets, const int* 
   q.offsets = offsets;
   q.slots = slots;
   q.fresh = fresh;
-  q.workspace = scan_ws_;
-  q.workspace_bytes = scan_ws_bytes_;
-  if (selective_scan_workspace(q) > scan_ws_bytes_) {
+  q.workspace = slot_->scan_ws;
+  q.workspace_bytes = slot_->scan_ws_bytes;
+  if (selective_scan_workspace(q) > slot_->scan_ws_bytes) {
     err = "internal error: scan workspace too small";
     return false;
   }
@@ -2066,7 +2140,7 @@ bool Mamba::run_slots(long long rows, int n_seq, const int* offsets, const int* 
   r.rows = c.rows;
   r.dim = static_cast<std::uint64_t>(dm);
   r.x_ld = r.residual_ld = r.out_ld = dm;
-  r.x = proj_out_;
+  r.x = slot_->proj_out;
   r.residual = hidden_;
   r.out = normed;
   r.scale = 1.0f;
@@ -2086,7 +2160,7 @@ bool Mamba::run_slots(long long rows, int n_seq, const int* offsets, const int* 
     q.dt_b = Ly.dt_b;
     q.state = c.window + static_cast<std::size_t>(di) * dc;
     if (launch_selective_scan(q, st) != 0) return false;
-    if (!project(Ly.out_proj, y_, di, yb_, rows, proj_out_, dm, st, err)) return false;
+    if (!project(Ly.out_proj, y_, di, yb_, rows, slot_->proj_out, dm, st, err)) return false;
     r.weight = li + 1 < layers_.size() ? layers_[li + 1].norm : norm_f_;
     if (launch_residual_norm(r, st) != 0) return false;
   }
@@ -2104,8 +2178,8 @@ bool Mamba::embed_and_run(long long rows, int n_seq, const int* offsets, const i
 int Mamba::prompt_device(const std::int32_t* tokens, std::size_t rows, const std::int32_t* offsets,
                          const std::int32_t* slots, const std::uint8_t* fresh, std::size_t n_seq, float* last_hidden,
                          std::int32_t* status, void* stream, std::string& err) noexcept {
-  if (slot_rows_ == 0 || rows > slot_rows_ || n_seq > slot_pool_) {
-    err = slot_rows_ == 0 ? "no slots are reserved" : "rows or sequences exceed the reserved capacity";
+  if (n_slots_ == 0 || rows > slot_rows() || n_seq > n_slots_) {
+    err = n_slots_ == 0 ? "no slots are reserved" : "rows or sequences exceed the reserved capacity";
     return 2;
   }
   cudaSetDevice(ctx_->device);
@@ -2129,22 +2203,22 @@ int Mamba::prompt_device(const std::int32_t* tokens, std::size_t rows, const std
 // launches themselves.
 int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, std::size_t n, float* out,
                        std::int32_t* status, void* stream, std::string& err) noexcept {
-  if (slot_rows_ == 0 || n > slot_rows_) {
-    err = slot_rows_ == 0 ? "no slots are reserved" : "rows exceed the reserved capacity";
+  if (n_slots_ == 0 || n > slot_rows()) {
+    err = n_slots_ == 0 ? "no slots are reserved" : "rows exceed the reserved capacity";
     return 2;
   }
   cudaSetDevice(ctx_->device);
   cudaStream_t st = stream != nullptr ? static_cast<cudaStream_t>(stream) : ctx_->stream;
   const int rows = static_cast<int>(n);
   if ((tokens != tokens_ && cudaMemcpyAsync(tokens_, tokens, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess) ||
-      (slots != slot_ids_ && cudaMemcpyAsync(slot_ids_, slots, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess)) {
+      (slots != slot_->ids && cudaMemcpyAsync(slot_->ids, slots, n * 4, cudaMemcpyDeviceToDevice, st) != cudaSuccess)) {
     err = "token copy failed";
     return 2;
   }
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   cudaStreamIsCapturing(st, &capturing);
   if (capturing != cudaStreamCaptureStatusNone || status != nullptr) {
-    if (!embed_and_run(rows, rows, nullptr, slot_ids_, nullptr, status, st, err)) {
+    if (!embed_and_run(rows, rows, nullptr, slot_->ids, nullptr, status, st, err)) {
       if (err.empty()) err = std::string("step launch failed: ") + cudaGetErrorString(cudaGetLastError());
       return 2;
     }
@@ -2157,7 +2231,7 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
       bool ok = cudaStreamCreateWithFlags(&cap, cudaStreamNonBlocking) == cudaSuccess &&
                 cudaStreamBeginCapture(cap, cudaStreamCaptureModeThreadLocal) == cudaSuccess;
       if (ok) {
-        const bool ran = embed_and_run(rows, rows, nullptr, slot_ids_, nullptr, nullptr, cap, err);
+        const bool ran = embed_and_run(rows, rows, nullptr, slot_->ids, nullptr, nullptr, cap, err);
         ok = cudaStreamEndCapture(cap, &graph) == cudaSuccess && ran && graph != nullptr &&
              cudaGraphInstantiate(&exec, graph, 0) == cudaSuccess;
       }
@@ -2184,7 +2258,7 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
       return 2;
     }
   }
-  gather_slots_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(out_, nullptr, slot_ids_, static_cast<int>(n_slots_),
+  gather_slots_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(out_, nullptr, slot_->ids, static_cast<int>(n_slots_),
                                                                rows, static_cast<int>(cfg_.d_model), out);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
@@ -2211,7 +2285,7 @@ int Mamba::prompt(const std::int32_t* tokens, const std::size_t* lengths, const 
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
   const std::size_t dm = cfg_.d_model;
-  auto* ptok = reinterpret_cast<std::int32_t*>(slot_pinned_);
+  auto* ptok = reinterpret_cast<std::int32_t*>(slot_->pinned);
   auto* pslot = ptok + rows;
   auto* poff = pslot + n_seq;
   auto* pfresh = reinterpret_cast<unsigned char*>(poff + n_seq + 1);
@@ -2221,12 +2295,12 @@ int Mamba::prompt(const std::int32_t* tokens, const std::size_t* lengths, const 
   for (std::size_t s = 0; s < n_seq; ++s) poff[s + 1] = poff[s] + static_cast<std::int32_t>(lengths[s]);
   std::memset(pfresh, resume ? 0 : 1, n_seq);
   cudaMemcpyAsync(tokens_, ptok, rows * 4, cudaMemcpyHostToDevice, st);
-  cudaMemcpyAsync(slot_ids_, pslot, n_seq * 4, cudaMemcpyHostToDevice, st);
-  cudaMemcpyAsync(slot_offsets_, poff, (n_seq + 1) * 4, cudaMemcpyHostToDevice, st);
-  cudaMemcpyAsync(slot_fresh_, pfresh, n_seq, cudaMemcpyHostToDevice, st);
-  if (prompt_device(tokens_, rows, slot_offsets_, slot_ids_, slot_fresh_, n_seq, proj_out_, nullptr, st, err) != 0) return 2;
-  auto* prows = reinterpret_cast<float*>(slot_pinned_ + slot_pinned_rows_);
-  cudaMemcpyAsync(prows, proj_out_, n_seq * dm * 4, cudaMemcpyDeviceToHost, st);
+  cudaMemcpyAsync(slot_->ids, pslot, n_seq * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_->offsets, poff, (n_seq + 1) * 4, cudaMemcpyHostToDevice, st);
+  cudaMemcpyAsync(slot_->fresh, pfresh, n_seq, cudaMemcpyHostToDevice, st);
+  if (prompt_device(tokens_, rows, slot_->offsets, slot_->ids, slot_->fresh, n_seq, slot_->proj_out, nullptr, st, err) != 0) return 2;
+  auto* prows = reinterpret_cast<float*>(slot_->pinned + slot_->pinned_rows);
+  cudaMemcpyAsync(prows, slot_->proj_out, n_seq * dm * 4, cudaMemcpyDeviceToHost, st);
   if (finish_slots(st, err) != 0) return 2;
   std::memcpy(last_hidden, prows, n_seq * dm * 4);
   return 0;
@@ -2238,14 +2312,14 @@ int Mamba::step_slots(const std::int32_t* tokens, const std::int32_t* slots, std
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
   const std::size_t dm = cfg_.d_model;
-  auto* ptok = reinterpret_cast<std::int32_t*>(slot_pinned_);
+  auto* ptok = reinterpret_cast<std::int32_t*>(slot_->pinned);
   std::memcpy(ptok, tokens, n * 4);
   std::memcpy(ptok + n, slots, n * 4);
   cudaMemcpyAsync(tokens_, ptok, n * 4, cudaMemcpyHostToDevice, st);
-  cudaMemcpyAsync(slot_ids_, ptok + n, n * 4, cudaMemcpyHostToDevice, st);
-  if (step_device(tokens_, slot_ids_, n, proj_out_, nullptr, st, err) != 0) return 2;
-  auto* prows = reinterpret_cast<float*>(slot_pinned_ + slot_pinned_rows_);
-  cudaMemcpyAsync(prows, proj_out_, n * dm * 4, cudaMemcpyDeviceToHost, st);
+  cudaMemcpyAsync(slot_->ids, ptok + n, n * 4, cudaMemcpyHostToDevice, st);
+  if (step_device(tokens_, slot_->ids, n, slot_->proj_out, nullptr, st, err) != 0) return 2;
+  auto* prows = reinterpret_cast<float*>(slot_->pinned + slot_->pinned_rows);
+  cudaMemcpyAsync(prows, slot_->proj_out, n * dm * 4, cudaMemcpyDeviceToHost, st);
   if (finish_slots(st, err) != 0) return 2;
   std::memcpy(out, prows, n * dm * 4);
   return 0;

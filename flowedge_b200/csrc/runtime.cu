@@ -11,6 +11,20 @@ namespace {
 std::atomic<std::uint64_t> g_device_mallocs{0};
 std::atomic<std::uint64_t> g_host_mallocs{0};
 
+// Allocations that fail_allocations() refuses: those from g_fail_first on, of
+// the ones still to come, g_fail_count of them.
+std::atomic<long> g_fail_first{0}, g_fail_count{0};
+
+bool refused() {
+  if (g_fail_count.load() == 0) return false;
+  if (g_fail_first.load() > 1) {
+    g_fail_first.fetch_sub(1);
+    return false;
+  }
+  g_fail_count.fetch_sub(1);
+  return true;
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -72,12 +86,19 @@ bool encode_tmap_2d(CUtensorMap* map, const void* ptr, std::uint64_t inner, std:
 std::uint64_t device_malloc_count() noexcept { return g_device_mallocs.load(); }
 std::uint64_t host_malloc_count() noexcept { return g_host_mallocs.load(); }
 
+void fail_allocations(long first, long count) noexcept {
+  g_fail_first.store(first);
+  g_fail_count.store(count);
+}
+
 cudaError_t counted_malloc(void** ptr, std::size_t bytes) {
+  if (refused()) return cudaErrorMemoryAllocation;
   g_device_mallocs.fetch_add(1);
   return cudaMalloc(ptr, bytes);
 }
 
 cudaError_t counted_host_malloc(void** ptr, std::size_t bytes) {
+  if (refused()) return cudaErrorMemoryAllocation;
   g_host_mallocs.fetch_add(1);
   return cudaMallocHost(ptr, bytes);
 }

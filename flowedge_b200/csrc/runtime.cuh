@@ -28,6 +28,9 @@ struct DeviceContext {
 // cudaMalloc / cudaFree with the allocation counter.
 cudaError_t counted_malloc(void** ptr, std::size_t bytes);
 cudaError_t counted_host_malloc(void** ptr, std::size_t bytes);
+// For tests: of the allocations to come, the first-th (from 1) and the count - 1
+// behind it fail as if there were no memory; count 0 ends that.
+void fail_allocations(long first, long count) noexcept;
 
 // One device allocation carved by a bump pointer (256-byte aligned pieces).
 class DeviceArena {

@@ -150,3 +150,5 @@ extern "C" int febtest_check_fp16_storable(const char* name, const float* w, siz
   }
   return ok ? 0 : 1;
 }
+
+extern "C" void febtest_fail_allocations(long first, long count) { feb::fail_allocations(first, count); }

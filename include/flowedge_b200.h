@@ -348,7 +348,8 @@ int fe_engine_run_device(fe_engine* engine, const int32_t* tokens, size_t batch,
  * Slots are apart from the one state of fe_engine_step.  Growth moves buffers:
  * a graph in which the caller captured one of the calls below is no longer
  * valid behind it (a prompt_batch or step_batch of more rows than there is
- * room for grows too). */
+ * room for grows too, and a growth that fails for want of memory may have moved
+ * them all the same; it changes no state and no capacity otherwise). */
 int fe_engine_reserve_slots(fe_engine* engine, size_t n_slots);
 /* Zero states for n slots. */
 int fe_engine_reset_slots(fe_engine* engine, const int32_t* slots, size_t n);

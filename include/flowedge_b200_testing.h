@@ -41,6 +41,11 @@ int febtest_conv_16(const uint16_t* x, int B, int L, int C, const uint16_t* W, c
 int febtest_check_fp16_storable(const char* name, const float* w, size_t n, int bf16_mode, char* message,
                                 size_t message_len);
 
+/* Of this process's allocations (device and pinned) to come, the `first`-th
+ * (from 1) and the `count` - 1 behind it fail as if there were no memory;
+ * `count` 0 ends that.  Host only. */
+void febtest_fail_allocations(long first, long count);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
