@@ -55,6 +55,11 @@ std::shared_ptr<DeviceContext> make_device_context(int device, std::string& err)
 int context_device(const DeviceContext& ctx) noexcept;
 // Waits for all work on the context's stream; non-zero on a device error.
 int synchronize_context(DeviceContext& ctx) noexcept;
+// A call on device buffers is about to be enqueued: its faults are still unread
+// when the next host call begins.
+void note_device_call(DeviceContext& ctx) noexcept;
+// For tests: `code` as if a kernel of such a call had left it.
+int post_device_error(DeviceContext& ctx, int code) noexcept;
 
 struct DiffusionConfig {
   std::size_t action_dim{}, horizon{}, action_steps{}, observation_steps{}, condition_dim{};

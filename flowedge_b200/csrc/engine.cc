@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../include/flowedge_b200.h"
+#include "../../include/flowedge_b200_testing.h"
 #include "device.h"
 #include "loader.h"
 
@@ -628,6 +629,7 @@ int fe_engine_sample_diffusion_device(fe_engine* engine, const float* condition,
     return 4;
   }
   std::string err;
+  feb::note_device_call(*engine->ctx);
   const int rc = engine->unet->sample_device(condition, noise, batch, steps, scheduler, seed, action, stream, err);
   if (rc != 0) set_error("Diffusion sampling failed: " + err);
   return rc;
@@ -741,6 +743,7 @@ int fe_engine_sample_condition_device(fe_engine* engine, const float* condition,
     return FE_STATUS_UNSUPPORTED_MODEL;
   }
   std::string err;
+  feb::note_device_call(*engine->ctx);
   const int rc = engine->flow->sample_device(condition, noise, batch, steps, method, action, stream, err);
   if (rc != 0) set_error("Flow sampling failed: " + err);
   return rc;
@@ -763,6 +766,7 @@ int fe_engine_sample_condition_static(fe_engine* engine, const float* condition,
     return FE_STATUS_UNSUPPORTED_MODEL;
   }
   std::string err;
+  feb::note_device_call(*engine->ctx);
   const int rc = engine->flow->sample_static(condition, noise, batch, steps, method, action, stream, err);
   if (rc != 0) set_error("Static-scratch flow sampling failed: " + err);
   return rc;
@@ -930,6 +934,7 @@ int fe_engine_run_device(fe_engine* engine, const int32_t* tokens, size_t batch,
     return FE_STATUS_UNSUPPORTED_MODEL;
   }
   std::string err;
+  feb::note_device_call(*engine->ctx);
   if (engine->mamba->forward_device(tokens, batch, seq_len, last_hidden, stream, err) != 0) {
     set_error("Mamba forward failed: " + err);
     return FE_STATUS_RESOURCE_EXHAUSTED;
@@ -1129,6 +1134,7 @@ int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t row
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_prompt_device"); rc != 0) return rc;
     std::string err;
+    feb::note_device_call(*engine->ctx);
     if (engine->mamba->prompt_device(tokens, rows, offsets, slots, fresh, n_seq, last_hidden, status, stream, err) != 0)
       return slots_failed("Mamba prompt", err);
     return FE_STATUS_OK;
@@ -1167,6 +1173,7 @@ int fe_engine_step_device(fe_engine* engine, const int32_t* tokens, const int32_
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_step_device"); rc != 0) return rc;
     std::string err;
+    feb::note_device_call(*engine->ctx);
     if (engine->mamba->step_device(tokens, slots, n, out, status, stream, err) != 0)
       return slots_failed("Mamba step", err);
     return FE_STATUS_OK;
@@ -1451,6 +1458,7 @@ int fe_engine_smolvla_sample_device(fe_engine* engine, const float* initial_nois
     return FE_STATUS_UNSUPPORTED_MODEL;
   }
   std::string err;
+  feb::note_device_call(*engine->ctx);
   const int rc = engine->smolvla->sample(initial_noise, batch, chunk_size, steps, prefix_keys, prefix_values,
                                          prefix_mask, prefix_length, shared_prefix != 0, out, true, stream, err);
   if (rc != 0) set_error(err);
@@ -1509,6 +1517,8 @@ int fe_engine_synchronize(fe_engine* engine) {
   }
   return FE_STATUS_OK;
 }
+
+int febtest_post_device_error(fe_engine* engine, int code) { return feb::post_device_error(*engine->ctx, code); }
 
 uint64_t fe_engine_kernel_launches(const fe_engine* engine) {
   if (engine == nullptr) return 0;

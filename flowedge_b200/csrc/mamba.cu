@@ -805,17 +805,13 @@ __global__ void embed_kernel(const int* tokens, long long n_tok, const float* em
 }
 
 // embed_kernel for ids that the host has not checked: a row whose id is out of
-// range becomes zeros and the fault is recorded
-__global__ void embed_checked_kernel(const int* tokens, long long n_tok, const float* emb, int dm, int vocab,
-                                     float* hidden, int* err) {
+// range is zero (gather_slots_kernel reports it, where its sequence ran)
+__global__ void embed_checked_kernel(const int* tokens, long long n_tok, const float* emb, int dm, int vocab, float* hidden) {
   const long long total = n_tok * dm;
   for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long tok = i / dm;
-    const int c = static_cast<int>(i - tok * dm), id = tokens[tok];
-    const bool ok = id >= 0 && id < vocab;
-    hidden[i] = ok ? emb[static_cast<long long>(id) * dm + c] : 0.0f;
-    if (!ok && c == 0) atomicCAS(err, 0, kErrTokenRange);
+    const int id = tokens[i / dm];
+    hidden[i] = id >= 0 && id < vocab ? emb[static_cast<long long>(id) * dm + i % dm] : 0.0f;
   }
 }
 
@@ -830,13 +826,18 @@ __global__ void act16_kernel(const float* in, long long rows, int width, __half*
 // Row offsets[s + 1] - 1 (row s without offsets) of every sequence that ran and
 // has rows -> out[s]; a CTA per sequence.  A slot outside the pool, or one that
 // an earlier sequence has, did not run (the rule of the operators on slots).
+// A token of theirs that is out of range is reported here: what rows of skipped
+// sequences and rows behind the last one hold is no fault.
 __global__ void gather_slots_kernel(const float* hidden, const int* offsets, const int* slots, int n_slots,
-                                    long long rows, int dm, float* out) {
+                                    long long rows, int dm, const int* tokens, int vocab, int* err, float* out) {
   const int q = blockIdx.x, slot = slots[q];
   const long long begin = offsets != nullptr ? offsets[q] : q, end = offsets != nullptr ? offsets[q + 1] : q + 1;
   int twice = 0;
   for (int i = threadIdx.x; i < q; i += blockDim.x) twice |= slots[i] == slot;
   if (__syncthreads_or(twice) || slot < 0 || slot >= n_slots || begin < 0 || end <= begin || end > rows) return;
+  bool bad = false;
+  for (long long i = begin + threadIdx.x; i < end; i += blockDim.x) bad |= tokens[i] < 0 || tokens[i] >= vocab;
+  if (bad) atomicCAS(err, 0, kErrTokenRange);
   for (int c = threadIdx.x; c < dm; c += blockDim.x) out[static_cast<long long>(q) * dm + c] = hidden[(end - 1) * dm + c];
 }
 
@@ -1106,6 +1107,8 @@ class Mamba final : public MambaDevice {
     slot_graphs_.clear();
   }
   int finish_slots(cudaStream_t st, std::string& err) noexcept;
+  // a fault that an earlier call on device buffers left: known before a state advances
+  int earlier_fault(cudaStream_t st, std::string& err) noexcept;
   // rows that a call over slots may have
   [[nodiscard]] std::size_t slot_rows() const noexcept { return slot_ ? std::min(slot_->rows, cap_tokens_) : 0; }
   std::unique_ptr<SlotBuffers> make_slot_buffers(std::size_t rows, std::size_t n_slots, std::string& err) noexcept;
@@ -1853,6 +1856,7 @@ int Mamba::step(std::int32_t token, float* out, std::string& err) noexcept {
   }
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
+  if (earlier_fault(st, err) != 0) return 2;
   if (step_graph_ == nullptr) {
     cudaStream_t cap = nullptr;
     cudaStreamCreateWithFlags(&cap, cudaStreamNonBlocking);
@@ -2171,7 +2175,7 @@ bool Mamba::embed_and_run(long long rows, int n_seq, const int* offsets, const i
                           std::int32_t* status, cudaStream_t st, std::string& err) {
   const int dm = static_cast<int>(cfg_.d_model);
   embed_checked_kernel<<<ew_grid(rows * dm, 256, *ctx_), 256, 0, st>>>(tokens_, rows, emb_, dm,
-                                                                      static_cast<int>(cfg_.vocab), hidden_, ctx_->d_err);
+                                                                      static_cast<int>(cfg_.vocab), hidden_);
   return run_slots(rows, n_seq, offsets, slots, fresh, status, st, err);
 }
 
@@ -2194,7 +2198,7 @@ int Mamba::prompt_device(const std::int32_t* tokens, std::size_t rows, const std
   }
   gather_slots_kernel<<<static_cast<unsigned>(n_seq), 256, 0, st>>>(
       out_, offsets, slots, static_cast<int>(n_slots_), static_cast<long long>(rows), static_cast<int>(cfg_.d_model),
-      last_hidden);
+      tokens_, static_cast<int>(cfg_.vocab), ctx_->d_err + kTokenWord, last_hidden);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 
@@ -2259,8 +2263,17 @@ int Mamba::step_device(const std::int32_t* tokens, const std::int32_t* slots, st
     }
   }
   gather_slots_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(out_, nullptr, slot_->ids, static_cast<int>(n_slots_),
-                                                               rows, static_cast<int>(cfg_.d_model), out);
+                                                               rows, static_cast<int>(cfg_.d_model), tokens_,
+                                                               static_cast<int>(cfg_.vocab), ctx_->d_err + kTokenWord,
+                                                               out);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+int Mamba::earlier_fault(cudaStream_t st, std::string& err) noexcept {
+  if (!ctx_->device_calls) return 0;
+  const int code = take_device_error(*ctx_, st);
+  if (code != 0) err = std::string("an earlier call on device buffers: ") + device_error_text(code);
+  return code == 0 ? 0 : 2;
 }
 
 int Mamba::finish_slots(cudaStream_t st, std::string& err) noexcept {
@@ -2284,6 +2297,7 @@ int Mamba::prompt(const std::int32_t* tokens, const std::size_t* lengths, const 
   if (make_room(rows, err) != 0) return 2;
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
+  if (earlier_fault(st, err) != 0) return 2;
   const std::size_t dm = cfg_.d_model;
   auto* ptok = reinterpret_cast<std::int32_t*>(slot_->pinned);
   auto* pslot = ptok + rows;
@@ -2311,6 +2325,7 @@ int Mamba::step_slots(const std::int32_t* tokens, const std::int32_t* slots, std
   if (make_room(n, err) != 0) return 2;
   cudaSetDevice(ctx_->device);
   cudaStream_t st = ctx_->stream;
+  if (earlier_fault(st, err) != 0) return 2;
   const std::size_t dm = cfg_.d_model;
   auto* ptok = reinterpret_cast<std::int32_t*>(slot_->pinned);
   std::memcpy(ptok, tokens, n * 4);

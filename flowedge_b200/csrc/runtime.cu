@@ -193,7 +193,19 @@ int context_device(const DeviceContext& ctx) noexcept { return ctx.device; }
 int synchronize_context(DeviceContext& ctx) noexcept {
   cudaSetDevice(ctx.device);
   if (cudaStreamSynchronize(ctx.stream) != cudaSuccess) return 2;
-  return take_device_error(ctx, ctx.stream) == 0 ? 0 : 2;
+  const int code = take_device_error(ctx, ctx.stream);
+  int token = 0;
+  if (cudaMemcpy(&token, ctx.d_err + kTokenWord, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return 2;
+  if (token != 0) cudaMemset(ctx.d_err + kTokenWord, 0, sizeof(int));
+  return code == 0 && token == 0 ? 0 : 2;
+}
+
+void note_device_call(DeviceContext& ctx) noexcept { ctx.device_calls = true; }
+
+int post_device_error(DeviceContext& ctx, int code) noexcept {
+  cudaSetDevice(ctx.device);
+  ctx.device_calls = true;
+  return cudaMemcpy(ctx.d_err, &code, sizeof(int), cudaMemcpyHostToDevice) == cudaSuccess ? 0 : 2;
 }
 
 const char* device_error_text(int code) noexcept {
@@ -213,6 +225,7 @@ const char* device_error_text(int code) noexcept {
 
 int take_device_error(DeviceContext& ctx, cudaStream_t stream) {
   int host = 0;
+  ctx.device_calls = false;
   if (cudaMemcpyAsync(&host, ctx.d_err, sizeof(int), cudaMemcpyDeviceToHost, stream) != cudaSuccess) return -1;
   if (cudaStreamSynchronize(stream) != cudaSuccess) return -1;
   if (host != 0) cudaMemsetAsync(ctx.d_err, 0, sizeof(int), stream);

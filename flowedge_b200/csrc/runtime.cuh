@@ -16,11 +16,16 @@
 
 namespace feb {
 
+// Word of d_err that takes kErrTokenRange: a fault of a caller's data, which
+// synchronize_context reports and no later call is charged with.
+constexpr int kTokenWord = 1;
+
 struct DeviceContext {
   int device = 0;
   cudaStream_t stream = nullptr;
   int sm_count = 0;
-  int* d_err = nullptr;  // device error word written by kernels (never trapped)
+  int* d_err = nullptr;  // device error word written by kernels (never trapped), and at kTokenWord one for tokens
+  bool device_calls = false;  // a call on device buffers was enqueued since the error word was read
   int pair_clusters = 0;  // co-resident 2-CTA clusters of the paired GroupNorm GEMM (0: unavailable)
   ~DeviceContext();
 };

@@ -365,8 +365,10 @@ int fe_engine_prompt_batch(fe_engine* engine, const int32_t* tokens, const size_
  * sequence is skipped), fresh [n_seq] (nonzero: from a zero state; NULL: all
  * continue), sequences checked as in part 3 with their bits in *status (may
  * be NULL).  Rows of last_hidden without a sequence that ran are left as they
- * were.  A token outside the vocabulary reads as a zero embedding, and
- * fe_engine_synchronize reports it.  rows must fit max_batch x max_sequence
+ * were.  A token outside the vocabulary reads as a zero embedding, and where its
+ * sequence ran fe_engine_synchronize reports it (what rows that do not run hold
+ * is no fault).  Any other fault of a call on device buffers is reported by the
+ * next call on host buffers before that changes a state.  rows must fit max_batch x max_sequence
  * and n_seq the reserved slots.  Calls of one engine share its workspace:
  * they must not overlap. */
 int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t rows, const int32_t* offsets,

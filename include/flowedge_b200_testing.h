@@ -10,6 +10,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "flowedge_b200.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -45,6 +47,10 @@ int febtest_check_fp16_storable(const char* name, const float* w, size_t n, int 
  * (from 1) and the `count` - 1 behind it fail as if there were no memory;
  * `count` 0 ends that.  Host only. */
 void febtest_fail_allocations(long first, long count);
+
+/* Leaves `code` in the engine's device error word, as a kernel of a call on
+ * device buffers does whose wait gave up. */
+int febtest_post_device_error(fe_engine* engine, int code);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
