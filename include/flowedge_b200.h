@@ -283,8 +283,12 @@ typedef struct fe_engine_options {
   uint64_t max_sequence;   /* Mamba prefill capacity in tokens (0 = 512) */
   /* 32, 64 or 128: the Mamba in / x / out projections' weights are rounded to
    * 4 bits with one scale per that many inputs (the rule of
-   * fe_w4_quantize_device); every Mamba entry point computes with them, the
-   * calls over slots of fewer than 128 rows from the packed form.  0: off.  A
+   * fe_w4_quantize_device), and every Mamba entry point computes with them.
+   * Calls over slots read the packed form for fewer than 128 rows, and for any
+   * number in projections whose inputs (d_model; d_inner) are no multiple of
+   * 64, which the tensor path does not take.  All others read the full-width
+   * copy, which a bf16 engine holds in fp16 (rounded once more) and which stays
+   * beside the packed one: the option saves time, not memory.  0: off.  A
    * structure that ends before this field (struct_size 40) reads as 0. */
   uint32_t weights4_group;
   uint32_t reserved;
