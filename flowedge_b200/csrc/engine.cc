@@ -140,6 +140,10 @@ fe_engine* create_engine(std::shared_ptr<const feb::ModelWeights> weights, const
     set_error("weights4_group must be 0, 32, 64 or 128");
     return nullptr;
   }
+  if (opt.reserved != 0) {
+    set_error("The reserved field of the engine options must be 0");
+    return nullptr;
+  }
   if (env_flag("FLOWEDGE_CUDA_FORCE_HOST")) {
     set_error("FLOWEDGE_CUDA_FORCE_HOST=1 is not supported: this library has no host kernels");
     return nullptr;

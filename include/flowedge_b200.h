@@ -289,9 +289,9 @@ typedef struct fe_engine_options {
    * 64, which the tensor path does not take.  All others read the full-width
    * copy, which a bf16 engine holds in fp16 (rounded once more) and which stays
    * beside the packed one: the option saves time, not memory.  0: off.  A
-   * structure that ends before this field (struct_size 40) reads as 0. */
+   * structure that ends before this field (struct_size 32) reads as 0. */
   uint32_t weights4_group;
-  uint32_t reserved;
+  uint32_t reserved; /* 0 (of a structure that holds it, struct_size 40) */
 } fe_engine_options;
 
 /* Load with explicit options (device, precision, batch capacity). */
