@@ -1272,6 +1272,11 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
     }
     packed_ok = launch_w4_quantize(a, nullptr) == 0 && launch_w4_dequantize(a, nullptr) == 0 &&
                 cudaMemcpy(w.data(), a.y, w.size() * 4, cudaMemcpyDeviceToHost) == cudaSuccess;
+    // 7 times a scale's rounding may pass the end of fp16, in which the tensor path holds the values
+    if (packed_ok && std::any_of(w.begin(), w.end(), [](float v) { return std::isinf(__half2float(__float2half_rn(v))); })) {
+      err = "a projection's weights rounded to 4 bits pass the fp16 range (65504)";
+      packed_ok = false;
+    }
   };
   auto put_mat = [&](std::vector<float>& w, int rows, int cols, Mat& m) {
     if (w4_group_ > 0) pack_w4(w, rows, cols, m);
