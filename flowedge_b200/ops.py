@@ -9,10 +9,11 @@ Each call checks its arguments, enqueues its kernels on the current stream of
 its tensors' device and returns; it keeps nothing.  A refused argument raises
 FlowEdgeError (status 1) before anything is launched.  These are inference
 operators: tensors that require a gradient are refused while gradients are
-being recorded.  Outputs share no element with inputs; states are updated in
-place, which autograd's record of changed tensors does not see.  With `out`
-given, rows of skipped sequences and rows behind the last sequence keep what
-they held; without it they are undefined.
+being recorded, and tensors with a forward-mode tangent.  Outputs share no
+element with inputs; states are updated in place, which autograd's record of
+changed tensors does not see.  With `out` given, rows of skipped sequences and
+rows behind the last sequence keep what they held; without it they are
+undefined.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ from __future__ import annotations
 import struct
 
 import torch
+import torch.autograd.forward_ad as _forward
 from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from .engine import FlowEdgeError, load_library
@@ -63,6 +65,13 @@ def _explain(t, name: str, shape, dtype, device: int):
         _refuse(f"{name} requires a gradient: this operator has none")
     if t.layout != torch.strided or t.shape != shape:
         _refuse(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+
+
+def _no_tangents(**tensors):
+    """Refuses dual tensors (called inside a dual level alone: there are none outside)."""
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None:
+            _refuse(f"{name} has a forward-mode tangent: this operator has none")
 
 
 def _matrix(t, name: str, shape: tuple, dtype, device: int) -> int:
@@ -146,6 +155,8 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     float32, d_conv 1 to 8.  `window` [slots, d_inner, d_conv] float32 holds each slot's last inputs, newest last; a
     sequence reads the inputs before its first row there and leaves its own last ones.  Returns u like x.
     """
+    if _forward._current_level >= 0:
+        _no_tangents(x=x, weight=weight, bias=bias, window=window, out=out)
     shape, dtype, device = _first(x, "x")
     rows, di = shape
     x_ld = _matrix(x, "x", shape, dtype, device)
@@ -178,6 +189,8 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     dt_w [dt_rank, d_inner] and dt_b [d_inner] float32, d_state 1 to 32, dt_rank 1 to 512.  `state` [slots, d_state,
     d_inner] float32.  Returns y like u.
     """
+    if _forward._current_level >= 0:
+        _no_tangents(u=u, proj=proj, a=a, d=d, dt_w=dt_w, dt_b=dt_b, z=z, state=state, out=out)
     shape, dtype, device = _first(u, "u")
     rows, di = shape
     u_ld = _matrix(u, "u", shape, dtype, device)
@@ -234,6 +247,8 @@ def w4_quantize(weight, group: int = 64, *, layout: str = "blocks") -> tuple:
     groups of 32 and 64 read blocks faster); scales [m, ceil(k / group)].  Its type tells the other calls which layout a
     packed weight has.
     """
+    if _forward._current_level >= 0:
+        _no_tangents(weight=weight)
     shape, dtype, device = _first(weight, "weight")
     m, k = shape
     ld = _matrix(weight, "weight", shape, dtype, device)
@@ -264,6 +279,8 @@ def _w4_weight(packed, scales, k: int, group: int, device: int) -> int:
 
 def w4_dequantize(packed, scales, k: int, *, group: int = 64, dtype=torch.float32):
     """The matrix [m, k] that a packed weight of either layout stands for, rounded to `dtype`."""
+    if _forward._current_level >= 0:
+        _no_tangents(scales=scales)
     if dtype not in _DTYPES:
         _refuse("dtype is float32, bfloat16 or float16")
     if not isinstance(packed, torch.Tensor) or not packed.is_cuda:
@@ -285,6 +302,8 @@ def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
     float32, bfloat16 or float16 x and result; sums in float32, the weight exact.  packed is uint8 with its words in the
     order of their elements, or int8 in blocks (w4_quantize).
     """
+    if _forward._current_level >= 0:
+        _no_tangents(x=x, scales=scales, out=out)
     shape, dtype, device = _first(x, "x")
     rows, k = shape
     x_ld = _matrix(x, "x", shape, dtype, device)
@@ -308,6 +327,8 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
     float32 or the same; weights [dim] float32, dim 1 to 16384.  Without post_weight x is added as it is.  The returned
     norm is taken before the residual is rounded to its type.
     """
+    if _forward._current_level >= 0:
+        _no_tangents(x=x, residual=residual, weight=weight, post_weight=post_weight, gate=gate, out=out)
     shape, dtype, device = _first(x, "x")
     rows, dim = shape
     x_ld = _matrix(x, "x", shape, dtype, device)
