@@ -10,10 +10,11 @@ its tensors' device and returns; it keeps nothing.  A refused argument raises
 FlowEdgeError (status 1) before anything is launched.  These are inference
 operators: tensors that require a gradient are refused while gradients are
 being recorded, and tensors with a forward-mode tangent.  Outputs share no
-element with inputs; states are updated in place, which autograd's record of
-changed tensors does not see.  With `out` given, rows of skipped sequences and
-rows behind the last sequence keep what they held; without it they are
-undefined.
+element with inputs; states, the residual and a given `out` are changed in
+place, which their version counters show (a tensor that autograd saved for a
+backward pass and that is changed is found out there).  With `out` given, rows
+of skipped sequences and rows behind the last sequence keep what they held;
+without it they are undefined.
 """
 
 from __future__ import annotations
@@ -144,6 +145,16 @@ def _pool(state, name: str, inner: tuple, device: int) -> tuple:
     return n_slots, outer if n_slots > 1 or outer > per else per
 
 
+def _changed(*tensors):
+    """Raises the version counters of tensors that a call has written (inference tensors have none)."""
+    try:
+        torch._C._increment_version(tensors)
+    except RuntimeError:
+        for t in tensors:
+            if not t.is_inference():
+                torch._C._increment_version((t,))
+
+
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -167,8 +178,11 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     _flat(bias, "bias", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
     n_slots, stride = (0, 0) if window is None else _pool(window, "window", (di, dc), device)
+    written = () if window is None else (window,)
     if out is None:
         out = torch.empty_like(x)
+    else:
+        written += (out,)
     u_ld = _matrix(out, "out", shape, dtype, device)
     args = _CONV.pack(_CONV.size, device, _DTYPES[dtype], dc, rows, di, n_seq, n_slots, x_ld, u_ld, stride,
                       x.data_ptr(), weight.data_ptr(), bias.data_ptr(), out.data_ptr(), _ptr(window), _ptr(offsets),
@@ -176,6 +190,8 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     rc = load_library().fe_causal_conv_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
+    if written:
+        _changed(*written)
     return out
 
 
@@ -205,8 +221,11 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     _flat(dt_b, "dt_b", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
     n_slots, stride = (0, 0) if state is None else _pool(state, "state", (ds, di), device)
+    written = () if state is None else (state,)
     if out is None:
         out = torch.empty_like(u)
+    else:
+        written += (out,)
     y_ld = _matrix(out, "out", shape, dtype, device)
     lib = load_library()
     workspace, size = 0, 0
@@ -225,6 +244,8 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     rc = lib.fe_selective_scan_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
+    if written:
+        _changed(*written)
     return out
 
 
@@ -308,15 +329,18 @@ def w4_matvec(x, packed, scales, *, group: int = 64, out=None):
     rows, k = shape
     x_ld = _matrix(x, "x", shape, dtype, device)
     m = _w4_weight(packed, scales, k, group, device)
-    if out is None:
-        out, y_ld = x.new_empty((rows, m)), m
-    else:
+    given = out is not None
+    if given:
         y_ld = _matrix(out, "out", (rows, m), dtype, device)
+    else:
+        out, y_ld = x.new_empty((rows, m)), m
     args = _W4.pack(_W4_SIZE, device, _DTYPES[dtype], group, rows, m, k, x_ld, y_ld, x.data_ptr(), packed.data_ptr(),
                     scales.data_ptr(), out.data_ptr()) + _W4_LAYOUT[packed.dtype]
     rc = load_library().fe_w4_matvec_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
+    if given:
+        _changed(out)
     return out
 
 
@@ -342,8 +366,11 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
         one = isinstance(gate, torch.Tensor) and gate.dim() == 2 and gate.shape[0] == 1
         gate_ld = _matrix(gate, "gate", (1, dim) if one else shape, dtype, device)
         gate_ld = 0 if one else gate_ld
+    written = (residual,)
     if out is None:
         out = torch.empty_like(x)
+    else:
+        written += (out,)
     y_ld = _matrix(out, "out", shape, dtype, device)
     try:
         args = _NORM.pack(_NORM.size, device, _DTYPES[dtype], _DTYPES[r_dtype], rows, dim, x_ld, r_ld, gate_ld, y_ld,
@@ -354,4 +381,5 @@ def residual_norm(x, residual, weight, *, post_weight=None, gate=None, scale: fl
     rc = load_library().fe_residual_norm_device(args, _raw_stream(device))
     if rc:
         _failed(rc)
+    _changed(*written)
     return out

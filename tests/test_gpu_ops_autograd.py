@@ -39,3 +39,24 @@ def test_a_forward_mode_tangent_is_refused():
                 with pytest.raises(ops.FlowEdgeError, match="tangent"):
                     call(tensors | {name: dual})
             call(tensors)
+
+
+CHANGED = [("window", "out"), ("state", "out"), ("residual", "out"), ("out",), (), ()]
+
+
+def test_tensors_changed_in_place_show_it():
+    for (call, tensors), changed in zip(_calls(), CHANGED):
+        before = {name: t._version for name, t in tensors.items()}
+        call(tensors)
+        assert {name for name, t in tensors.items() if t._version != before[name]} == set(changed)
+        with torch.inference_mode():  # tensors made here have no counter
+            call({name: t.clone() if i % 2 else t for i, (name, t) in enumerate(tensors.items())})
+
+
+def test_a_saved_tensor_that_was_changed_is_found_out():
+    call, tensors = next(c for c in _calls() if "residual" in c[1])
+    scale = torch.ones(6, 64, device="cuda", requires_grad=True)
+    product = scale * tensors["residual"]  # saves the residual
+    call(tensors)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
