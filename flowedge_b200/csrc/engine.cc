@@ -24,6 +24,7 @@
 #include "../../include/flowedge_b200_testing.h"
 #include "device.h"
 #include "loader.h"
+#include "ops.h"
 
 static_assert(sizeof(fe_model_digest) == 16);
 static_assert(sizeof(fe_model_metadata) == 96);
@@ -1052,6 +1053,13 @@ int check_slot_list(const fe_engine* engine, const std::int32_t* slots, std::siz
 
 constexpr std::size_t kMaxSlotRows = std::size_t(1) << 30;
 
+// Sequences of one call (the bound of the operators on slots).
+int check_sequence_count(std::size_t n) {
+  if (n <= feb::kMaxSlotSequences) return FE_STATUS_OK;
+  set_error("A call over slots has at most 2^16 sequences");
+  return FE_STATUS_INVALID_ARGUMENT;
+}
+
 int slots_failed(const char* what, const std::string& err) {
   set_error(std::string(what) + " failed: " + err);
   return FE_STATUS_RESOURCE_EXHAUSTED;
@@ -1107,6 +1115,7 @@ int fe_engine_prompt_batch(fe_engine* engine, const int32_t* tokens, const size_
   }
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_prompt_batch"); rc != 0) return rc;
+    if (int rc = check_sequence_count(n_seq); rc != 0) return rc;
     if (int rc = check_slot_list(engine, slots, n_seq); rc != 0) return rc;
     std::size_t rows = 0;
     for (std::size_t s = 0; s < n_seq; ++s) {
@@ -1137,6 +1146,7 @@ int fe_engine_prompt_device(fe_engine* engine, const int32_t* tokens, size_t row
   }
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_prompt_device"); rc != 0) return rc;
+    if (int rc = check_sequence_count(n_seq); rc != 0) return rc;
     std::string err;
     feb::note_device_call(*engine->ctx);
     if (engine->mamba->prompt_device(tokens, rows, offsets, slots, fresh, n_seq, last_hidden, status, stream, err) != 0)
@@ -1156,6 +1166,7 @@ int fe_engine_step_batch(fe_engine* engine, const int32_t* tokens, const int32_t
   }
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_step_batch"); rc != 0) return rc;
+    if (int rc = check_sequence_count(n); rc != 0) return rc;
     if (int rc = check_slot_list(engine, slots, n); rc != 0) return rc;
     if (const int rc = check_tokens(engine, tokens, n); rc != 0) return rc;
     std::string err;
@@ -1176,6 +1187,7 @@ int fe_engine_step_device(fe_engine* engine, const int32_t* tokens, const int32_
   }
   try {
     if (int rc = check_slots_engine(engine, "fe_engine_step_device"); rc != 0) return rc;
+    if (int rc = check_sequence_count(n); rc != 0) return rc;
     std::string err;
     feb::note_device_call(*engine->ctx);
     if (engine->mamba->step_device(tokens, slots, n, out, status, stream, err) != 0)

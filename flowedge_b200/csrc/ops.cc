@@ -86,6 +86,7 @@ void check_sequences(Checks& c, const Args& a, const float* state, std::uint64_t
   if (state != nullptr) {
     c.need(a.n_slots >= 1, "a state needs n_slots");
     c.need(a.slots != nullptr || a.n_slots >= a.n_seq, "without slots n_slots is at least n_seq");
+    c.need(a.slots == nullptr || a.n_seq <= feb::kMaxSlotSequences, "a call with slots has at most 2^16 sequences");
     c.need(a.slot_stride >= static_cast<std::int64_t>(per_slot) && a.slot_stride <= (std::int64_t(1) << 40),
            "slot_stride is at least one slot's state");
   }

@@ -13,6 +13,12 @@
 
 namespace feb {
 
+// Sequences of a call with states in slots: every CTA searches the slots before
+// its own for the same one, which is a small part of the call up to some 8192
+// and grows with the square (131072 prompts of one row x 256: scan 42 ms, 4
+// without slots).
+constexpr std::uint64_t kMaxSlotSequences = 1 << 16;
+
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept;
 
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept;

@@ -84,7 +84,7 @@ __device__ __forceinline__ Seq resolve(const SeqParams& q, int s) {
 }
 
 // The last test before anything is written: a sequence whose slot an earlier
-// one of the call has is skipped.  Every thread of the CTA calls it; `report`
+// one of the call has is skipped (kMaxSlotSequences bounds the search).  Every thread of the CTA calls it; `report`
 // writes the sequence's faults to the status.
 __device__ __forceinline__ bool writes(const SeqParams& q, int s, Seq& r, bool report) {
   if (q.stateful && q.slots != nullptr && r.slot >= 0) {

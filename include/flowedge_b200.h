@@ -349,7 +349,8 @@ int fe_engine_run_device(fe_engine* engine, const int32_t* tokens, size_t batch,
  * fe_engine_reserve_slots makes room for slots 0 .. n_slots - 1 (zero states;
  * a larger pool keeps the states of a smaller one) and, together with
  * fe_engine_reserve_batch and max_batch x max_sequence, is what allocates.
- * Slots are apart from the one state of fe_engine_step.  Growth moves buffers:
+ * Slots are apart from the one state of fe_engine_step.  A call takes at most
+ * 2^16 sequences.  Growth moves buffers:
  * a graph in which the caller captured one of the calls below is no longer
  * valid behind it (a prompt_batch or step_batch of more rows than there is
  * room for grows too, and a growth that fails for want of memory may have moved
@@ -446,6 +447,10 @@ uint64_t fe_engine_kernel_launches(const fe_engine* engine);
  * sequence with fresh[s] != 0 starts from a zero state whatever its slot
  * holds.  A state pointer of NULL means: every sequence starts from zero and
  * no state is kept.
+ *
+ * A call with states and slots has at most 2^16 sequences (each looks for its
+ * slot among those before it, so the cost grows with their square: up to some
+ * 8192 it is a small part of the call).
  *
  * Offsets and slots are read on the device.  A sequence whose offsets lie
  * outside the rows, whose slot is n_slots or more, or whose slot an earlier
