@@ -130,7 +130,7 @@ def _sequences(rows: int, offsets, slots, fresh, status, device: int) -> int:
     return n_seq
 
 
-def _pool(state, name: str, inner: tuple, device: int) -> tuple:
+def _pool(state, name: str, inner: tuple, n_seq: int, device: int) -> tuple:
     """Checks a pool of slot states and returns (slots, distance of two slots)."""
     if not isinstance(state, torch.Tensor) or state.dim() != 3:
         _refuse(f"{name} is a tensor of shape {('slots',) + inner}")
@@ -141,6 +141,8 @@ def _pool(state, name: str, inner: tuple, device: int) -> tuple:
     outer, mid, last = state.stride()
     if (mid != inner[1] and inner[0] > 1) or (last != 1 and inner[1] > 1):
         _refuse(f"{name} has slots that are not contiguous")
+    if n_slots == 0 and n_seq > 0:  # (an empty tensor has no address: the call would run without states)
+        _refuse(f"{name} has no slots")
     per = inner[0] * inner[1]
     return n_slots, outer if n_slots > 1 or outer > per else per
 
@@ -177,7 +179,7 @@ def conv(x, weight, bias, *, window=None, offsets=None, slots=None, fresh=None, 
     _flat(weight, "weight", (di, dc), torch.float32, device)
     _flat(bias, "bias", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
-    n_slots, stride = (0, 0) if window is None else _pool(window, "window", (di, dc), device)
+    n_slots, stride = (0, 0) if window is None else _pool(window, "window", (di, dc), n_seq, device)
     written = () if window is None else (window,)
     if out is None:
         out = torch.empty_like(x)
@@ -220,7 +222,7 @@ def scan(u, proj, a, d, dt_w, dt_b, *, z=None, state=None, offsets=None, slots=N
     _flat(dt_w, "dt_w", (dr, di), torch.float32, device)
     _flat(dt_b, "dt_b", (di,), torch.float32, device)
     n_seq = _sequences(rows, offsets, slots, fresh, status, device)
-    n_slots, stride = (0, 0) if state is None else _pool(state, "state", (ds, di), device)
+    n_slots, stride = (0, 0) if state is None else _pool(state, "state", (ds, di), n_seq, device)
     written = () if state is None else (state,)
     if out is None:
         out = torch.empty_like(u)
