@@ -21,6 +21,9 @@ constexpr std::uint64_t kMaxSlotSequences = 1 << 16;
 
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept;
 
+// Rows that a tile of prompts has, for tests, with `across` CTAs over the channels.
+int causal_conv_chunk(std::size_t rows, std::size_t n_seq, std::size_t across) noexcept;
+
 std::size_t selective_scan_workspace(const fe_scan_args& a) noexcept;
 // At least selective_scan_workspace() of any call of up to `rows` rows and
 // `n_seq` sequences on the current device.

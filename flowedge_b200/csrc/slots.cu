@@ -318,6 +318,15 @@ __global__ void __launch_bounds__(128, 5) conv_prompt_kernel(const ConvParams p)
   }
 }
 
+// Rows of a conv tile: as few as let every tile be resident at once (five CTAs
+// to an SM; half of the sequences' last tiles are extra), from 8 to 64.
+// `across` CTAs go over the channels.  Measured at 96 prompts of 12289 rows x
+// 1024: 16 rows 25.0 us, 24 23.8, 40 (this rule) 21.1, 64 25.8
+int conv_chunk(long long rows, long long n_seq, long long across) {
+  const long long resident = std::max(1LL, 5LL * current_sm_count() / across - n_seq / 2);
+  return static_cast<int>(std::clamp((rows / resident + 7) / 8 * 8, 8LL, 64LL));
+}
+
 template <typename T, int DC>
 int conv_prompts(ConvParams p, cudaStream_t st) {
   // 16 bytes of a row to a thread where its rows allow it (at most four
@@ -331,12 +340,7 @@ int conv_prompts(ConvParams p, cudaStream_t st) {
   const int threads = wide ? p.di / kVec : p.di;  // for a row
   const unsigned block = static_cast<unsigned>(std::min(128, (threads + 31) / 32 * 32));
   const long long across = (threads + block - 1) / block;
-  // rows to a tile: as few as let every tile be resident at once (five CTAs to
-  // an SM; half of the sequences' last tiles are extra), from 8 to 64.
-  // Measured at 96 prompts of 12289 rows x 1024: 16 rows 25.0 us, 24 23.8,
-  // 40 (this rule) 21.1, 64 25.8
-  const long long resident = std::max(1LL, 5LL * current_sm_count() / across - p.q.n_seq / 2);
-  p.chunk = static_cast<int>(std::clamp((p.q.rows / resident + 7) / 8 * 8, 8LL, 64LL));
+  p.chunk = conv_chunk(p.q.rows, p.q.n_seq, across);
   const dim3 grid(static_cast<unsigned>(p.q.rows / p.chunk + p.q.n_seq), static_cast<unsigned>(across));
   if (wide)
     conv_prompt_kernel<T, DC, kVec><<<grid, block, 0, st>>>(p);
@@ -1126,6 +1130,10 @@ int current_sm_count() noexcept {
     counts[device].store(v, std::memory_order_relaxed);
   }
   return v;
+}
+
+int causal_conv_chunk(std::size_t rows, std::size_t n_seq, std::size_t across) noexcept {
+  return conv_chunk(static_cast<long long>(rows), static_cast<long long>(n_seq), static_cast<long long>(across));
 }
 
 int launch_causal_conv(const fe_conv_args& a, void* stream) noexcept {

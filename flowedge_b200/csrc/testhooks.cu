@@ -5,6 +5,7 @@
 #include <vector>
 
 #include "../../include/flowedge_b200_testing.h"
+#include "ops.h"
 #include "runtime.cuh"
 
 namespace {
@@ -152,3 +153,7 @@ extern "C" int febtest_check_fp16_storable(const char* name, const float* w, siz
 }
 
 extern "C" void febtest_fail_allocations(long first, long count) { feb::fail_allocations(first, count); }
+
+extern "C" int febtest_conv_chunk(size_t rows, size_t n_seq, size_t across) {
+  return feb::causal_conv_chunk(rows, n_seq, across);
+}

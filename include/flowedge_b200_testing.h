@@ -48,6 +48,10 @@ int febtest_check_fp16_storable(const char* name, const float* w, size_t n, int 
  * `count` 0 ends that.  Host only. */
 void febtest_fail_allocations(long first, long count);
 
+/* Rows of a tile in fe_causal_conv_device's form of prompts, on the current
+ * device, where `across` blocks go over the channels. */
+int febtest_conv_chunk(size_t rows, size_t n_seq, size_t across);
+
 /* Leaves `code` in the engine's device error word, as a kernel of a call on
  * device buffers does whose wait gave up. */
 int febtest_post_device_error(fe_engine* engine, int code);
