@@ -1008,7 +1008,10 @@ __global__ void __launch_bounds__(kCarryThreads) scan_carry_kernel(const ScanPar
 #pragma unroll
       for (int i = 0; i < kCarryStates; ++i) {
         if (n0 + i < p.ds) ws[j * step + static_cast<long long>(1 + n0 + i) * p.di] = h[i];
-        h[i] = fmaf(ex2_approx(dt[j] * an[i]), h[i], e[j][i]);
+        // (a tile's decay may be below float32's range though no row's is: an
+        // infinite state stays infinite)
+        const float x = dt[j] * an[i], decay = ex2_approx(x);
+        h[i] = fmaf(x > -INFINITY ? max_nan(decay, 1.4e-45f) : decay, h[i], e[j][i]);
       }
     }
     ws += kCarryAhead * step;

@@ -155,3 +155,21 @@ def test_scan_decays_to_nothing(form, n, di):
     case["a"][:, 5] = -1e30
     case["state"][:, :, 5] = 3e38
     _check_scan(case, offsets)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ds", [8, 16])
+def test_an_infinite_state_stays_infinite_over_tiles(dtype, ds):
+    """Tiles of 16 rows whose decay is below float32's range, while every row's is above it: the state behind an infinite
+    input is infinite in prompts as it is in single tokens."""
+    lengths, di = [75, 16, 40], 130
+    case = _scan_case(7, sum(lengths), di, ds, 4, dtype, 3)
+    case["a"] = -(torch.rand(ds, di, generator=torch.Generator().manual_seed(1)) * 6 + 2).cuda()
+    case["dt_w"] *= 0.1
+    case["dt_b"] = torch.full((di,), 5.0, device="cuda")  # sums of 16 steps near 80, decays e^-160 to e^-640
+    case["proj"][:, 4:] = case["proj"][:, 4:].abs() + 0.25
+    case["u"], case["d"], case["state"] = case["u"].abs(), case["d"].abs() + 0.1, case["state"].abs()
+    case["u"][3, ::3] = INF
+    case["u"][95, 1] = INF
+    case["state"][1, 0, 5] = INF
+    _check_scan(case, _offsets(lengths))
