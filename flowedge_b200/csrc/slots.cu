@@ -454,7 +454,7 @@ cudaError_t allow_smem(K kernel, int bytes) {
 // whose product is above 2^-25 of the whole, smallest first.  Terms of an
 // infinity or of a value that bf16 rounds to one do not add up to it (infinity
 // times terms of two signs, or of zero, is NaN): a sum that is not finite is
-// made again from the operands.  16384 x 2048, dt rank 64, bf16: 73 us, 21 of
+// made again from the operands.  16384 x 2048, dt rank 64, bf16: 74 us, 21 of
 // them the bytes of dt.
 template <typename T>
 constexpr int kDtTerms = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;
@@ -776,8 +776,8 @@ constexpr int kPolyPairs = DS / 16;
 // B and C sit in shared memory (every channel reads them), the next kStage
 // rows' are requested before the arithmetic; dt, u and z are requested kTok
 // rows ahead.  All arithmetic on pairs (FFMA2): states two and two.  16384 rows
-// x 2048, 16 states, bf16: the main pass adds 188 us to the call, the summaries
-// 143.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469
+// x 2048, 16 states, bf16: the main pass adds 191 us to the call, the summaries
+// 140.  Four CTAs on an SM: three 466 us for the whole scan, four 420, five 469
 // (with two state pairs on the FMA pipe in the summaries).  DS is d_state
 // rounded up to a multiple of four; PADDED: the last states do not exist and
 // stay out of y, as for single tokens.
