@@ -32,3 +32,15 @@ def test_a_pool_without_slots_is_refused(name, form):
     assert _call(name, 4, None, None, slots=slots, offsets=offsets).shape == (4, 32)  # without states
     none = torch.zeros(1, dtype=torch.int32, device="cuda")
     assert _call(name, 0, *empty, offsets=none if form == "prompts" else None).shape == (0, 32)
+
+
+def test_prompts_that_are_all_empty():
+    """No rows at all: a fresh sequence's slot becomes zero, another's stays."""
+    offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
+    slots = torch.tensor([2, 0, -1], dtype=torch.int32, device="cuda")
+    fresh = torch.tensor([1, 0, 1], dtype=torch.uint8, device="cuda")
+    for name, pool in (("conv", torch.ones(3, 32, 4, device="cuda")), ("scan", torch.ones(3, 8, 32, device="cuda"))):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = _call(name, 0, pool, pool, offsets=offsets, slots=slots, fresh=fresh, status=status)
+        assert out.shape == (0, 32) and int(status) == 0
+        assert (pool[:2] == 1).all() and (pool[2] == 0).all()
