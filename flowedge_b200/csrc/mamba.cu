@@ -1206,6 +1206,7 @@ bool Mamba::load(const TensorTable& t, std::string& err) {
     err = "no Mamba layers";
     return false;
   }
+  kept_state_.reserve(state_floats());  // (reserve(), which may not throw, fills it)
   const bool bf = prec_ == Precision::kBF16;
   auto mat_bytes = [&](std::size_t rows, std::size_t cols) {
     const std::size_t rp = (rows + 127) / 128 * 128, cp = (cols + 63) / 64 * 64;
